@@ -330,6 +330,31 @@ VF4_API int vf4_gptq_block(const float* w, int64_t ldw, const float* hinv, int64
                            int64_t ldb, const float* global_scale, int64_t N, int64_t col0, int64_t count,
                            uint8_t* codes, int64_t ldc, float* err, int64_t lde, vf4_stream_t stream);
 
+/* FP8 block format: E4M3 codes (one byte each) with one fp32 scale per 128 consecutive columns of a row
+ * (activations, block_rows = 1) or per 128 x 128 block (weights, block_rows = 128):
+ *   amax' = max(amax |x| over the block, 1e-12),  scale = RN(amax' / 448),  code = e4m3(RN(448 x / amax'))
+ * (nearest even; decode: code * scale).  x: (M, K) rows of stride ld elements, VF4_BF16 or VF4_F32, any
+ * K and alignment (16-byte aligned rows with K % 8 == 0 take vector loads).  codes: rows of ldc bytes, 16-byte
+ * aligned, ldc % 16 == 0, ldc >= K (columns K .. K rounded up to 8 are written as 0); scale: element
+ * (row block, column block) at row_block * stride_m + column_block * stride_k.  A block that holds a NaN
+ * becomes NaN; an infinite element becomes a NaN and its block's finite ones 0.  No counterpart in the
+ * reference (its per-row E4M3 round trip is fp8.py:6-17). */
+VF4_API int vf4_cast_fp8_block(const void* x, int dtype, int64_t M, int64_t K, int64_t ld, int block_rows,
+                               uint8_t* codes, int64_t ldc, float* scale, int64_t stride_m, int64_t stride_k,
+                               vf4_stream_t stream);
+
+/* Product of two operands of the FP8 block format on tcgen05 tensor cores (kind::f8f6f4, fp32 accumulation
+ * per block of 128 columns, the blocks' scales applied in fp32):
+ *   out[m, n] = sum_g as[m, g] bs[n / 128, g] sum_{k in block g} a[m, k] b[n, k]  (+ bias[n])
+ * a: (M, K) codes, rows lda bytes apart, scale (m, g) at m * as_m + g * as_k; b: (N, K) codes, rows ldb bytes
+ * apart, scale (n / 128, g) at (n / 128) * bs_n + g * bs_k; code rows 16-byte aligned (lda, ldb % 16 == 0).  bias
+ * (N,) VF4_BF16 or VF4_F32 or NULL; out (M, N), rows ldo elements apart, VF4_BF16 (one rounding of the fp32
+ * sum) or VF4_F32.  Any M, N and K (bytes past K in a row are not used).  Deterministic; no workspace. */
+VF4_API int vf4_gemm_fp8_block(const uint8_t* a, int64_t lda, const float* a_scale, int64_t as_m, int64_t as_k,
+                               const uint8_t* b, int64_t ldb, const float* b_scale, int64_t bs_n, int64_t bs_k,
+                               int64_t M, int64_t N, int64_t K, const void* bias, int bias_dtype, void* out,
+                               int64_t ldo, int out_dtype, vf4_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

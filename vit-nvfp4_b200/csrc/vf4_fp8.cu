@@ -1,0 +1,606 @@
+// FP8 block format (E4M3 codes, one fp32 scale per 128 columns or per 128 x 128 block): the cast and
+// the product
+//
+//   y[m, n] = sum_g sa[m, g] sb[n / 128, g] sum_{k in block g} a[m, k] b[n, k]  (+ bias[n])
+//
+// No counterpart in the reference, whose formats are bf16 and NVFP4; the framework's layers that stay
+// out of NVFP4 (heads, first and last blocks, projections of a cross attention) take this one.
+#include <string.h>
+
+#include "vf4_fp8_block.cuh"
+#include "vf4_host.h"
+
+namespace vf4 {
+
+static __device__ int g_fp8_err;
+
+int fp8_device_error(int clear) {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, g_fp8_err, sizeof(int));
+  if (clear) {
+    int z = 0;
+    cudaMemcpyToSymbol(g_fp8_err, &z, sizeof(int));
+  }
+  return v;
+}
+
+// ---------------------------------------------------------------------------------------
+// Cast of activations: 16 lanes hold the 128 columns of one block, 8 each (one 16-byte load of bf16).
+// The blocks of all rows are numbered in one sequence, row by row, and dealt to the half-warps, so
+// short and long rows fill the machine alike.  Bound by memory: 1 byte out per 2 (bf16) or 4 (fp32)
+// bytes in; kU blocks per half-warp are loaded before the first is reduced, to keep enough bytes in
+// flight.
+// ---------------------------------------------------------------------------------------
+template <typename T, bool kVec, int kU>
+__global__ void __launch_bounds__(256) fp8_cast_rows_kernel(const T* __restrict__ x, int64_t M, int K, int64_t ld,
+                                                            uint8_t* __restrict__ codes, int64_t ldc,
+                                                            float* __restrict__ scale, int64_t s_m, int64_t s_k) {
+  const int kb = (K + 127) >> 7;
+  const int64_t blocks = M * kb;
+  const int l = threadIdx.x & 15;
+  const int64_t hw = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 4;
+  const int64_t n_hw = ((int64_t)gridDim.x * blockDim.x) >> 4;
+  // the trip count is the same for both halves of a warp (the shuffles below name all its lanes)
+  for (int64_t b0 = hw & ~int64_t(1); b0 < blocks; b0 += n_hw * kU) {
+    float v[kU][8];
+    int64_t row[kU];
+    int g[kU], nv[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int64_t b = b0 + (hw & 1) + u * n_hw;
+      row[u] = b / kb;
+      g[u] = (int)(b - row[u] * kb);
+      const int col = g[u] * 128 + l * 8;
+      nv[u] = b < blocks ? min(8, K - col) : 0;
+      load8<T, kVec>(x + row[u] * ld + col, nv[u], v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      uint32_t m = amax8_bits(v[u]);
+#pragma unroll
+      for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+      const Fp8Block q = fp8_block(m);
+      if (nv[u] > 0) {   // columns of the row's padding (ldc >= K rounded up to 16) are written as 0
+        *reinterpret_cast<uint2*>(codes + row[u] * ldc + g[u] * 128 + l * 8) = fp8_encode8(v[u], q);
+        if (l == 0) scale[row[u] * s_m + g[u] * s_k] = q.scale;
+      }
+    }
+  }
+}
+
+// Cast of weights: one CTA per 128 x 128 block, every thread 8 columns of 8 rows.  Runs once per weight.
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(256) fp8_cast_tile_kernel(const T* __restrict__ x, int64_t M, int K, int64_t ld,
+                                                            uint8_t* __restrict__ codes, int64_t ldc,
+                                                            float* __restrict__ scale, int64_t s_m, int64_t s_k) {
+  __shared__ uint32_t red[8];
+  const int kb = (K + 127) >> 7;
+  const int64_t mb = blockIdx.x / kb;
+  const int g = (int)(blockIdx.x - mb * kb);
+  const int l = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+  const int col = g * 128 + l * 8;
+  const int nc = min(8, K - col);
+  float v[8][8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = mb * 128 + r0 + 16 * i;
+    load8<T, kVec>(x + row * ld + col, row < M ? nc : 0, v[i]);
+    m = max(m, amax8_bits(v[i]));
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, red[i]);
+  const Fp8Block q = fp8_block(m);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = mb * 128 + r0 + 16 * i;
+    if (row < M && nc > 0) *reinterpret_cast<uint2*>(codes + row * ldc + col) = fp8_encode8(v[i], q);
+  }
+  if (threadIdx.x == 0) scale[mb * s_m + g * s_k] = q.scale;
+}
+
+// ---------------------------------------------------------------------------------------
+// The product.  One K block of 128 columns is four tcgen05 MMAs (kind::f8f6f4, K = 32) into an
+// accumulator of its own in tensor memory; the epilogue warps read it, multiply it by the block's
+// scales and add it to the running fp32 sums in their registers, while the tensor cores fill the next
+// accumulator.  The scales are arbitrary fp32 numbers, so they cannot go through the MMA (its
+// hardware scales are powers of two or E4M3).
+//
+//   warp 0      TMA: 128 rows of A and BN rows of B, 128 bytes of K each, 128-byte swizzle
+//   warp 1      TMEM allocation, MMAs
+//   warps 2..   epilogue: each TMEM lane quadrant's rows, NC of the BN columns per warp
+//
+// Two roles of the operands:
+//   kSwap = false  A = activations, B = weight.  A row's scale is per thread, the weight's per 128
+//                  columns: one multiplication per thread and block.
+//   kSwap = true   A = weight, B = activations, for up to 64 rows of activations: BN is 16, 32 or 64
+//                  instead of padding the activations to 128 rows; y^T comes out, a lane per n.
+//
+// Few tiles: a cluster of `split` CTAs shares one tile, each taking a run of K blocks, and adds its
+// sums up through distributed shared memory, in the order of the ranks (no atomics, no workspace: the
+// result does not depend on timing).
+// ---------------------------------------------------------------------------------------
+template <int BN, bool kSwap>
+struct F8Cfg {
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+  static constexpr int ACCS = BN == 256 ? 2 : 4;
+  static constexpr int TMEM_COLS = ACCS * BN;            // 64 .. 512, a power of two
+  static constexpr int EW = BN >= 128 ? 2 : 1;           // epilogue warps per lane quadrant
+  static constexpr int NC = BN / EW;                     // columns per epilogue warp
+  static constexpr int EPI_WARPS = 4 * EW;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int BAR_OFF = STAGES * STAGE_BYTES;
+  static constexpr int SMEM = 1024 + BAR_OFF + 8 * (2 * STAGES + 2 * ACCS) + 16;
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+  static_assert(BN * 128 * 4 <= STAGES * STAGE_BYTES, "the split sums reuse the stages");
+};
+
+struct F8Params {
+  const float* sa;     // activation scales: element (m, g) at m * sa_m + g * sa_k
+  const float* sb;     // weight scales: element (n / 128, g) at (n / 128) * sb_n + g * sb_k
+  int64_t sa_m, sa_k, sb_n, sb_k;
+  int M, N, kb;
+  int tiles_r, tiles_c, split;   // tiles of 128 (A rows) and of BN (B rows)
+  const void* bias;
+  int bias_f32;
+  void* out;
+  int64_t ldo;
+  int out_vec;         // rows of out may be written 16 bytes at a time
+};
+
+VF4_DEV float bias_at(const F8Params& p, int n) {
+  if (!p.bias || n >= p.N) return 0.f;
+  return p.bias_f32 ? __ldg(static_cast<const float*>(p.bias) + n)
+                    : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n]);
+}
+
+// Eight sums of one row of y, columns n0 .. n0 + 7: + bias, one rounding to the output type.
+template <bool kF32>
+VF4_DEV void store8(const F8Params& p, int64_t m, int n0, const float* y) {
+  if (m >= p.M || n0 >= p.N) return;
+  float z[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = y[i] + bias_at(p, n0 + i);
+  if constexpr (kF32) {
+    float* o = static_cast<float*>(p.out) + m * p.ldo + n0;
+    if (p.out_vec && n0 + 8 <= p.N) {
+      reinterpret_cast<float4*>(o)[0] = make_float4(z[0], z[1], z[2], z[3]);
+      reinterpret_cast<float4*>(o)[1] = make_float4(z[4], z[5], z[6], z[7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n0 + i < p.N) o[i] = z[i];
+    }
+  } else {
+    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + m * p.ldo + n0;
+    if (p.out_vec && n0 + 8 <= p.N) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = bf16x2_round(f32x2_pack(z[2 * i], z[2 * i + 1]));
+      *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n0 + i < p.N) o[i] = __float2bfloat16_rn(z[i]);
+    }
+  }
+}
+
+template <bool kF32>
+VF4_DEV void store1(const F8Params& p, int m, int n, float y) {
+  if (m >= p.M || n >= p.N) return;
+  y += bias_at(p, n);
+  if constexpr (kF32) static_cast<float*>(p.out)[(int64_t)m * p.ldo + n] = y;
+  else static_cast<__nv_bfloat16*>(p.out)[(int64_t)m * p.ldo + n] = __float2bfloat16_rn(y);
+}
+
+VF4_DEV float ld_shared_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int BN, bool kSwap, bool kF32>
+__global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
+    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const F8Params p) {
+  using C = F8Cfg<BN, kSwap>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw0 = smem_u32(smem_raw);
+  const uint32_t base = (raw0 + 1023u) & ~1023u;
+  uint8_t* gb = smem_raw + (base - raw0);
+  const uint32_t bar = base + C::BAR_OFF;
+  auto full = [&](int i) { return bar + 8u * i; };
+  auto empty = [&](int i) { return bar + 8u * (C::STAGES + i); };
+  auto tfull = [&](int i) { return bar + 8u * (2 * C::STAGES + i); };
+  auto tempty = [&](int i) { return bar + 8u * (2 * C::STAGES + C::ACCS + i); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + C::BAR_OFF + 8 * (2 * C::STAGES + 2 * C::ACCS));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* err = &g_fp8_err;
+
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(full(i), 1);
+      mbar_init(empty(i), 1);
+    }
+    for (int i = 0; i < C::ACCS; ++i) {
+      mbar_init(tfull(i), 1);
+      mbar_init(tempty(i), C::EPI_WARPS);
+    }
+    fence_mbar_init();
+    tma_prefetch(&tmA);
+    tma_prefetch(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  fence_async_shared();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+
+  // this CTA's run of K blocks, and its tiles (split > 1: one per cluster)
+  const int rank = p.split > 1 ? (int)cluster_ctarank() : 0;
+  const int k0 = (int)((int64_t)p.kb * rank / p.split), k1 = (int)((int64_t)p.kb * (rank + 1) / p.split);
+  const int tiles = p.tiles_r * p.tiles_c;
+  const int first = blockIdx.x / p.split, step = gridDim.x / p.split;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += step) {
+        const int tr = tile / p.tiles_c, tc = tile - tr * p.tiles_c;
+        for (int kb = k0; kb < k1; ++kb, ++it) {
+          const int s = it % C::STAGES;
+          if (it >= C::STAGES && !mbar_wait(empty(s), (uint32_t)(it / C::STAGES - 1) & 1u, err, kDevErrTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(full(s), C::STAGE_BYTES);
+          const uint32_t st = base + s * C::STAGE_BYTES;
+          tma_load_2d(st, &tmA, kb * 128, tr * 128, full(s));
+          tma_load_2d(st + C::A_BYTES, &tmB, kb * 128, tc * BN, full(s));
+        }
+      }
+      // no copy may still be writing shared memory when the CTA exits
+      for (int i = it > C::STAGES ? it - C::STAGES : 0; i < it; ++i)
+        mbar_wait(full(i % C::STAGES), (uint32_t)(i / C::STAGES) & 1u, err, kDevErrTimeoutFull);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      constexpr uint32_t idesc = idesc_f8_e4m3(BN);
+      for (int tile = first; tile < tiles && ok; tile += step) {
+        for (int kb = k0; kb < k1; ++kb, ++it) {
+          const int s = it % C::STAGES, a = it % C::ACCS;
+          if (!mbar_wait(full(s), (uint32_t)(it / C::STAGES) & 1u, err, kDevErrTimeoutFull) ||
+              (it >= C::ACCS && !mbar_wait(tempty(a), (uint32_t)(it / C::ACCS - 1) & 1u, err, kDevErrTimeoutTmem))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t st = base + s * C::STAGE_BYTES;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f8f6f4(tmem + a * BN, smem_desc(st + 32u * kk, 16, 1024, 2),
+                       smem_desc(st + C::A_BYTES + 32u * kk, 16, 1024, 2), idesc, kk > 0 ? 1u : 0u);
+          tc_commit(empty(s));
+          tc_commit(tfull(a));
+        }
+      }
+      // the tensor core must be done with shared and tensor memory before the CTA leaves
+      if (it > 0) mbar_wait(tfull((it - 1) % C::ACCS), (uint32_t)((it - 1) / C::ACCS) & 1u, err, kDevErrTimeoutDrain);
+    }
+    __syncwarp();
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    const int r = quad * 32 + lane;                       // row of the tile, lane of tensor memory
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * C::NC);
+    int it = 0;
+    bool ok = true;
+    for (int tile = first; tile < tiles; tile += step) {
+      const int tr = tile / p.tiles_c, tc = tile - tr * p.tiles_c;
+      const int row = tr * 128 + r, col0 = tc * BN + half * C::NC;
+      // scale pointers: the thread's own row, or (kSwap) one activation row per lane
+      const float* s_own;
+      int64_t step_own;
+      const float* s_blk;
+      int64_t step_blk = p.sb_k;
+      bool have;
+      if constexpr (!kSwap) {
+        have = row < p.M;
+        s_own = p.sa + (int64_t)(have ? row : 0) * p.sa_m;
+        step_own = p.sa_k;
+        s_blk = p.sb + (int64_t)min(col0, p.N - 1) / 128 * p.sb_n;
+      } else {
+        have = lane < C::NC && col0 + lane < p.M;
+        s_own = p.sa + (int64_t)(have ? col0 + lane : 0) * p.sa_m;
+        step_own = p.sa_k;
+        s_blk = p.sb + (int64_t)tr * p.sb_n;
+      }
+      // kSwap with 64 columns: a second activation row per lane
+      const bool have2 = kSwap && C::NC > 32 && col0 + 32 + lane < p.M;
+      const int64_t off2 = 32 * p.sa_m;
+      auto scales = [&](int kb, float& s0, float& s1) {
+        const float w = __ldg(s_blk + kb * step_blk);
+        s0 = have ? __ldg(s_own + kb * step_own) * w : 0.f;
+        s1 = have2 ? __ldg(s_own + off2 + kb * step_own) * w : 0.f;
+      };
+      unsigned long long acc[C::NC / 2];
+#pragma unroll
+      for (int i = 0; i < C::NC / 2; ++i) acc[i] = 0ull;
+      float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
+      if (k0 < k1) scales(k0, s0, s1);
+      for (int kb = k0; kb < k1; ++kb, ++it) {
+        if (kb + 1 < k1) scales(kb + 1, t0, t1);
+        const int a = it % C::ACCS;
+        if (!__all_sync(0xFFFFFFFFu, ok && mbar_wait(tfull(a), (uint32_t)(it / C::ACCS) & 1u, err, kDevErrTimeoutTmem)))
+          ok = false;   // the whole warp gives up together: the loads below are warp-wide
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t v[2][16];
+        tmem_ld_32x32b_x16(lane_base + a * BN, v[0]);
+#pragma unroll
+        for (int c = 0; c < C::NC / 16; ++c) {
+          tmem_wait_ld();
+          reg_fence16(v[c & 1]);
+          if (c + 1 < C::NC / 16) {
+            tmem_ld_32x32b_x16(lane_base + a * BN + 16 * (c + 1), v[(c + 1) & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(tempty(a));
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            unsigned long long s2;
+            if constexpr (!kSwap) {
+              s2 = f32x2_pack(s0, s0);
+            } else {
+              const float u = c < 2 ? s0 : s1;
+              s2 = f32x2_pack(__shfl_sync(0xFFFFFFFFu, u, (16 * c + 2 * i) & 31),
+                              __shfl_sync(0xFFFFFFFFu, u, (16 * c + 2 * i + 1) & 31));
+            }
+            acc[8 * c + i] = fma_f32x2(f32x2_pack(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])),
+                                       s2, acc[8 * c + i]);
+          }
+        }
+        s0 = t0;
+        s1 = t1;
+      }
+      if (p.split == 1) {
+        float y[8];
+#pragma unroll
+        for (int c = 0; c < C::NC / 8; ++c) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f32x2_unpack(acc[4 * c + i], &y[2 * i], &y[2 * i + 1]);
+          if constexpr (!kSwap) {
+            store8<kF32>(p, row, col0 + 8 * c, y);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) store1<kF32>(p, col0 + 8 * c + i, row, y[i]);
+          }
+        }
+      } else {
+        // this CTA's sums, column by column, into the stages (every MMA that read them is done)
+        float* red = reinterpret_cast<float*>(gb) + (half * C::NC) * 128 + r;
+#pragma unroll
+        for (int i = 0; i < C::NC / 2; ++i) {
+          float y0, y1;
+          f32x2_unpack(acc[i], &y0, &y1);
+          red[(2 * i) * 128] = y0;
+          red[(2 * i + 1) * 128] = y1;
+        }
+      }
+    }
+  }
+
+  if (p.split > 1) {
+    __syncwarp();
+    cluster_sync_all();
+    // rank's share of the columns, summed over the ranks in their order
+    if (warp >= 2 && first < tiles) {
+      const int tr = first / p.tiles_c, tc = first - tr * p.tiles_c;
+      const int quad = warp & 3, half = (warp - 2) >> 2, r = quad * 32 + lane;
+      const int per = BN / 8 / p.split > 0 ? BN / 8 / p.split : 1;   // runs of 8 columns
+      if constexpr (!kSwap) {
+        for (int c = rank * per + half; c < (rank + 1) * per; c += C::EW) {
+          float y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = 0.f;
+          for (int q = 0; q < p.split; ++q) {
+            const uint32_t src = mapa_shared(base, (uint32_t)q) + (uint32_t)((8 * c) * 128 + r) * 4u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] += ld_shared_cluster(src + (uint32_t)i * 512u);
+          }
+          store8<kF32>(p, tr * 128 + r, tc * BN + 8 * c, y);
+        }
+      } else {
+        const int cols = BN / p.split;
+        for (int c = rank * cols + half; c < (rank + 1) * cols; c += C::EW) {
+          float y = 0.f;
+          for (int q = 0; q < p.split; ++q)
+            y += ld_shared_cluster(mapa_shared(base, (uint32_t)q) + (uint32_t)(c * 128 + r) * 4u);
+          store1<kF32>(p, tc * BN + c, tr * 128 + r, y);
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();   // no CTA leaves while another reads its shared memory
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, C::TMEM_COLS);
+}
+
+static int make_code_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t K, int64_t ld, int box_rows) {
+  EncodeTiledFn enc = encode_tiled();
+  if (!enc) return fail(VF4_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+  cuuint32_t es[2] = {1u, 1u};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, es,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(VF4_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return VF4_OK;
+}
+
+struct F8Operand {
+  const uint8_t* ptr;
+  int64_t rows, ld;
+};
+
+template <int BN, bool kSwap, bool kF32>
+static int launch_fp8_gemm(F8Operand a, F8Operand b, int64_t K, F8Params p, cudaStream_t s) {
+  using C = F8Cfg<BN, kSwap>;
+  CUtensorMap ta, tb;
+  if (int st = make_code_map(&ta, a.ptr, a.rows, K, a.ld, 128)) return st;
+  if (int st = make_code_map(&tb, b.ptr, b.rows, K, b.ld, BN)) return st;
+  auto kern = fp8_gemm_kernel<BN, kSwap, kF32>;
+  if (int st = smem_optin(kern, C::SMEM)) return st;
+  p.tiles_r = (int)((a.rows + 127) / 128);
+  p.tiles_c = (int)((b.rows + BN - 1) / BN);
+  const int tiles = p.tiles_r * p.tiles_c, sms = num_sms();
+  // share a tile among up to 8 CTAs (the portable cluster size) while that leaves no SM two of them
+  p.split = 1;
+  while (p.split < 8 && tiles * p.split * 2 <= sms && p.split * 2 <= p.kb) p.split *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.split > 1 ? tiles * p.split : (tiles < sms ? tiles : sms)));
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)p.split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.split > 1 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kern, ta, tb, p) != cudaSuccess) return launch_status("vf4_gemm_fp8_block");
+  return launch_status("vf4_gemm_fp8_block");
+}
+
+template <bool kF32>
+static int dispatch_fp8_gemm(F8Operand x, F8Operand w, int64_t K, const F8Params& p, cudaStream_t s) {
+  if (x.rows <= 16) return launch_fp8_gemm<16, true, kF32>(w, x, K, p, s);
+  if (x.rows <= 32) return launch_fp8_gemm<32, true, kF32>(w, x, K, p, s);
+  if (x.rows <= 64) return launch_fp8_gemm<64, true, kF32>(w, x, K, p, s);
+  const int64_t big = (x.rows + 127) / 128 * ((w.rows + 255) / 256);
+  if (big >= num_sms()) return launch_fp8_gemm<256, false, kF32>(x, w, K, p, s);
+  return launch_fp8_gemm<128, false, kF32>(x, w, K, p, s);
+}
+
+}  // namespace vf4
+
+using namespace vf4;
+
+extern "C" {
+
+int vf4_cast_fp8_block(const void* x, int dtype, int64_t M, int64_t K, int64_t ld, int block_rows, uint8_t* codes,
+                       int64_t ldc, float* scale, int64_t stride_m, int64_t stride_k, vf4_stream_t stream) {
+  if (int st = check_device()) return st;
+  if (M < 0 || K <= 0 || ld < K || (block_rows != 1 && block_rows != 128))
+    return fail(VF4_ERR_ARG, "vf4_cast_fp8_block: bad sizes (M=%lld K=%lld ld=%lld block_rows=%d)", (long long)M,
+                (long long)K, (long long)ld, block_rows);
+  if (dtype != VF4_BF16 && dtype != VF4_F32) return fail(VF4_ERR_ARG, "vf4_cast_fp8_block: bad dtype %d", dtype);
+  if (K > (1 << 20) || M > INT32_MAX) return fail(VF4_ERR_UNSUPPORTED, "vf4_cast_fp8_block: sizes too large");
+  if (M == 0) return VF4_OK;
+  if (!x || !codes || !scale) return fail(VF4_ERR_ARG, "vf4_cast_fp8_block: null pointer");
+  if (!aligned16(codes) || ldc % 16 || ldc < K)
+    return fail(VF4_ERR_ALIGN, "vf4_cast_fp8_block: code rows need 16-byte aligned starts of at least K bytes (ldc=%lld)",
+                (long long)ldc);
+  const int esz = dtype == VF4_BF16 ? 2 : 4;
+  if (reinterpret_cast<uintptr_t>(x) % esz) return fail(VF4_ERR_ALIGN, "vf4_cast_fp8_block: x is misaligned for its type");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const bool vec = aligned16(x) && K % 8 == 0 && ld * esz % 16 == 0;
+  const int64_t kb = (K + 127) / 128;
+  const auto* xb = static_cast<const __nv_bfloat16*>(x);
+  const auto* xf = static_cast<const float*>(x);
+  if (block_rows == 1) {
+    const int64_t want = (M * kb + 15) / 16;   // 16 blocks per CTA and step
+    const int64_t most = (int64_t)num_sms() * 8;
+    const unsigned grid = (unsigned)(want < most ? want : most);
+    const int K32 = (int)K;
+#define VF4_CAST_ROWS(T, X, V) \
+  fp8_cast_rows_kernel<T, V, 4><<<grid, 256, 0, s>>>(X, M, K32, ld, codes, ldc, scale, stride_m, stride_k)
+    if (dtype == VF4_BF16) {
+      if (vec) VF4_CAST_ROWS(__nv_bfloat16, xb, true);
+      else VF4_CAST_ROWS(__nv_bfloat16, xb, false);
+    } else {
+      if (vec) VF4_CAST_ROWS(float, xf, true);
+      else VF4_CAST_ROWS(float, xf, false);
+    }
+#undef VF4_CAST_ROWS
+  } else {
+    const int64_t tiles = (M + 127) / 128 * kb;
+    if (tiles > INT32_MAX) return fail(VF4_ERR_UNSUPPORTED, "vf4_cast_fp8_block: sizes too large");
+    const unsigned grid = (unsigned)tiles;
+    const int K32 = (int)K;
+#define VF4_CAST_TILE(T, X, V) \
+  fp8_cast_tile_kernel<T, V><<<grid, 256, 0, s>>>(X, M, K32, ld, codes, ldc, scale, stride_m, stride_k)
+    if (dtype == VF4_BF16) {
+      if (vec) VF4_CAST_TILE(__nv_bfloat16, xb, true);
+      else VF4_CAST_TILE(__nv_bfloat16, xb, false);
+    } else {
+      if (vec) VF4_CAST_TILE(float, xf, true);
+      else VF4_CAST_TILE(float, xf, false);
+    }
+#undef VF4_CAST_TILE
+  }
+  return launch_status("vf4_cast_fp8_block");
+}
+
+int vf4_gemm_fp8_block(const uint8_t* a, int64_t lda, const float* a_scale, int64_t as_m, int64_t as_k,
+                       const uint8_t* b, int64_t ldb, const float* b_scale, int64_t bs_n, int64_t bs_k, int64_t M,
+                       int64_t N, int64_t K, const void* bias, int bias_dtype, void* out, int64_t ldo, int out_dtype,
+                       vf4_stream_t stream) {
+  if (int st = check_device()) return st;
+  if (M < 0 || N <= 0 || K <= 0 || ldo < N)
+    return fail(VF4_ERR_ARG, "vf4_gemm_fp8_block: bad sizes M=%lld N=%lld K=%lld ldo=%lld", (long long)M, (long long)N,
+                (long long)K, (long long)ldo);
+  if (M > (1 << 30) || N > (1 << 24) || K > (1 << 20) || (M + 127) / 128 * ((N + 127) / 128) > INT32_MAX)
+    return fail(VF4_ERR_UNSUPPORTED, "vf4_gemm_fp8_block: sizes too large");
+  if ((out_dtype != VF4_BF16 && out_dtype != VF4_F32) || (bias && bias_dtype != VF4_BF16 && bias_dtype != VF4_F32))
+    return fail(VF4_ERR_ARG, "vf4_gemm_fp8_block: bad dtype");
+  if (M == 0) return VF4_OK;
+  if (!a || !b || !a_scale || !b_scale || !out) return fail(VF4_ERR_ARG, "vf4_gemm_fp8_block: null operand");
+  if (!aligned16(a) || !aligned16(b) || lda % 16 || ldb % 16 || lda < K || ldb < K)
+    return fail(VF4_ERR_ALIGN, "vf4_gemm_fp8_block: code rows need 16-byte aligned starts of at least K bytes "
+                "(lda=%lld ldb=%lld)", (long long)lda, (long long)ldb);
+  const int esz = out_dtype == VF4_BF16 ? 2 : 4;
+  if (reinterpret_cast<uintptr_t>(out) % esz || reinterpret_cast<uintptr_t>(a_scale) % 4 ||
+      reinterpret_cast<uintptr_t>(b_scale) % 4 || (bias && reinterpret_cast<uintptr_t>(bias) % (bias_dtype == VF4_BF16 ? 2 : 4)))
+    return fail(VF4_ERR_ALIGN, "vf4_gemm_fp8_block: out, scales or bias misaligned for their types");
+  F8Params p{};
+  p.sa = a_scale;
+  p.sb = b_scale;
+  p.sa_m = as_m;
+  p.sa_k = as_k;
+  p.sb_n = bs_n;
+  p.sb_k = bs_k;
+  p.M = (int)M;
+  p.N = (int)N;
+  p.kb = (int)((K + 127) / 128);
+  p.bias = bias;
+  p.bias_f32 = bias_dtype == VF4_F32;
+  p.out = out;
+  p.ldo = ldo;
+  p.out_vec = aligned16(out) && ldo * esz % 16 == 0;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const F8Operand x{a, M, lda}, w{b, N, ldb};
+  return out_dtype == VF4_F32 ? dispatch_fp8_gemm<true>(x, w, K, p, s) : dispatch_fp8_gemm<false>(x, w, K, p, s);
+}
+
+}  // extern "C"

@@ -130,7 +130,8 @@ int vf4_device_error(int clear) {
   int a = vf4::cast_device_error(clear);
   int b = vf4::gemm_device_error(clear);
   int c = vf4::attn_device_error(clear);
-  return a ? a : (b ? b : c);
+  int d = vf4::fp8_device_error(clear);
+  return a ? a : (b ? b : (c ? c : d));
 }
 
 }  // extern "C"

@@ -8,6 +8,7 @@ from .pack import pack_e2m1, unpack_e2m1, pad_to_block, as_float4_x2, to_blocked
 from .gemm import (nvfp4_gemm, nvfp4_linear, register_backend, available_backends, gemm_packed,
                    cast_nvfp4, linear_packed)
 from .fp8 import fp8_e4m3_quant_dequant
+from .fp8_block import quantize_to_fp8_block, dequantize_fp8_block, fp8_block_gemm, fp8_block_linear
 from .attention import quant_sdpa
 
 __all__ = [
@@ -16,4 +17,5 @@ __all__ = [
     "nvfp4_gemm", "nvfp4_linear", "register_backend", "available_backends", "gemm_packed",
     "cast_nvfp4", "linear_packed",
     "fp8_e4m3_quant_dequant", "quant_sdpa",
+    "quantize_to_fp8_block", "dequantize_fp8_block", "fp8_block_gemm", "fp8_block_linear",
 ]

@@ -215,6 +215,97 @@ def gptq_block(w: torch.Tensor, hinv: torch.Tensor, block_scale: torch.Tensor, g
     _launched()
 
 
+def _on_device_of(*ts: torch.Tensor | None):
+    """All tensors on one CUDA device (else an error); a context that makes it the current one, so the
+    launch and the stream it goes to are that device's."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            _need_cuda(t)
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise _lib.VitFp4Error(f"tensors on two devices: {dev} and {t.device}")
+    return _same_device if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+class _SameDevice:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        return None
+
+
+_same_device = _SameDevice()
+
+
+def _rows_2d(x: torch.Tensor) -> torch.Tensor:
+    """(M, K) view of (..., K) with unit column stride and non-overlapping rows (copies only if needed)."""
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1 and x2.shape[1] > 1 or x2.stride(0) < x2.shape[1] and x2.shape[0] > 1:
+        x2 = x2.contiguous()
+    return x2
+
+
+def _ld(x2: torch.Tensor) -> int:
+    """Row stride of a 2-D tensor, as the kernels take it (a single row may carry any stride)."""
+    return x2.stride(0) if x2.shape[0] > 1 else max(x2.stride(0), x2.shape[1])
+
+
+def cast_fp8_block(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
+    """FP8 block cast of (M, K) bf16 / fp32 rows: codes float8_e4m3fn (M, K), in rows padded to 16 bytes,
+    and fp32 scales (ceil(M / block_rows), ceil(K / 128)); block_rows is 1 (activations) or 128 (weights).
+    The activation scales are stored column block by column block, the order the product reads them in."""
+    with _on_device_of(x):
+        code = _dtype_code(x)
+        x2 = _rows_2d(x)
+        M, K = x2.shape
+        if K < 1:
+            raise _lib.VitFp4Error("the FP8 block cast needs at least one column")
+        ldc, kb = (K + 15) // 16 * 16, (K + 127) // 128
+        codes = torch.empty((M, ldc), dtype=torch.float8_e4m3fn, device=x.device)
+        if block_rows == 1:
+            scale = torch.empty((kb, M), dtype=torch.float32, device=x.device)
+            s_m, s_k, scale = 1, M, scale.t()
+        else:
+            scale = torch.empty(((M + block_rows - 1) // block_rows, kb), dtype=torch.float32, device=x.device)
+            s_m, s_k = kb, 1
+        with _Timed(f"cast_fp8_block_{M}x{K}", M * K * (x2.element_size() + 1) + scale.numel() * 4):
+            _lib.call("vf4_cast_fp8_block", x2.data_ptr(), code, M, K, _ld(x2), block_rows, codes.data_ptr(), ldc,
+                      scale.data_ptr(), s_m, s_k, _stream())
+        _launched()
+    return (codes if ldc == K else codes[:, :K]), scale
+
+
+def _code_rows(t: torch.Tensor) -> torch.Tensor:
+    """(rows, K) E4M3 codes whose rows start on 16-byte boundaries, as the tensor copies need them."""
+    if t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    rows, K = t.shape
+    buf = torch.empty((rows, (K + 15) // 16 * 16), dtype=torch.uint8, device=t.device)
+    buf[:, :K] = t.view(torch.uint8)
+    return buf[:, :K].view(torch.float8_e4m3fn)
+
+
+def gemm_fp8_block(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+                   bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """(M, K) x (N, K) FP8 block operands -> (M, N) bf16 or fp32 (+ bias)."""
+    with _on_device_of(a, a_scale, b, b_scale, bias):
+        a, b = _code_rows(a), _code_rows(b)
+        (M, K), N = a.shape, b.shape[0]
+        out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+        with _Timed(f"gemm_fp8_block_{M}x{N}x{K}", 2.0 * M * N * K):
+            _lib.call("vf4_gemm_fp8_block", a.data_ptr(), _ld(a), a_scale.data_ptr(), a_scale.stride(0),
+                      a_scale.stride(1), b.data_ptr(), _ld(b), b_scale.data_ptr(), b_scale.stride(0),
+                      b_scale.stride(1), M, N, K, _ptr(bias), 0 if bias is None else _dtype_code(bias),
+                      out.data_ptr(), N, _dtype_code(out), _stream())
+        _launched()
+    return out
+
+
 def to_blocked(sf: torch.Tensor) -> torch.Tensor:
     """(R, C) E4M3 scales (uint8 or float8_e4m3fn) -> flat 128x4-tiled uint8."""
     _need_cuda(sf)
