@@ -32,37 +32,45 @@ int fp8_device_error(int clear) {
 // flight.
 // ---------------------------------------------------------------------------------------
 template <typename T, bool kVec, int kU>
-__global__ void __launch_bounds__(256) fp8_cast_rows_kernel(const T* __restrict__ x, int64_t M, int K, int64_t ld,
-                                                            uint8_t* __restrict__ codes, int64_t ldc,
-                                                            float* __restrict__ scale, int64_t s_m, int64_t s_k) {
+__global__ void __launch_bounds__(256, 4) fp8_cast_rows_kernel(const T* __restrict__ x, int64_t M, int K, int64_t ld,
+                                                               uint8_t* __restrict__ codes, int64_t ldc,
+                                                               float* __restrict__ scale, int64_t s_m, int64_t s_k) {
   const int kb = (K + 127) >> 7;
-  const int64_t blocks = M * kb;
   const int l = threadIdx.x & 15;
-  const int64_t hw = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 4;
-  const int64_t n_hw = ((int64_t)gridDim.x * blockDim.x) >> 4;
-  // the trip count is the same for both halves of a warp (the shuffles below name all its lanes)
-  for (int64_t b0 = hw & ~int64_t(1); b0 < blocks; b0 += n_hw * kU) {
-    float v[kU][8];
-    int64_t row[kU];
-    int g[kU], nv[kU];
+  const int hw = (blockIdx.x * blockDim.x + threadIdx.x) >> 4, n_hw = (gridDim.x * blockDim.x) >> 4;
+  // (row, column block) of this half-warp's next block; a step of n_hw blocks is (d_row, d_g) with a carry,
+  // so no division runs per block.  Both halves of a warp take as many steps (the shuffles name all lanes).
+  const int d_row = n_hw / kb, d_g = n_hw - d_row * kb;
+  int row = hw / kb, g = hw - row * kb;
+  const int64_t steps = (M * kb - (hw & ~1) + n_hw - 1) / n_hw;
+  for (int64_t i = 0; i < steps; i += kU) {
+    Raw8<T, kVec> v[kU];
+    int at_row[kU], at_g[kU], nv[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int64_t b = b0 + (hw & 1) + u * n_hw;
-      row[u] = b / kb;
-      g[u] = (int)(b - row[u] * kb);
-      const int col = g[u] * 128 + l * 8;
-      nv[u] = b < blocks ? min(8, K - col) : 0;
-      load8<T, kVec>(x + row[u] * ld + col, nv[u], v[u]);
+      at_row[u] = row;
+      at_g[u] = g;
+      const int col = g * 128 + l * 8;
+      nv[u] = row < M ? min(8, K - col) : 0;
+      v[u].load(x + row * ld + col, nv[u]);
+      row += d_row;
+      g += d_g;
+      if (g >= kb) {
+        g -= kb;
+        ++row;
+      }
     }
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      uint32_t m = amax8_bits(v[u]);
+      uint32_t m = v[u].amax_bits();
 #pragma unroll
       for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
       const Fp8Block q = fp8_block(m);
       if (nv[u] > 0) {   // columns of the row's padding (ldc >= K rounded up to 16) are written as 0
-        *reinterpret_cast<uint2*>(codes + row[u] * ldc + g[u] * 128 + l * 8) = fp8_encode8(v[u], q);
-        if (l == 0) scale[row[u] * s_m + g[u] * s_k] = q.scale;
+        float f[8];
+        v[u].get(f);
+        *reinterpret_cast<uint2*>(codes + at_row[u] * ldc + at_g[u] * 128 + l * 8) = fp8_encode8(f, q);
+        if (l == 0) scale[at_row[u] * s_m + at_g[u] * s_k] = q.scale;
       }
     }
   }
@@ -112,7 +120,8 @@ __global__ void __launch_bounds__(256) fp8_cast_tile_kernel(const T* __restrict_
 //
 //   warp 0      TMA: 128 rows of A and BN rows of B, 128 bytes of K each, 128-byte swizzle
 //   warp 1      TMEM allocation, MMAs
-//   warps 2..   epilogue: each TMEM lane quadrant's rows, NC of the BN columns per warp
+//   warps 2..   epilogue (4.. with the 256-column tile): each TMEM lane quadrant's rows, NC of the BN
+//               columns per warp
 //
 // Two roles of the operands:
 //   kSwap = false  A = activations, B = weight.  A row's scale is per thread, the weight's per 128
@@ -133,8 +142,19 @@ struct F8Cfg {
   static constexpr int EW = BN >= 128 ? 2 : 1;           // epilogue warps per lane quadrant
   static constexpr int NC = BN / EW;                     // columns per epilogue warp
   static constexpr int EPI_WARPS = 4 * EW;
-  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int BAR_OFF = STAGES * STAGE_BYTES;
+  // columns per TMEM load, two loads' registers per thread: the next load is in flight while one is
+  // multiplied in (tcgen05.ld takes about 100 clocks whatever its width, so wide ones)
+  static constexpr int CH = NC >= 64 ? 32 : 16;
+  // the 256-column tile needs 128 sums + 64 loaded values per thread: its epilogue warps take registers
+  // over from the four warps of the control group (2 of them idle)
+  static constexpr bool kRegs = BN == 256;
+  static constexpr int EPI0 = kRegs ? 4 : 2;             // first epilogue warp
+  static constexpr int THREADS = 32 * (EPI0 + EPI_WARPS);
+  static constexpr int kLaunchRegs = 168, kControlRegs = 40, kEpiRegs = 232;   // 384 threads: 168 at launch
+  static_assert(!kRegs || 128 * kControlRegs + 256 * kEpiRegs <= THREADS * kLaunchRegs, "register split");
+  static constexpr int STG_OFF = STAGES * STAGE_BYTES;   // bf16 output staging, 32 rows x 64 columns per warp
+  static constexpr int STG_BYTES = kSwap ? 0 : EPI_WARPS * 4096;
+  static constexpr int BAR_OFF = STG_OFF + STG_BYTES;
   static constexpr int SMEM = 1024 + BAR_OFF + 8 * (2 * STAGES + 2 * ACCS) + 16;
   static_assert(SMEM <= 227 * 1024, "shared memory");
   static_assert(BN * 128 * 4 <= STAGES * STAGE_BYTES, "the split sums reuse the stages");
@@ -147,10 +167,11 @@ struct F8Params {
   int M, N, kb;
   int tiles_r, tiles_c, split;   // tiles of 128 (A rows) and of BN (B rows)
   const void* bias;
-  int bias_f32;
+  int bias_f32, bias_vec;   // its type; whether 8 values may be loaded at once
   void* out;
   int64_t ldo;
   int out_vec;         // rows of out may be written 16 bytes at a time
+  int out_tma;         // bf16 rows are staged in shared memory and written by TMA (tmO)
 };
 
 VF4_DEV float bias_at(const F8Params& p, int n) {
@@ -159,13 +180,21 @@ VF4_DEV float bias_at(const F8Params& p, int n) {
                     : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n]);
 }
 
-// Eight sums of one row of y, columns n0 .. n0 + 7: + bias, one rounding to the output type.
-template <bool kF32>
-VF4_DEV void store8(const F8Params& p, int64_t m, int n0, const float* y) {
-  if (m >= p.M || n0 >= p.N) return;
-  float z[8];
+// The bias of columns n0 .. n0 + 7 (0 past N).
+VF4_DEV void bias8(const F8Params& p, int n0, float* y) {
+  if (p.bias_vec && n0 + 8 <= p.N) {
+    if (p.bias_f32) load8<float, true>(static_cast<const float*>(p.bias) + n0, 8, y);
+    else load8<__nv_bfloat16, true>(static_cast<const __nv_bfloat16*>(p.bias) + n0, 8, y);
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) z[i] = y[i] + bias_at(p, n0 + i);
+    for (int i = 0; i < 8; ++i) y[i] = bias_at(p, n0 + i);
+  }
+}
+
+// Eight sums of one row of y, columns n0 .. n0 + 7, with one rounding to the output type.
+template <bool kF32>
+VF4_DEV void store8(const F8Params& p, int64_t m, int n0, const float* z) {
+  if (m >= p.M || n0 >= p.N) return;
   if constexpr (kF32) {
     float* o = static_cast<float*>(p.out) + m * p.ldo + n0;
     if (p.out_vec && n0 + 8 <= p.N) {
@@ -208,7 +237,7 @@ VF4_DEV float ld_shared_cluster(uint32_t addr) {
 template <int BN, bool kSwap, bool kF32>
 __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                    const F8Params p) {
+                    const __grid_constant__ CUtensorMap tmO, const F8Params p) {
   using C = F8Cfg<BN, kSwap>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw0 = smem_u32(smem_raw);
@@ -235,6 +264,7 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
     fence_mbar_init();
     tma_prefetch(&tmA);
     tma_prefetch(&tmB);
+    if (p.out_tma) tma_prefetch(&tmO);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
@@ -252,58 +282,62 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
   const int tiles = p.tiles_r * p.tiles_c;
   const int first = blockIdx.x / p.split, step = gridDim.x / p.split;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      int it = 0;
-      bool ok = true;
-      for (int tile = first; tile < tiles && ok; tile += step) {
-        const int tr = tile / p.tiles_c, tc = tile - tr * p.tiles_c;
-        for (int kb = k0; kb < k1; ++kb, ++it) {
-          const int s = it % C::STAGES;
-          if (it >= C::STAGES && !mbar_wait(empty(s), (uint32_t)(it / C::STAGES - 1) & 1u, err, kDevErrTimeoutEmpty)) {
-            ok = false;
-            break;
+  if (warp < C::EPI0) {
+    if constexpr (C::kRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kControlRegs));
+    if (warp == 0) {
+      if (lane == 0) {
+        int it = 0;
+        bool ok = true;
+        for (int tile = first; tile < tiles && ok; tile += step) {
+          const int tr = tile / p.tiles_c, tc = tile - tr * p.tiles_c;
+          for (int kb = k0; kb < k1; ++kb, ++it) {
+            const int s = it % C::STAGES;
+            if (it >= C::STAGES && !mbar_wait(empty(s), (uint32_t)(it / C::STAGES - 1) & 1u, err, kDevErrTimeoutEmpty)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(full(s), C::STAGE_BYTES);
+            const uint32_t st = base + s * C::STAGE_BYTES;
+            tma_load_2d(st, &tmA, kb * 128, tr * 128, full(s));
+            tma_load_2d(st + C::A_BYTES, &tmB, kb * 128, tc * BN, full(s));
           }
-          mbar_arrive_expect_tx(full(s), C::STAGE_BYTES);
-          const uint32_t st = base + s * C::STAGE_BYTES;
-          tma_load_2d(st, &tmA, kb * 128, tr * 128, full(s));
-          tma_load_2d(st + C::A_BYTES, &tmB, kb * 128, tc * BN, full(s));
         }
+        // no copy may still be writing shared memory when the CTA exits
+        for (int i = it > C::STAGES ? it - C::STAGES : 0; i < it; ++i)
+          mbar_wait(full(i % C::STAGES), (uint32_t)(i / C::STAGES) & 1u, err, kDevErrTimeoutFull);
       }
-      // no copy may still be writing shared memory when the CTA exits
-      for (int i = it > C::STAGES ? it - C::STAGES : 0; i < it; ++i)
-        mbar_wait(full(i % C::STAGES), (uint32_t)(i / C::STAGES) & 1u, err, kDevErrTimeoutFull);
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    if (lane == 0) {
-      int it = 0;
-      bool ok = true;
-      constexpr uint32_t idesc = idesc_f8_e4m3(BN);
-      for (int tile = first; tile < tiles && ok; tile += step) {
-        for (int kb = k0; kb < k1; ++kb, ++it) {
-          const int s = it % C::STAGES, a = it % C::ACCS;
-          if (!mbar_wait(full(s), (uint32_t)(it / C::STAGES) & 1u, err, kDevErrTimeoutFull) ||
-              (it >= C::ACCS && !mbar_wait(tempty(a), (uint32_t)(it / C::ACCS - 1) & 1u, err, kDevErrTimeoutTmem))) {
-            ok = false;
-            break;
+      __syncwarp();
+    } else if (warp == 1) {
+      if (lane == 0) {
+        int it = 0;
+        bool ok = true;
+        constexpr uint32_t idesc = idesc_f8_e4m3(BN);
+        for (int tile = first; tile < tiles && ok; tile += step) {
+          for (int kb = k0; kb < k1; ++kb, ++it) {
+            const int s = it % C::STAGES, a = it % C::ACCS;
+            if (!mbar_wait(full(s), (uint32_t)(it / C::STAGES) & 1u, err, kDevErrTimeoutFull) ||
+                (it >= C::ACCS && !mbar_wait(tempty(a), (uint32_t)(it / C::ACCS - 1) & 1u, err, kDevErrTimeoutTmem))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t st = base + s * C::STAGE_BYTES;
+  #pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_f8f6f4(tmem + a * BN, smem_desc(st + 32u * kk, 16, 1024, 2),
+                         smem_desc(st + C::A_BYTES + 32u * kk, 16, 1024, 2), idesc, kk > 0 ? 1u : 0u);
+            tc_commit(empty(s));
+            tc_commit(tfull(a));
           }
-          tc_fence_after();
-          const uint32_t st = base + s * C::STAGE_BYTES;
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_f8f6f4(tmem + a * BN, smem_desc(st + 32u * kk, 16, 1024, 2),
-                       smem_desc(st + C::A_BYTES + 32u * kk, 16, 1024, 2), idesc, kk > 0 ? 1u : 0u);
-          tc_commit(empty(s));
-          tc_commit(tfull(a));
         }
+        // the tensor core must be done with shared and tensor memory before the CTA leaves
+        if (it > 0) mbar_wait(tfull((it - 1) % C::ACCS), (uint32_t)((it - 1) / C::ACCS) & 1u, err, kDevErrTimeoutDrain);
       }
-      // the tensor core must be done with shared and tensor memory before the CTA leaves
-      if (it > 0) mbar_wait(tfull((it - 1) % C::ACCS), (uint32_t)((it - 1) / C::ACCS) & 1u, err, kDevErrTimeoutDrain);
+      __syncwarp();
     }
-    __syncwarp();
   } else {
-    const int quad = warp & 3, half = (warp - 2) >> 2;
+    if constexpr (C::kRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kEpiRegs));
+    const int quad = warp & 3, half = (warp - C::EPI0) >> 2;
     const int r = quad * 32 + lane;                       // row of the tile, lane of tensor memory
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * C::NC);
     int it = 0;
@@ -339,6 +373,16 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
       unsigned long long acc[C::NC / 2];
 #pragma unroll
       for (int i = 0; i < C::NC / 2; ++i) acc[i] = 0ull;
+      // the sums start from the bias (on rank 0 of a split tile), so that nothing is left to load at the end
+      if (!kSwap && p.bias && rank == 0) {
+#pragma unroll
+        for (int c = 0; c < C::NC / 8; ++c) {
+          float y[8];
+          bias8(p, col0 + 8 * c, y);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[4 * c + i] = f32x2_pack(y[2 * i], y[2 * i + 1]);
+        }
+      }
       float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
       if (k0 < k1) scales(k0, s0, s1);
       for (int kb = k0; kb < k1; ++kb, ++it) {
@@ -348,37 +392,65 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
           ok = false;   // the whole warp gives up together: the loads below are warp-wide
         if (!ok) break;
         tc_fence_after();
-        uint32_t v[2][16];
-        tmem_ld_32x32b_x16(lane_base + a * BN, v[0]);
+        constexpr int CH = C::CH;
+        uint32_t v[2][CH];
+        auto load = [&](int c) {
+          if constexpr (CH == 32) tmem_ld_32x32b_x32(lane_base + a * BN + CH * c, v[c & 1]);
+          else tmem_ld_32x32b_x16(lane_base + a * BN + CH * c, v[c & 1]);
+        };
+        load(0);
 #pragma unroll
-        for (int c = 0; c < C::NC / 16; ++c) {
+        for (int c = 0; c < C::NC / CH; ++c) {
           tmem_wait_ld();
-          reg_fence16(v[c & 1]);
-          if (c + 1 < C::NC / 16) {
-            tmem_ld_32x32b_x16(lane_base + a * BN + 16 * (c + 1), v[(c + 1) & 1]);
+#pragma unroll
+          for (int i = 0; i < CH; i += 16) reg_fence16(&v[c & 1][i]);
+          if (c + 1 < C::NC / CH) {
+            load(c + 1);
           } else {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(tempty(a));
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < CH / 2; ++i) {
             unsigned long long s2;
             if constexpr (!kSwap) {
               s2 = f32x2_pack(s0, s0);
             } else {
-              const float u = c < 2 ? s0 : s1;
-              s2 = f32x2_pack(__shfl_sync(0xFFFFFFFFu, u, (16 * c + 2 * i) & 31),
-                              __shfl_sync(0xFFFFFFFFu, u, (16 * c + 2 * i + 1) & 31));
+              const float u = CH * c + 2 * i < 32 ? s0 : s1;
+              s2 = f32x2_pack(__shfl_sync(0xFFFFFFFFu, u, (CH * c + 2 * i) & 31),
+                              __shfl_sync(0xFFFFFFFFu, u, (CH * c + 2 * i + 1) & 31));
             }
-            acc[8 * c + i] = fma_f32x2(f32x2_pack(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])),
-                                       s2, acc[8 * c + i]);
+            unsigned long long& d = acc[CH / 2 * c + i];
+            d = fma_f32x2(f32x2_pack(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), s2, d);
           }
         }
         s0 = t0;
         s1 = t1;
       }
-      if (p.split == 1) {
+      if (!kSwap && !kF32 && p.out_tma) {
+        // bf16: 64 columns of the warp's 32 rows at a time through shared memory (128-byte swizzle), one TMA
+        // store each, so the warp is free for the next tile as soon as the sums are in shared memory
+        uint8_t* stg = gb + C::STG_OFF + (warp - C::EPI0) * 4096;
+#pragma unroll
+        for (int c = 0; c < C::NC / 64; ++c) {
+          if (lane == 0) bulk_wait_read();
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = bf16x2_round(acc[32 * c + 4 * j + i]);
+            *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0 && col0 + 64 * c < p.N) {   // rows past M and columns past N are clipped
+            tma_store_2d(&tmO, smem_u32(stg), col0 + 64 * c, tr * 128 + quad * 32);
+            bulk_commit();
+          }
+        }
+      } else if (p.split == 1) {
         float y[8];
 #pragma unroll
         for (int c = 0; c < C::NC / 8; ++c) {
@@ -403,16 +475,20 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
         }
       }
     }
+    if (!kSwap && !kF32 && p.out_tma) {
+      if (lane == 0) bulk_wait_all();
+      __syncwarp();
+    }
   }
 
   if (p.split > 1) {
     __syncwarp();
     cluster_sync_all();
     // rank's share of the columns, summed over the ranks in their order
-    if (warp >= 2 && first < tiles) {
+    if (warp >= C::EPI0 && first < tiles) {
       const int tr = first / p.tiles_c, tc = first - tr * p.tiles_c;
-      const int quad = warp & 3, half = (warp - 2) >> 2, r = quad * 32 + lane;
-      const int per = BN / 8 / p.split > 0 ? BN / 8 / p.split : 1;   // runs of 8 columns
+      const int quad = warp & 3, half = (warp - C::EPI0) >> 2, r = quad * 32 + lane;
+      const int per = BN / 8 / p.split;   // runs of 8 columns
       if constexpr (!kSwap) {
         for (int c = rank * per + half; c < (rank + 1) * per; c += C::EW) {
           float y[8];
@@ -458,6 +534,20 @@ static int make_code_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t 
   return VF4_OK;
 }
 
+// Output map of the TMA-store epilogue: bf16 (M, N), boxes of 32 rows x 64 columns, 128-byte swizzle.
+static int make_bf16_out_map(CUtensorMap* m, void* ptr, int64_t rows, int64_t cols, int64_t ld) {
+  EncodeTiledFn enc = encode_tiled();
+  if (!enc) return fail(VF4_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  cuuint32_t box[2] = {64u, 32u};
+  cuuint32_t es[2] = {1u, 1u};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(VF4_ERR_CUDA, "cuTensorMapEncodeTiled (output) failed (%d)", (int)r);
+  return VF4_OK;
+}
+
 struct F8Operand {
   const uint8_t* ptr;
   int64_t rows, ld;
@@ -466,17 +556,29 @@ struct F8Operand {
 template <int BN, bool kSwap, bool kF32>
 static int launch_fp8_gemm(F8Operand a, F8Operand b, int64_t K, F8Params p, cudaStream_t s) {
   using C = F8Cfg<BN, kSwap>;
-  CUtensorMap ta, tb;
+  CUtensorMap ta, tb, to;
+  memset(&to, 0, sizeof(to));
   if (int st = make_code_map(&ta, a.ptr, a.rows, K, a.ld, 128)) return st;
   if (int st = make_code_map(&tb, b.ptr, b.rows, K, b.ld, BN)) return st;
   auto kern = fp8_gemm_kernel<BN, kSwap, kF32>;
   if (int st = smem_optin(kern, C::SMEM)) return st;
+  if (C::kRegs) {   // the register split of the kernel relies on what its launch allocates
+    static const int regs = [] {
+      cudaFuncAttributes a;
+      return cudaFuncGetAttributes(&a, fp8_gemm_kernel<BN, kSwap, kF32>) == cudaSuccess ? a.numRegs : 0;
+    }();
+    if (regs != C::kLaunchRegs) return fail(VF4_ERR_UNSUPPORTED, "vf4_gemm_fp8_block: built with %d registers", regs);
+  }
   p.tiles_r = (int)((a.rows + 127) / 128);
   p.tiles_c = (int)((b.rows + BN - 1) / BN);
   const int tiles = p.tiles_r * p.tiles_c, sms = num_sms();
   // share a tile among up to 8 CTAs (the portable cluster size) while that leaves no SM two of them
   p.split = 1;
   while (p.split < 8 && tiles * p.split * 2 <= sms && p.split * 2 <= p.kb) p.split *= 2;
+  p.out_tma = !kSwap && !kF32 && p.split == 1 && p.out_vec;
+  if (p.out_tma) {
+    if (int st = make_bf16_out_map(&to, p.out, p.M, p.N, p.ldo)) return st;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.split > 1 ? tiles * p.split : (tiles < sms ? tiles : sms)));
   cfg.blockDim = dim3(C::THREADS);
@@ -488,7 +590,7 @@ static int launch_fp8_gemm(F8Operand a, F8Operand b, int64_t K, F8Params p, cuda
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = p.split > 1 ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, kern, ta, tb, p) != cudaSuccess) return launch_status("vf4_gemm_fp8_block");
+  if (cudaLaunchKernelEx(&cfg, kern, ta, tb, to, p) != cudaSuccess) return launch_status("vf4_gemm_fp8_block");
   return launch_status("vf4_gemm_fp8_block");
 }
 
@@ -515,7 +617,7 @@ int vf4_cast_fp8_block(const void* x, int dtype, int64_t M, int64_t K, int64_t l
     return fail(VF4_ERR_ARG, "vf4_cast_fp8_block: bad sizes (M=%lld K=%lld ld=%lld block_rows=%d)", (long long)M,
                 (long long)K, (long long)ld, block_rows);
   if (dtype != VF4_BF16 && dtype != VF4_F32) return fail(VF4_ERR_ARG, "vf4_cast_fp8_block: bad dtype %d", dtype);
-  if (K > (1 << 20) || M > INT32_MAX) return fail(VF4_ERR_UNSUPPORTED, "vf4_cast_fp8_block: sizes too large");
+  if (K > (1 << 20) || M > (1 << 30)) return fail(VF4_ERR_UNSUPPORTED, "vf4_cast_fp8_block: sizes too large");
   if (M == 0) return VF4_OK;
   if (!x || !codes || !scale) return fail(VF4_ERR_ARG, "vf4_cast_fp8_block: null pointer");
   if (!aligned16(codes) || ldc % 16 || ldc < K)
@@ -530,7 +632,7 @@ int vf4_cast_fp8_block(const void* x, int dtype, int64_t M, int64_t K, int64_t l
   const auto* xf = static_cast<const float*>(x);
   if (block_rows == 1) {
     const int64_t want = (M * kb + 15) / 16;   // 16 blocks per CTA and step
-    const int64_t most = (int64_t)num_sms() * 8;
+    const int64_t most = (int64_t)num_sms() * 4;   // the CTAs that are resident at once
     const unsigned grid = (unsigned)(want < most ? want : most);
     const int K32 = (int)K;
 #define VF4_CAST_ROWS(T, X, V) \
@@ -595,6 +697,7 @@ int vf4_gemm_fp8_block(const uint8_t* a, int64_t lda, const float* a_scale, int6
   p.kb = (int)((K + 127) / 128);
   p.bias = bias;
   p.bias_f32 = bias_dtype == VF4_F32;
+  p.bias_vec = aligned16(bias);
   p.out = out;
   p.ldo = ldo;
   p.out_vec = aligned16(out) && ldo * esz % 16 == 0;

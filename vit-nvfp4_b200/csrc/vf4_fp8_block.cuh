@@ -21,15 +21,24 @@ struct Fp8Block {
   bool plain;
 };
 
+// RN(a / 448) for normal a >= 1e-12 by one Markstein step on y = RN(1 / 448); checked against the
+// correctly rounded division for every significand (both sides scale exactly by powers of two).
+VF4_DEV float div448_rn(float a) {
+  const float y = 0.00223214295692741870880126953125f;   // RN(1/448) = 0x3B124925
+  const float q = __fmul_rn(a, y);
+  return __fmaf_rn(__fmaf_rn(-q, 448.0f, a), y, q);
+}
+
 VF4_DEV Fp8Block fp8_block(uint32_t amax_bits) {
   float a = __uint_as_float(amax_bits);
   a = a < 1e-12f ? 1e-12f : a;   // keeps a NaN
   Fp8Block b;
-  b.scale = __fdiv_rn(a, 448.f);
+  b.scale = div448_rn(a);
   const bool big = a >= 0x1p96f;
   b.mul = big ? 448.f * 0x1p-32f : 448.f;
   b.div = big ? a * 0x1p-32f : a;
   b.plain = !(a < __uint_as_float(0x7F800000u));
+  if (b.plain) b.scale = a;
   b.inv = __frcp_rn(b.div);
   return b;
 }
@@ -98,5 +107,38 @@ VF4_DEV void load8(const T* p, int nv, float* v) {
     for (int i = 0; i < 8; ++i) v[i] = i < nv ? (float)p[i] : 0.f;
   }
 }
+
+// The same eight elements kept as they were loaded (bf16: four registers instead of eight).
+template <typename T, bool kVec>
+struct Raw8 {
+  float v[8];
+  VF4_DEV void load(const T* p, int nv) { load8<T, kVec>(p, nv, v); }
+  VF4_DEV uint32_t amax_bits() const { return amax8_bits(v); }
+  VF4_DEV void get(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = v[i];
+  }
+};
+
+template <>
+struct Raw8<__nv_bfloat16, true> {
+  uint4 w;
+  VF4_DEV void load(const __nv_bfloat16* p, int nv) {
+    w = nv > 0 ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+  }
+  VF4_DEV uint32_t amax_bits() const {   // two 16-bit lanes: the magnitudes' order is their bits' order
+    const uint32_t k = 0x7FFF7FFFu;
+    const uint32_t m = umax_u16x2(umax_u16x2(w.x & k, w.y & k), umax_u16x2(w.z & k, w.w & k));
+    return max(m << 16, m & 0x7FFF0000u);
+  }
+  VF4_DEV void get(float* f) const {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(u[i] << 16);
+      f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+    }
+  }
+};
 
 }  // namespace vf4
