@@ -365,10 +365,15 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
       // kSwap with 64 columns: a second activation row per lane
       const bool have2 = kSwap && C::NC > 32 && col0 + 32 + lane < p.M;
       const int64_t off2 = 32 * p.sa_m;
-      auto scales = [&](int kb, float& s0, float& s1) {
-        const float w = __ldg(s_blk + kb * step_blk);
-        s0 = have ? __ldg(s_own + kb * step_own) * w : 0.f;
-        s1 = have2 ? __ldg(s_own + off2 + kb * step_own) * w : 0.f;
+      // the scales of K blocks kb + 1 and kb + 2 are on their way while kb is worked on, and multiplied only
+      // when used: a product right after the load would wait for L2 once per block
+      constexpr int kAhead = 3;
+      float sw[kAhead], sx[kAhead], sy[kAhead];
+      auto fetch = [&](int kb, int slot) {
+        if (kb >= k1) return;
+        sw[slot] = __ldg(s_blk + kb * step_blk);
+        sx[slot] = have ? __ldg(s_own + kb * step_own) : 0.f;
+        if constexpr (kSwap && C::NC > 32) sy[slot] = have2 ? __ldg(s_own + off2 + kb * step_own) : 0.f;
       };
       unsigned long long acc[C::NC / 2];
 #pragma unroll
@@ -383,14 +388,17 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
           for (int i = 0; i < 4; ++i) acc[4 * c + i] = f32x2_pack(y[2 * i], y[2 * i + 1]);
         }
       }
-      float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
-      if (k0 < k1) scales(k0, s0, s1);
-      for (int kb = k0; kb < k1; ++kb, ++it) {
-        if (kb + 1 < k1) scales(kb + 1, t0, t1);
+#pragma unroll
+      for (int u = 0; u + 1 < kAhead; ++u) fetch(k0 + u, u);
+      auto block = [&](int kb, int slot) {
+        fetch(kb + kAhead - 1, (slot + kAhead - 1) % kAhead);
+        const float s0 = sx[slot] * sw[slot];
+        float s1 = 0.f;
+        if constexpr (kSwap && C::NC > 32) s1 = sy[slot] * sw[slot];
         const int a = it % C::ACCS;
         if (!__all_sync(0xFFFFFFFFu, ok && mbar_wait(tfull(a), (uint32_t)(it / C::ACCS) & 1u, err, kDevErrTimeoutTmem)))
           ok = false;   // the whole warp gives up together: the loads below are warp-wide
-        if (!ok) break;
+        if (!ok) return;
         tc_fence_after();
         constexpr int CH = C::CH;
         uint32_t v[2][CH];
@@ -425,8 +433,12 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
             d = fma_f32x2(f32x2_pack(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), s2, d);
           }
         }
-        s0 = t0;
-        s1 = t1;
+        ++it;
+      };
+      for (int kb = k0; kb < k1 && ok; kb += kAhead) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (kb + u < k1 && ok) block(kb + u, u);
       }
       if (!kSwap && !kF32 && p.out_tma) {
         // bf16: 64 columns of the warp's 32 rows at a time through shared memory (128-byte swizzle), one TMA
