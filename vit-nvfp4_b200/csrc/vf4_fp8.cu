@@ -135,8 +135,12 @@ __global__ void __launch_bounds__(256) fp8_cast_tile_kernel(const T* __restrict_
 // ---------------------------------------------------------------------------------------
 template <int BN, bool kSwap>
 struct F8Cfg {
-  static constexpr int A_BYTES = 128 * 128, B_BYTES = BN * 128, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+  // 256 columns: a pair of CTAs (one cluster) shares a 256 x 256 tile, each holding 128 rows of A and 128
+  // of B's 256 rows in its own shared memory
+  static constexpr bool kPair = BN == 256;
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = (kPair ? 128 : BN) * 128, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int ROWS = kPair ? 256 : 128;         // rows of a tile
+  static constexpr int STAGES = BN >= 128 ? 5 : 8;
   static constexpr int ACCS = BN == 256 ? 2 : 4;
   static constexpr int TMEM_COLS = ACCS * BN;            // 64 .. 512, a power of two
   static constexpr int EW = BN >= 128 ? 2 : 1;           // epilogue warps per lane quadrant
@@ -147,17 +151,23 @@ struct F8Cfg {
   static constexpr int CH = NC >= 64 ? 32 : 16;
   // the 256-column tile needs 128 sums + 64 loaded values per thread: its epilogue warps take registers
   // over from the four warps of the control group (2 of them idle)
-  static constexpr bool kRegs = BN == 256;
+  static constexpr bool kRegs = kPair;
   static constexpr int EPI0 = kRegs ? 4 : 2;             // first epilogue warp
   static constexpr int THREADS = 32 * (EPI0 + EPI_WARPS);
   static constexpr int kLaunchRegs = 168, kControlRegs = 40, kEpiRegs = 232;   // 384 threads: 168 at launch
   static_assert(!kRegs || 128 * kControlRegs + 256 * kEpiRegs <= THREADS * kLaunchRegs, "register split");
   static constexpr int STG_OFF = STAGES * STAGE_BYTES;   // bf16 output staging, 32 rows x 64 columns per warp
   static constexpr int STG_BYTES = kSwap ? 0 : EPI_WARPS * 4096;
-  static constexpr int BAR_OFF = STG_OFF + STG_BYTES;
-  static constexpr int SMEM = 1024 + BAR_OFF + 8 * (2 * STAGES + 2 * ACCS) + 16;
+  // scales on their way to the epilogue threads (kSwap loads them into registers instead): kRing K blocks
+  // ahead, across tiles, {own row's, weight block's} per thread
+  static constexpr int kRing = kSwap ? 0 : 8;
+  static constexpr int RING_OFF = STG_OFF + STG_BYTES, RING_SLOT = 32 * EPI_WARPS * 8;
+  static constexpr int BIAS_OFF = RING_OFF + kRing * RING_SLOT;   // each epilogue warp's bias values
+  static constexpr int BAR_OFF = BIAS_OFF + (kSwap ? 0 : EPI_WARPS * NC * 4);
+  static constexpr int NBAR = 2 * STAGES + 2 * ACCS;
+  static constexpr int SMEM = 1024 + BAR_OFF + 8 * NBAR + 16;
   static_assert(SMEM <= 227 * 1024, "shared memory");
-  static_assert(BN * 128 * 4 <= STAGES * STAGE_BYTES, "the split sums reuse the stages");
+  static_assert(kPair || BN * 128 * 4 <= STAGES * STAGE_BYTES, "the split sums reuse the stages");
 };
 
 struct F8Params {
@@ -165,7 +175,7 @@ struct F8Params {
   const float* sb;     // weight scales: element (n / 128, g) at (n / 128) * sb_n + g * sb_k
   int64_t sa_m, sa_k, sb_n, sb_k;
   int M, N, kb;
-  int tiles_r, tiles_c, split;   // tiles of 128 (A rows) and of BN (B rows)
+  int tiles_r, tiles_c, split;   // tiles of ROWS (A rows) and of BN (B rows); CTAs that share a tile's K blocks
   const void* bias;
   int bias_f32, bias_vec;   // its type; whether 8 values may be loaded at once
   void* out;
@@ -228,6 +238,21 @@ VF4_DEV void store1(const F8Params& p, int m, int n, float y) {
   else static_cast<__nv_bfloat16*>(p.out)[(int64_t)m * p.ldo + n] = __float2bfloat16_rn(y);
 }
 
+// 4 bytes global -> shared, or zeros; tracked by this thread's groups.
+VF4_DEV void cp_async4(uint32_t dst, const float* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+VF4_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+VF4_DEV void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+VF4_DEV float2 ld_shared_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
 VF4_DEV float ld_shared_cluster(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -248,9 +273,11 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
   auto empty = [&](int i) { return bar + 8u * (C::STAGES + i); };
   auto tfull = [&](int i) { return bar + 8u * (2 * C::STAGES + i); };
   auto tempty = [&](int i) { return bar + 8u * (2 * C::STAGES + C::ACCS + i); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + C::BAR_OFF + 8 * (2 * C::STAGES + 2 * C::ACCS));
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + C::BAR_OFF + 8 * C::NBAR);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* err = &g_fp8_err;
+  // kPair: rank in the pair; otherwise the rank among the CTAs that share a tile's K blocks
+  const int rank = C::kPair || p.split > 1 ? (int)cluster_ctarank() : 0;
 
   if (warp == 0 && lane == 0) {
     for (int i = 0; i < C::STAGES; ++i) {
@@ -259,7 +286,7 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
     }
     for (int i = 0; i < C::ACCS; ++i) {
       mbar_init(tfull(i), 1);
-      mbar_init(tempty(i), C::EPI_WARPS);
+      mbar_init(tempty(i), C::EPI_WARPS * (C::kPair ? 2 : 1));
     }
     fence_mbar_init();
     tma_prefetch(&tmA);
@@ -267,67 +294,112 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
     if (p.out_tma) tma_prefetch(&tmO);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
-    tmem_relinquish();
+    if constexpr (C::kPair) {
+      tmem_alloc_pair(smem_u32(tmem_slot), C::TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+      tmem_relinquish();
+    }
   }
   fence_async_shared();
   tc_fence_before();
-  __syncthreads();
+  if constexpr (C::kPair) cluster_sync_all();
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
 
   // this CTA's run of K blocks, and its tiles (split > 1: one per cluster)
-  const int rank = p.split > 1 ? (int)cluster_ctarank() : 0;
-  const int k0 = (int)((int64_t)p.kb * rank / p.split), k1 = (int)((int64_t)p.kb * (rank + 1) / p.split);
+  const int k0 = C::kPair ? 0 : (int)((int64_t)p.kb * rank / p.split);
+  const int k1 = C::kPair ? p.kb : (int)((int64_t)p.kb * (rank + 1) / p.split);
   const int tiles = p.tiles_r * p.tiles_c;
-  const int first = blockIdx.x / p.split, step = gridDim.x / p.split;
+  const int share = C::kPair ? 2 : p.split;   // CTAs per tile
+  const int first = blockIdx.x / share, step = gridDim.x / share;
 
   if (warp < C::EPI0) {
     if constexpr (C::kRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kControlRegs));
+    // Both loops run as whole warps with one elected lane issuing: their addresses and descriptors then stay
+    // warp-uniform.  Inside a one-lane branch each MMA's operands were moved into uniform registers one at a
+    // time, and a block of four MMAs took 600 clocks to issue whatever its size (513 of 512 now).
+    const bool elected = elect_one();
     if (warp == 0) {
-      if (lane == 0) {
-        int it = 0;
-        bool ok = true;
-        for (int tile = first; tile < tiles && ok; tile += step) {
-          const int tr = tile / p.tiles_c, tc = tile - tr * p.tiles_c;
-          for (int kb = k0; kb < k1; ++kb, ++it) {
-            const int s = it % C::STAGES;
-            if (it >= C::STAGES && !mbar_wait(empty(s), (uint32_t)(it / C::STAGES - 1) & 1u, err, kDevErrTimeoutEmpty)) {
-              ok = false;
-              break;
+      int s = 0, it = 0;
+      uint32_t ph = 1;   // an unused stage counts as released
+      bool ok = true;
+      for (int tile = first; tile < tiles && ok; tile += step) {
+        const int tr = tile / p.tiles_c, tc = tile - tr * p.tiles_c;
+        const int ya = tr * C::ROWS + (C::kPair ? rank * 128 : 0), yb = tc * BN + (C::kPair ? rank * 128 : 0);
+        for (int kb = k0; kb < k1; ++kb, ++it) {
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(empty(s), ph, err, kDevErrTimeoutEmpty));
+          if (!ok) break;
+          const uint32_t st = base + s * C::STAGE_BYTES;
+          if (elected) {
+            if constexpr (C::kPair) {   // both CTAs' copies complete on the leader's barrier
+              if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * C::STAGE_BYTES);
+              const uint32_t fb = mapa_shared(full(s), 0);
+              tma_load_2d_pair(st, &tmA, kb * 128, ya, fb);
+              tma_load_2d_pair(st + C::A_BYTES, &tmB, kb * 128, yb, fb);
+            } else {
+              mbar_arrive_expect_tx(full(s), C::STAGE_BYTES);
+              tma_load_2d(st, &tmA, kb * 128, ya, full(s));
+              tma_load_2d(st + C::A_BYTES, &tmB, kb * 128, yb, full(s));
             }
-            mbar_arrive_expect_tx(full(s), C::STAGE_BYTES);
-            const uint32_t st = base + s * C::STAGE_BYTES;
-            tma_load_2d(st, &tmA, kb * 128, tr * 128, full(s));
-            tma_load_2d(st + C::A_BYTES, &tmB, kb * 128, tc * BN, full(s));
+          }
+          __syncwarp();
+          if (++s == C::STAGES) {
+            s = 0;
+            ph ^= 1u;
           }
         }
-        // no copy may still be writing shared memory when the CTA exits
+      }
+      // no copy may still be writing shared memory when the CTA exits (a pair leaves together)
+      if (!C::kPair || rank == 0)
         for (int i = it > C::STAGES ? it - C::STAGES : 0; i < it; ++i)
           mbar_wait(full(i % C::STAGES), (uint32_t)(i / C::STAGES) & 1u, err, kDevErrTimeoutFull);
-      }
       __syncwarp();
     } else if (warp == 1) {
-      if (lane == 0) {
-        int it = 0;
+      if (!C::kPair || rank == 0) {   // one CTA issues for the pair
+        int s = 0, a = 0, it = 0;
+        uint32_t ph = 0, pa = 1;
         bool ok = true;
-        constexpr uint32_t idesc = idesc_f8_e4m3(BN);
+        constexpr uint32_t idesc = idesc_f8_e4m3(BN, C::ROWS);
+        const uint64_t ad0 = smem_desc(base, 16, 1024, 2), bd0 = smem_desc(base + C::A_BYTES, 16, 1024, 2);
+        auto both = [&](uint32_t b_full, uint32_t b_free) {
+          if constexpr (C::kPair)
+            return mbar_wait_cluster(b_full, ph, err, kDevErrTimeoutFull) &&
+                   mbar_wait_cluster(b_free, pa, err, kDevErrTimeoutTmem);
+          else
+            return mbar_wait(b_full, ph, err, kDevErrTimeoutFull) && mbar_wait(b_free, pa, err, kDevErrTimeoutTmem);
+        };
         for (int tile = first; tile < tiles && ok; tile += step) {
           for (int kb = k0; kb < k1; ++kb, ++it) {
-            const int s = it % C::STAGES, a = it % C::ACCS;
-            if (!mbar_wait(full(s), (uint32_t)(it / C::STAGES) & 1u, err, kDevErrTimeoutFull) ||
-                (it >= C::ACCS && !mbar_wait(tempty(a), (uint32_t)(it / C::ACCS - 1) & 1u, err, kDevErrTimeoutTmem))) {
-              ok = false;
-              break;
-            }
+            ok = __all_sync(0xFFFFFFFFu, both(full(s), tempty(a)));
+            if (!ok) break;
             tc_fence_after();
-            const uint32_t st = base + s * C::STAGE_BYTES;
-  #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_f8f6f4(tmem + a * BN, smem_desc(st + 32u * kk, 16, 1024, 2),
-                         smem_desc(st + C::A_BYTES + 32u * kk, 16, 1024, 2), idesc, kk > 0 ? 1u : 0u);
-            tc_commit(empty(s));
-            tc_commit(tfull(a));
+            if (elected) {
+              const uint64_t ad = ad0 + (uint32_t)(s * (C::STAGE_BYTES >> 4)), bd = bd0 + (uint32_t)(s * (C::STAGE_BYTES >> 4));
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) {   // 32 bytes of K further: the descriptors' addresses count 16 bytes
+                if constexpr (C::kPair) mma_f8f6f4_pair(tmem + a * BN, ad + 2 * kk, bd + 2 * kk, idesc, kk > 0 ? 1u : 0u);
+                else mma_f8f6f4(tmem + a * BN, ad + 2 * kk, bd + 2 * kk, idesc, kk > 0 ? 1u : 0u);
+              }
+              if constexpr (C::kPair) {
+                tc_commit_pair(empty(s), 3);
+                tc_commit_pair(tfull(a), 3);
+              } else {
+                tc_commit(empty(s));
+                tc_commit(tfull(a));
+              }
+            }
+            __syncwarp();
+            if (++s == C::STAGES) {
+              s = 0;
+              ph ^= 1u;
+            }
+            if (++a == C::ACCS) {
+              a = 0;
+              pa ^= 1u;
+            }
           }
         }
         // the tensor core must be done with shared and tensor memory before the CTA leaves
@@ -340,63 +412,88 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
     const int quad = warp & 3, half = (warp - C::EPI0) >> 2;
     const int r = quad * 32 + lane;                       // row of the tile, lane of tensor memory
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * C::NC);
-    int it = 0;
     bool ok = true;
+    // !kSwap: the scales of the K blocks ahead, copied by each thread for itself through shared memory.  They
+    // have to be asked for that early: read two blocks ahead into registers they still cost the 16400 x 5120 x
+    // 5120 product a third of its time (each block's column of scales is a line that L1 has not seen).
+    uint32_t ring = 0;
+    int f_tile = first, f_kb = k1;
+    uint32_t f_dst = 0;
+    const float *f_a = p.sa, *f_b = p.sb;
+    bool f_row = false;
+    auto fetch_ring = [&]() {
+      if (f_kb == k1 && f_tile < tiles) {   // the first block of the next tile
+        const int tr = f_tile / p.tiles_c, tc = f_tile - tr * p.tiles_c;
+        const int row = tr * C::ROWS + (C::kPair ? rank * 128 : 0) + r;
+        f_row = row < p.M;
+        f_a = p.sa + (int64_t)(f_row ? row : 0) * p.sa_m + k0 * p.sa_k;
+        f_b = p.sb + (int64_t)(min(tc * BN + half * C::NC, p.N - 1) >> 7) * p.sb_n + k0 * p.sb_k;
+        f_kb = k0;
+        f_tile += step;
+      }
+      if (f_kb < k1) {
+        cp_async4(ring + f_dst, f_a, f_row);
+        cp_async4(ring + f_dst + 4, f_b, true);
+        f_a += p.sa_k;
+        f_b += p.sb_k;
+        ++f_kb;
+      }
+      cp_async_commit();   // also without a copy: the waits below count groups
+      f_dst = f_dst == (uint32_t)((C::kRing - 1) * C::RING_SLOT) ? 0u : f_dst + C::RING_SLOT;
+    };
+    if constexpr (!kSwap) {
+      ring = base + C::RING_OFF + (uint32_t)(threadIdx.x - 32 * C::EPI0) * 8u;
+      for (int i = 0; i + 1 < C::kRing; ++i) fetch_ring();
+    }
+    uint32_t use = 0;
+    int a = 0;
+    uint32_t pa = 0;
     for (int tile = first; tile < tiles; tile += step) {
       const int tr = tile / p.tiles_c, tc = tile - tr * p.tiles_c;
-      const int row = tr * 128 + r, col0 = tc * BN + half * C::NC;
-      // scale pointers: the thread's own row, or (kSwap) one activation row per lane
-      const float* s_own;
-      int64_t step_own;
-      const float* s_blk;
-      int64_t step_blk = p.sb_k;
-      bool have;
-      if constexpr (!kSwap) {
-        have = row < p.M;
-        s_own = p.sa + (int64_t)(have ? row : 0) * p.sa_m;
-        step_own = p.sa_k;
-        s_blk = p.sb + (int64_t)min(col0, p.N - 1) / 128 * p.sb_n;
-      } else {
-        have = lane < C::NC && col0 + lane < p.M;
-        s_own = p.sa + (int64_t)(have ? col0 + lane : 0) * p.sa_m;
-        step_own = p.sa_k;
-        s_blk = p.sb + (int64_t)tr * p.sb_n;
-      }
-      // kSwap with 64 columns: a second activation row per lane
-      const bool have2 = kSwap && C::NC > 32 && col0 + 32 + lane < p.M;
-      const int64_t off2 = 32 * p.sa_m;
-      // the scales of K blocks kb + 1 and kb + 2 are on their way while kb is worked on, and multiplied only
-      // when used: a product right after the load would wait for L2 once per block
+      const int row0 = tr * C::ROWS + (C::kPair ? rank * 128 : 0) + quad * 32;   // first row of this warp
+      const int row = row0 + lane, col0 = tc * BN + half * C::NC;
+      // kSwap: one activation row's scale per lane (two with 64 columns), the weight's alike for all.  The
+      // values of blocks kb + 1 and kb + 2 are on their way while kb is worked on, multiplied only when used.
       constexpr int kAhead = 3;
-      float sw[kAhead], sx[kAhead], sy[kAhead];
+      [[maybe_unused]] float sw[kAhead], sx[kAhead], sy[kAhead];
+      const bool have = kSwap && lane < C::NC && col0 + lane < p.M;
+      const bool have2 = kSwap && C::NC > 32 && col0 + 32 + lane < p.M;
+      const float* s_own = p.sa + (int64_t)(have ? col0 + lane : 0) * p.sa_m;
+      const float* s_blk = p.sb + (int64_t)tr * p.sb_n;
       auto fetch = [&](int kb, int slot) {
         if (kb >= k1) return;
-        sw[slot] = __ldg(s_blk + kb * step_blk);
-        sx[slot] = have ? __ldg(s_own + kb * step_own) : 0.f;
-        if constexpr (kSwap && C::NC > 32) sy[slot] = have2 ? __ldg(s_own + off2 + kb * step_own) : 0.f;
+        sw[slot] = __ldg(s_blk + kb * p.sb_k);
+        sx[slot] = have ? __ldg(s_own + kb * p.sa_k) : 0.f;
+        if constexpr (C::NC > 32) sy[slot] = have2 ? __ldg(s_own + 32 * p.sa_m + kb * p.sa_k) : 0.f;
       };
       unsigned long long acc[C::NC / 2];
 #pragma unroll
       for (int i = 0; i < C::NC / 2; ++i) acc[i] = 0ull;
-      // the sums start from the bias (on rank 0 of a split tile), so that nothing is left to load at the end
-      if (!kSwap && p.bias && rank == 0) {
+      // this warp's NC bias values, NC / 32 per lane, asked for here and needed after the last block
+      constexpr int BPL = C::NC >= 32 ? C::NC / 32 : 1;
+      [[maybe_unused]] float bias[BPL];
+      if (!kSwap && p.bias && p.split == 1) {
 #pragma unroll
-        for (int c = 0; c < C::NC / 8; ++c) {
-          float y[8];
-          bias8(p, col0 + 8 * c, y);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[4 * c + i] = f32x2_pack(y[2 * i], y[2 * i + 1]);
-        }
+        for (int i = 0; i < BPL; ++i) bias[i] = bias_at(p, col0 + BPL * lane + i);
       }
+      if constexpr (kSwap) {
 #pragma unroll
-      for (int u = 0; u + 1 < kAhead; ++u) fetch(k0 + u, u);
+        for (int u = 0; u + 1 < kAhead; ++u) fetch(k0 + u, u);
+      }
       auto block = [&](int kb, int slot) {
-        fetch(kb + kAhead - 1, (slot + kAhead - 1) % kAhead);
-        const float s0 = sx[slot] * sw[slot];
-        float s1 = 0.f;
-        if constexpr (kSwap && C::NC > 32) s1 = sy[slot] * sw[slot];
-        const int a = it % C::ACCS;
-        if (!__all_sync(0xFFFFFFFFu, ok && mbar_wait(tfull(a), (uint32_t)(it / C::ACCS) & 1u, err, kDevErrTimeoutTmem)))
+        float s0, s1 = 0.f;
+        if constexpr (kSwap) {
+          fetch(kb + kAhead - 1, (slot + kAhead - 1) % kAhead);
+          s0 = sx[slot] * sw[slot];
+          if constexpr (C::NC > 32) s1 = sy[slot] * sw[slot];
+        } else {
+          cp_async_wait<C::kRing - 2>();   // this block's pair, the oldest of the groups in flight
+          const float2 q = ld_shared_f2(ring + use);
+          use = use == (uint32_t)((C::kRing - 1) * C::RING_SLOT) ? 0u : use + C::RING_SLOT;
+          s0 = q.x * q.y;
+          fetch_ring();                    // into the slot read one block ago
+        }
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(tfull(a), pa, err, kDevErrTimeoutTmem)))
           ok = false;   // the whole warp gives up together: the loads below are warp-wide
         if (!ok) return;
         tc_fence_after();
@@ -417,7 +514,10 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
           } else {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(tempty(a));
+            if (lane == 0) {
+              if constexpr (C::kPair) mbar_arrive_peer(mapa_shared(tempty(a), 0));
+              else mbar_arrive(tempty(a));
+            }
           }
 #pragma unroll
           for (int i = 0; i < CH / 2; ++i) {
@@ -433,12 +533,27 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
             d = fma_f32x2(f32x2_pack(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), s2, d);
           }
         }
-        ++it;
+        if (++a == C::ACCS) {
+          a = 0;
+          pa ^= 1u;
+        }
       };
       for (int kb = k0; kb < k1 && ok; kb += kAhead) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
           if (kb + u < k1 && ok) block(kb + u, u);
+      }
+      if (!kSwap && p.bias && p.split == 1) {   // sums += bias, through shared memory (every lane needs all)
+        float* bs = reinterpret_cast<float*>(gb + C::BIAS_OFF) + (warp - C::EPI0) * C::NC;
+#pragma unroll
+        for (int i = 0; i < BPL; ++i) bs[BPL * lane + i] = bias[i];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < C::NC / 4; ++i) {
+          const float4 q = reinterpret_cast<const float4*>(bs)[i];
+          acc[2 * i] = add_f32x2(acc[2 * i], f32x2_pack(q.x, q.y));
+          acc[2 * i + 1] = add_f32x2(acc[2 * i + 1], f32x2_pack(q.z, q.w));
+        }
       }
       if (!kSwap && !kF32 && p.out_tma) {
         // bf16: 64 columns of the warp's 32 rows at a time through shared memory (128-byte swizzle), one TMA
@@ -457,8 +572,8 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
           }
           fence_async_shared();
           __syncwarp();
-          if (lane == 0 && col0 + 64 * c < p.N) {   // rows past M and columns past N are clipped
-            tma_store_2d(&tmO, smem_u32(stg), col0 + 64 * c, tr * 128 + quad * 32);
+          if (lane == 0 && col0 + 64 * c < p.N && row0 < p.M) {   // rows past M and columns past N are clipped
+            tma_store_2d(&tmO, smem_u32(stg), col0 + 64 * c, row0);
             bulk_commit();
           }
         }
@@ -487,13 +602,14 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
         }
       }
     }
+    if constexpr (!kSwap) cp_async_wait<0>();
     if (!kSwap && !kF32 && p.out_tma) {
       if (lane == 0) bulk_wait_all();
       __syncwarp();
     }
   }
 
-  if (p.split > 1) {
+  if (!C::kPair && p.split > 1) {
     __syncwarp();
     cluster_sync_all();
     // rank's share of the columns, summed over the ranks in their order
@@ -504,8 +620,7 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
       if constexpr (!kSwap) {
         for (int c = rank * per + half; c < (rank + 1) * per; c += C::EW) {
           float y[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = 0.f;
+          bias8(p, tc * BN + 8 * c, y);
           for (int q = 0; q < p.split; ++q) {
             const uint32_t src = mapa_shared(base, (uint32_t)q) + (uint32_t)((8 * c) * 128 + r) * 4u;
 #pragma unroll
@@ -527,9 +642,17 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
     cluster_sync_all();   // no CTA leaves while another reads its shared memory
   }
   tc_fence_before();
-  __syncthreads();
+  if constexpr (C::kPair) {
+    __syncwarp();
+    cluster_sync_all();   // the pair's MMAs read both CTAs' shared memory, and barriers are arrived on remotely
+  } else {
+    __syncthreads();
+  }
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, C::TMEM_COLS);
+  if (warp == 1) {
+    if constexpr (C::kPair) tmem_dealloc_pair(tmem, C::TMEM_COLS);
+    else tmem_dealloc(tmem, C::TMEM_COLS);
+  }
 }
 
 static int make_code_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t K, int64_t ld, int box_rows) {
@@ -571,7 +694,7 @@ static int launch_fp8_gemm(F8Operand a, F8Operand b, int64_t K, F8Params p, cuda
   CUtensorMap ta, tb, to;
   memset(&to, 0, sizeof(to));
   if (int st = make_code_map(&ta, a.ptr, a.rows, K, a.ld, 128)) return st;
-  if (int st = make_code_map(&tb, b.ptr, b.rows, K, b.ld, BN)) return st;
+  if (int st = make_code_map(&tb, b.ptr, b.rows, K, b.ld, C::kPair ? 128 : BN)) return st;
   auto kern = fp8_gemm_kernel<BN, kSwap, kF32>;
   if (int st = smem_optin(kern, C::SMEM)) return st;
   if (C::kRegs) {   // the register split of the kernel relies on what its launch allocates
@@ -581,27 +704,29 @@ static int launch_fp8_gemm(F8Operand a, F8Operand b, int64_t K, F8Params p, cuda
     }();
     if (regs != C::kLaunchRegs) return fail(VF4_ERR_UNSUPPORTED, "vf4_gemm_fp8_block: built with %d registers", regs);
   }
-  p.tiles_r = (int)((a.rows + 127) / 128);
+  p.tiles_r = (int)((a.rows + C::ROWS - 1) / C::ROWS);
   p.tiles_c = (int)((b.rows + BN - 1) / BN);
   const int tiles = p.tiles_r * p.tiles_c, sms = num_sms();
   // share a tile among up to 8 CTAs (the portable cluster size) while that leaves no SM two of them
   p.split = 1;
-  while (p.split < 8 && tiles * p.split * 2 <= sms && p.split * 2 <= p.kb) p.split *= 2;
+  while (!C::kPair && p.split < 8 && tiles * p.split * 2 <= sms && p.split * 2 <= p.kb) p.split *= 2;
   p.out_tma = !kSwap && !kF32 && p.split == 1 && p.out_vec;
   if (p.out_tma) {
     if (int st = make_bf16_out_map(&to, p.out, p.M, p.N, p.ldo)) return st;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.split > 1 ? tiles * p.split : (tiles < sms ? tiles : sms)));
+  const int pairs = sms / 2;
+  cfg.gridDim = dim3((unsigned)(C::kPair ? 2 * (tiles < pairs ? tiles : pairs)
+                                         : p.split > 1 ? tiles * p.split : (tiles < sms ? tiles : sms)));
   cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)p.split;
+  at[0].val.clusterDim.x = (unsigned)(C::kPair ? 2 : p.split);
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = p.split > 1 ? 1 : 0;
+  cfg.numAttrs = C::kPair || p.split > 1 ? 1 : 0;
   if (cudaLaunchKernelEx(&cfg, kern, ta, tb, to, p) != cudaSuccess) return launch_status("vf4_gemm_fp8_block");
   return launch_status("vf4_gemm_fp8_block");
 }
@@ -611,8 +736,8 @@ static int dispatch_fp8_gemm(F8Operand x, F8Operand w, int64_t K, const F8Params
   if (x.rows <= 16) return launch_fp8_gemm<16, true, kF32>(w, x, K, p, s);
   if (x.rows <= 32) return launch_fp8_gemm<32, true, kF32>(w, x, K, p, s);
   if (x.rows <= 64) return launch_fp8_gemm<64, true, kF32>(w, x, K, p, s);
-  const int64_t big = (x.rows + 127) / 128 * ((w.rows + 255) / 256);
-  if (big >= num_sms()) return launch_fp8_gemm<256, false, kF32>(x, w, K, p, s);
+  const int64_t big = (x.rows + 255) / 256 * ((w.rows + 255) / 256);
+  if (big >= num_sms() / 2) return launch_fp8_gemm<256, false, kF32>(x, w, K, p, s);
   return launch_fp8_gemm<128, false, kF32>(x, w, K, p, s);
 }
 
@@ -709,7 +834,7 @@ int vf4_gemm_fp8_block(const uint8_t* a, int64_t lda, const float* a_scale, int6
   p.kb = (int)((K + 127) / 128);
   p.bias = bias;
   p.bias_f32 = bias_dtype == VF4_F32;
-  p.bias_vec = aligned16(bias);
+  p.bias_vec = bias && aligned16(bias);   // (no bias: bias_at gives zeros)
   p.out = out;
   p.ldo = ldo;
   p.out_vec = aligned16(out) && ldo * esz % 16 == 0;
