@@ -355,6 +355,23 @@ VF4_API int vf4_gemm_fp8_block(const uint8_t* a, int64_t lda, const float* a_sca
                                int64_t M, int64_t N, int64_t K, const void* bias, int bias_dtype, void* out,
                                int64_t ldo, int out_dtype, vf4_stream_t stream);
 
+/* Norms before and after a block, fused with its gate and residual scale (sandwich / adaLN-gated blocks; a timm
+ * or DINOv2 block's LayerScale is the gate with one group and no post-norm):
+ *   x' = x + residual_scale * gate (.) N_post(y)        h = N_pre(x')
+ * x, y: (M, K) rows of ldx / ldy elements, both of dtype (VF4_BF16 or VF4_F32); K <= 16384.  post / pre: 0 none,
+ * 1 LayerNorm, 2 RMSNorm, with optional (K,) weight and bias; gate: (gate_groups, K), row m using group
+ * m / (M / gate_groups), or NULL; gate, weights and biases all of param_dtype.  All arithmetic in fp32; x'
+ * (M, K) is rounded once to dtype and enters N_pre before that rounding.  h: (M, K) in dtype, or (h_fp8) codes
+ * in rows of ldc bytes with scales at m * stride_m + (column / 128) * stride_k as vf4_cast_fp8_block writes them,
+ * cast from the fp32 values.  y NULL: h = N_pre(x) alone (x_out unused).  pre 0: x' alone.  x_out may be x
+ * or y when its rows are contiguous there.  16-byte aligned rows with K % 8 == 0 take vector accesses. */
+VF4_API int vf4_gated_residual_norm(const void* x, int64_t ldx, const void* y, int64_t ldy, int dtype, int64_t M,
+                                    int64_t K, const void* gate, int64_t gate_groups, float residual_scale, int post,
+                                    const void* post_w, const void* post_b, int pre, const void* pre_w,
+                                    const void* pre_b, int param_dtype, float eps, void* x_out, void* h, int h_fp8,
+                                    int64_t ldc, float* scale, int64_t stride_m, int64_t stride_k,
+                                    vf4_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

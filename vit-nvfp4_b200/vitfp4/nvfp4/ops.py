@@ -306,6 +306,47 @@ def gemm_fp8_block(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_sc
     return out
 
 
+NORM_KINDS = {None: 0, "layer": 1, "rms": 2}
+
+
+def gated_residual_norm(x: torch.Tensor, y: torch.Tensor | None, gate: torch.Tensor | None, residual_scale: float,
+                        post: str | None, post_w: torch.Tensor | None, post_b: torch.Tensor | None, pre: str | None,
+                        pre_w: torch.Tensor | None, pre_b: torch.Tensor | None, eps: float, fp8_out: bool):
+    """x' = x + residual_scale * gate * N_post(y), h = N_pre(x') on (M, K) rows (vf4_gated_residual_norm).
+
+    Returns (x' or None without y, h or None without pre, scales or None): h is (M, K) in x's dtype, or E4M3
+    codes with their scales.  The parameters share one dtype, bf16 or fp32."""
+    with _on_device_of(x, y, gate, post_w, post_b, pre_w, pre_b):
+        x2 = _rows_2d(x)
+        y2 = None if y is None else _rows_2d(y)
+        M, K = x2.shape
+        x_out = None if y is None else torch.empty((M, K), dtype=x.dtype, device=x.device)
+        h = scale = None
+        ldc = s_m = s_k = 0
+        if pre is not None and fp8_out:
+            ldc = (K + 15) // 16 * 16
+            h = torch.empty((M, ldc), dtype=torch.float8_e4m3fn, device=x.device)
+            scale = torch.empty(((K + 127) // 128, M), dtype=torch.float32, device=x.device).t()
+            s_m, s_k = 1, M
+        elif pre is not None:
+            h = torch.empty((M, K), dtype=x.dtype, device=x.device)
+        param = next((t for t in (gate, post_w, post_b, pre_w, pre_b) if t is not None), x)
+        groups = 1 if gate is None or gate.dim() == 1 else gate.shape[0]
+        esz = x.element_size()
+        if M == 0:   # empty tensors have no address, which would read as "not given"
+            return x_out, h if h is None else h[:, :K], scale
+        with _Timed(f"gated_norm_{M}x{K}", M * K * (esz * (1 if y is None else 3) +
+                                                   (0 if h is None else 1 if fp8_out else esz))):
+            _lib.call("vf4_gated_residual_norm", x2.data_ptr(), _ld(x2), _ptr(y2), 0 if y2 is None else _ld(y2),
+                      _dtype_code(x), M, K, _ptr(gate), groups, residual_scale, NORM_KINDS[post], _ptr(post_w),
+                      _ptr(post_b), NORM_KINDS[pre], _ptr(pre_w), _ptr(pre_b), _dtype_code(param), eps,
+                      _ptr(x_out), _ptr(h), int(fp8_out), ldc, _ptr(scale), s_m, s_k, _stream())
+        _launched()
+    if h is not None and ldc and ldc != K:
+        h = h[:, :K]
+    return x_out, h, scale
+
+
 def to_blocked(sf: torch.Tensor) -> torch.Tensor:
     """(R, C) E4M3 scales (uint8 or float8_e4m3fn) -> flat 128x4-tiled uint8."""
     _need_cuda(sf)
