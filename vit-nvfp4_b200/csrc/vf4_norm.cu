@@ -9,8 +9,8 @@
 // whose norm comes after the residual only and whose output is NVFP4.  No counterpart in the reference.
 //
 // A row lives in the registers of its threads (8 consecutive columns per thread and step, so that 16 lanes
-// hold a block of 128): the means and variances are taken in two passes over the registers, in fp32, and
-// x' enters the second norm before it is rounded for storage.  Bound by memory.
+// hold a block of 128).  Each thread takes the mean and the squared deviations of its own values, one pass
+// over the threads joins them, all in fp32; x' enters the second norm before it is rounded for storage.
 #include "vf4_fp8_block.cuh"
 #include "vf4_host.h"
 
@@ -20,7 +20,8 @@ enum NormKind : int { kNormNone = 0, kNormLayer = 1, kNormRms = 2 };
 
 struct NormParams {
   const void *x, *y, *gate, *w2, *b2, *w1, *b1;   // w2 / b2: post-norm, w1 / b1: pre-norm; NULL: 1 / 0
-  int64_t M, ldx, ldy, rows_per_gate;
+  int64_t M, ldx, ldy;
+  uint32_t rows_per_gate;
   int K, post, pre, p_f32;     // p_f32: the parameters' type (gate, weights, biases)
   float rs, eps;
   void *x_out, *h;
@@ -55,70 +56,116 @@ VF4_DEV void store_row8(T* p, int nv, const float* v) {
   }
 }
 
-// Sum over the threads of a row: a warp, or a CTA (red: one float per warp, used twice in turn).
+// (count, mean, sum of squared deviations) of two disjoint parts, by the update of Chan, Golub and LeVeque
+// ("Updating formulae and a pairwise algorithm for computing sample variances", 1979): one pass over the
+// threads gives mean and variance without the cancellation of E[v^2] - E[v]^2.
+struct Moments {
+  float n, mean, m2;
+};
+VF4_DEV Moments join(const Moments& a, const Moments& b) {
+  const float n = a.n + b.n, f = n > 0.f ? __fdividef(b.n, n) : 0.f, d = b.mean - a.mean;
+  return {n, fmaf(d, f, a.mean), a.m2 + b.m2 + d * d * a.n * f};
+}
+
+// The row's moments, joined over its threads: a warp, or a CTA (red: its warps' moments; the caller
+// alternates between two such areas, so one barrier per call is enough).  kind RMS: mean 0, m2 the sum of
+// squares.  even: every thread holds as many columns, and the joins need no weights.
 template <int kThreads>
-VF4_DEV float row_sum(float v, float* red) {
+VF4_DEV Moments row_moments(Moments v, int kind, bool even, Moments* red) {
+  if (kind == kNormRms) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    for (int o = 16; o; o >>= 1) v.m2 += __shfl_xor_sync(0xFFFFFFFFu, v.m2, o);
+  } else if (even) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float mean = __shfl_xor_sync(0xFFFFFFFFu, v.mean, o), m2 = __shfl_xor_sync(0xFFFFFFFFu, v.m2, o);
+      const float d = mean - v.mean;
+      v.mean = 0.5f * (v.mean + mean);
+      v.m2 = fmaf(d * d, 0.5f * v.n, v.m2 + m2);
+      v.n *= 2.f;
+    }
+  } else {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      Moments q{__shfl_xor_sync(0xFFFFFFFFu, v.n, o), __shfl_xor_sync(0xFFFFFFFFu, v.mean, o),
+                __shfl_xor_sync(0xFFFFFFFFu, v.m2, o)};
+      // both lanes of a pair join in the same order, so that all lanes end with the same values
+      v = (threadIdx.x & o) ? join(q, v) : join(v, q);
+    }
+  }
   if constexpr (kThreads > 32) {
-    __syncthreads();   // the previous sum has been read
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = 0.f;
+    v = red[0];
 #pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) v += red[i];
+    for (int i = 1; i < kThreads / 32; ++i) {
+      if (kind == kNormRms) v.m2 += red[i].m2;
+      else v = join(v, red[i]);
+    }
   }
   return v;
 }
 
-// N(v) in place over the NV * 8 values of this thread's part of the row.
+// Centres v (LayerNorm) over the NV * 8 values of this thread's part of the row and returns 1 / sqrt(var + eps).
 template <int kThreads, int NV, bool kVec>
-VF4_DEV void normalize(float (*v)[8], const int* nv, int t, int kind, int K, float eps, const void* w, const void* b,
-                       int f32, float* red) {
-  const float inv_k = 1.0f / (float)K;
-  float mean = 0.f;
+VF4_DEV float centre(float (*v)[8], const int* nv, int kind, int K, float eps, Moments* red) {
+  Moments m{0.f, 0.f, 0.f};
   if (kind == kNormLayer) {
     float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+      m.n += (float)nv[j];
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += v[j][i];   // columns past K hold 0
-    mean = row_sum<kThreads>(s, red) * inv_k;
+    }
+    m.mean = m.n > 0.f ? __fdividef(s, m.n) : 0.f;
   }
-  float q = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (kVec ? nv[j] > 0 : i < nv[j]) {
-        v[j][i] -= mean;
-        q = fmaf(v[j][i], v[j][i], q);
+        const float d = v[j][i] - m.mean;
+        m.m2 = fmaf(d, d, m.m2);
       }
-  const float r = rsqrtf(fmaf(row_sum<kThreads>(q, red), inv_k, eps));
+  m = row_moments<kThreads>(m, kind, K % (8 * kThreads) == 0, red);
+  if (kind == kNormLayer) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    if (nv[j] <= 0) continue;
-    const int col = (j * kThreads + t) * 8;
-    float p[8];
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[j][i] *= r;
-    if (w) {
-      param8<kVec>(w, col, f32, nv[j], p);
+      for (int i = 0; i < 8; ++i)
+        if (kVec ? nv[j] > 0 : i < nv[j]) v[j][i] -= m.mean;   // columns past K stay 0
+  }
+  return rsqrtf(__fdividef(m.m2, (float)K) + eps);
+}
+
+// z = v * r * w + b for eight columns.
+template <bool kVec>
+VF4_DEV void affine8(float* v, float r, const void* w, const void* b, int col, int f32, int nv) {
+  float p[8];
+  if (w) {
+    param8<kVec>(w, col, f32, nv, p);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] *= p[i];
-    }
-    if (b) {
-      param8<kVec>(b, col, f32, nv[j], p);
+    for (int i = 0; i < 8; ++i) p[i] *= r;
+  } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] += p[i];
-    }
+    for (int i = 0; i < 8; ++i) p[i] = r;
+  }
+  if (b) {
+    float q[8];
+    param8<kVec>(b, col, f32, nv, q);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], p[i], q[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= p[i];
   }
 }
 
 // kThreads = 32: a warp per row, 8 rows per CTA in turn; else a CTA per row.  kOut: 0 no h, 1 h in T, 2 FP8.
 template <typename T, int kThreads, int NV, bool kVec, int kOut>
-__global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) gated_norm_kernel(const NormParams p) {
-  __shared__ float red[kThreads > 32 ? kThreads / 32 : 1];
+__global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads, kThreads == 32 ? 2 : 1) gated_norm_kernel(const NormParams p) {
+  __shared__ Moments red[2][kThreads > 32 ? kThreads / 32 : 1];
   constexpr int kRows = kThreads == 32 ? 8 : 1;
   const int t = kThreads == 32 ? (threadIdx.x & 31) : threadIdx.x;
   const T *X = static_cast<const T*>(p.x), *Y = static_cast<const T*>(p.y);
@@ -126,31 +173,55 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) gated_norm_ke
   int nv[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) nv[j] = max(0, min(8, p.K - (j * kThreads + t) * 8));
-  for (int64_t row = blockIdx.x * (int64_t)kRows + (kThreads == 32 ? threadIdx.x >> 5 : 0); row < p.M;
-       row += gridDim.x * (int64_t)kRows) {
-    Raw8<T, kVec> xr[NV];
-    float v[NV][8];
+  // kAhead: the next row's x and y are loaded while this one is worked on (one warp per row leaves too few
+  // warps per SM to keep the memory busy otherwise)
+  constexpr bool kAhead = kThreads == 32 && sizeof(T) == 2 && kVec;
+  const int64_t row0 = blockIdx.x * (int64_t)kRows + (kThreads == 32 ? threadIdx.x >> 5 : 0), step = gridDim.x * (int64_t)kRows;
+  Raw8<T, kVec> xr[NV], yr[NV], xn[kAhead ? NV : 1], yn[kAhead ? NV : 1];
+  auto fetch = [&](int64_t row, Raw8<T, kVec>* a, Raw8<T, kVec>* b) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) xr[j].load(X + row * p.ldx + (j * kThreads + t) * 8, nv[j]);
+    for (int j = 0; j < NV; ++j) a[j].load(X + row * p.ldx + (j * kThreads + t) * 8, row < p.M ? nv[j] : 0);
     if (p.y) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) load8<T, kVec>(Y + row * p.ldy + (j * kThreads + t) * 8, nv[j], v[j]);
-      if (p.post != kNormNone) normalize<kThreads, NV, kVec>(v, nv, t, p.post, p.K, p.eps, p.w2, p.b2, p.p_f32, red);
-      const int64_t gate_row = p.gate ? row / p.rows_per_gate * p.K : 0;
+      for (int j = 0; j < NV; ++j) b[j].load(Y + row * p.ldy + (j * kThreads + t) * 8, row < p.M ? nv[j] : 0);
+    }
+  };
+  if (kAhead) fetch(row0, xn, yn);
+  for (int64_t row = row0; row < p.M; row += step) {
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        xr[j] = xn[j];
+        yr[j] = yn[j];
+      }
+      fetch(row + step, xn, yn);
+    } else {
+      fetch(row, xr, yr);
+    }
+    float v[NV][8];
+    if (p.y) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) yr[j].get(v[j]);
+      float r2 = 1.f;
+      if (p.post != kNormNone) r2 = centre<kThreads, NV, kVec>(v, nv, p.post, p.K, p.eps, red[0]);
+      const int64_t gate_row = p.gate ? (int64_t)((uint32_t)row / p.rows_per_gate) * p.K : 0;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (nv[j] <= 0) continue;
         const int col = (j * kThreads + t) * 8;
-        float x[8];
+        float x[8], g[8];
+        if (p.post != kNormNone) affine8<kVec>(v[j], r2, p.w2, p.b2, col, p.p_f32, nv[j]);
         if (p.gate) {
-          float g[8];
           param8<kVec>(p.gate, gate_row + col, p.p_f32, nv[j], g);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[j][i] *= g[i];
+          for (int i = 0; i < 8; ++i) g[i] *= p.rs;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[i] = p.rs;
         }
         xr[j].get(x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[j][i] = fmaf(v[j][i], p.rs, x[i]);
+        for (int i = 0; i < 8; ++i) v[j][i] = fmaf(v[j][i], g[i], x[i]);
         store_row8<T, kVec>(XO + row * p.K + col, nv[j], v[j]);
       }
     } else {
@@ -158,10 +229,11 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) gated_norm_ke
       for (int j = 0; j < NV; ++j) xr[j].get(v[j]);
     }
     if constexpr (kOut != 0) {
-      normalize<kThreads, NV, kVec>(v, nv, t, p.pre, p.K, p.eps, p.w1, p.b1, p.p_f32, red);
+      const float r1 = centre<kThreads, NV, kVec>(v, nv, p.pre, p.K, p.eps, red[1]);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int col = (j * kThreads + t) * 8;
+        if (nv[j] > 0) affine8<kVec>(v[j], r1, p.w1, p.b1, col, p.p_f32, nv[j]);
         if constexpr (kOut == 1) {
           if (nv[j] > 0) store_row8<T, kVec>(H + row * p.K + col, nv[j], v[j]);
         } else {
@@ -172,9 +244,17 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads) gated_norm_ke
 #pragma unroll
           for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
           if (nv[j] > 0) {
-            const Fp8Block q = fp8_block(m);
-            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.h) + row * p.ldc + col) = fp8_encode8(v[j], q);
-            if ((t & 15) == 0) p.scale[row * p.s_m + (col >> 7) * p.s_k] = q.scale;
+            // the quotient as one product: h is itself an fp32 result, off by more than the product's two
+            // roundings (the cast's correctly rounded quotient costs four times as much here)
+            float a = __uint_as_float(m);
+            a = a < 1e-12f ? 1e-12f : a;
+            const float q = __fdividef(448.f, a);
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = e4m3x2(v[j][2 * i] * q, v[j][2 * i + 1] * q);
+            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.h) + row * p.ldc + col) =
+                make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+            if ((t & 15) == 0) p.scale[row * p.s_m + (col >> 7) * p.s_k] = __fdiv_rn(a, 448.f);
           }
         }
       }
@@ -194,14 +274,18 @@ static void launch_norm(const NormParams& p, int out, cudaStream_t s) {
   else gated_norm_kernel<T, kThreads, NV, kVec, 2><<<grid, block, 0, s>>>(p);
 }
 
-// Threads per row and steps of 8 columns per thread by the row's length: a warp up to 1024 columns, then a
-// CTA with as few steps as give each thread at least two 16-byte loads in flight.
+// Threads per row and steps of 8 columns per thread by the rows' number and length.  Up to 1024 columns a warp
+// takes a row, unless there are so few rows that most SMs would get none or one: then, as for longer rows, a
+// CTA takes a row, of the threads that the row fills in one step where that is at most 256.
 template <typename T, bool kVec>
 static void dispatch_norm(const NormParams& p, int out, cudaStream_t s) {
+  const bool few = p.M <= 8 * (int64_t)num_sms();
   if (p.K <= 256) launch_norm<T, 32, 1, kVec>(p, out, s);
-  else if (p.K <= 512) launch_norm<T, 32, 2, kVec>(p, out, s);
-  else if (p.K <= 1024) launch_norm<T, 32, 4, kVec>(p, out, s);
-  else if (p.K <= 2048) launch_norm<T, 128, 2, kVec>(p, out, s);
+  else if (p.K <= 512 && !few) launch_norm<T, 32, 2, kVec>(p, out, s);
+  else if (p.K <= 1024 && !few) launch_norm<T, 32, 4, kVec>(p, out, s);
+  else if (p.K <= 1024) launch_norm<T, 128, 1, kVec>(p, out, s);
+  else if (p.K <= 1280) launch_norm<T, 160, 1, kVec>(p, out, s);
+  else if (p.K <= 2048) launch_norm<T, 256, 1, kVec>(p, out, s);
   else if (p.K <= 4096) launch_norm<T, 256, 2, kVec>(p, out, s);
   else if (p.K <= 8192) launch_norm<T, 256, 4, kVec>(p, out, s);
   else launch_norm<T, 512, 4, kVec>(p, out, s);
@@ -220,6 +304,7 @@ extern "C" int vf4_gated_residual_norm(const void* x, int64_t ldx, const void* y
   const char* me = "vf4_gated_residual_norm";
   if (int st = check_device()) return st;
   if (M < 0 || K <= 0 || ldx < K || (y && ldy < K)) return fail(VF4_ERR_ARG, "%s: bad sizes (M=%lld K=%lld)", me, (long long)M, (long long)K);
+  if (M > INT32_MAX) return fail(VF4_ERR_UNSUPPORTED, "%s: too many rows (%lld)", me, (long long)M);
   if (K > 16384) return fail(VF4_ERR_UNSUPPORTED, "%s: rows of at most 16384 columns (K=%lld)", me, (long long)K);
   if ((dtype != VF4_BF16 && dtype != VF4_F32) || (param_dtype != VF4_BF16 && param_dtype != VF4_F32))
     return fail(VF4_ERR_ARG, "%s: bad dtype", me);
@@ -248,7 +333,7 @@ extern "C" int vf4_gated_residual_norm(const void* x, int64_t ldx, const void* y
   NormParams p{};
   p.x = x; p.y = y; p.gate = gate; p.w2 = post_w; p.b2 = post_b; p.w1 = pre_w; p.b1 = pre_b;
   p.M = M; p.ldx = ldx; p.ldy = ldy;
-  p.rows_per_gate = gate ? M / gate_groups : 1;
+  p.rows_per_gate = gate ? (uint32_t)(M / gate_groups) : 1u;
   p.K = (int)K; p.post = post; p.pre = pre;
   p.p_f32 = param_dtype == VF4_F32;
   p.rs = residual_scale; p.eps = eps;
