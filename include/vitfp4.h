@@ -372,6 +372,24 @@ VF4_API int vf4_gated_residual_norm(const void* x, int64_t ldx, const void* y, i
                                     int64_t ldc, float* scale, int64_t stride_m, int64_t stride_k,
                                     vf4_stream_t stream);
 
+/* Cross attention: queries over keys and values of another length (an encoder's states), bf16 operands, exact
+ * softmax, fp32 accumulation: attention pooling, resamplers, decoders over a ViT's tokens.  No counterpart in the
+ * reference.
+ *   q (B, H, Sq, D), k and v (B, Hkv, Skv, D), out (B, H, Sq, D): element (b, h, s, d) at b * *_b + h * *_h +
+ *   s * *_s + d; strides multiples of 8 elements (0 for a broadcast batch or head), 16-byte aligned pointers;
+ *   H % Hkv == 0, query head h using key head h / (H / Hkv); D % 8 == 0, D <= 128; any Sq and Skv.
+ *   kv_lens: NULL or (B,) int32 device values, keys j >= kv_lens[b] are not used (clamped to 0 .. Skv).
+ *   key_mask: NULL or (B, Skv) bytes with rows mask_b apart, 0 = not used.  Unused keys and values may hold
+ *   anything (NaN included).  A query whose keys are all unused gives 0.
+ * workspace: vf4_cross_attn_workspace_size bytes on the current device (0: none needed), 16-byte aligned, used
+ * until the call's work is done; calls that may overlap need one each.  Deterministic. */
+VF4_API int64_t vf4_cross_attn_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D);
+VF4_API int vf4_cross_attn(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const void* k, int64_t k_b, int64_t k_h,
+                           int64_t k_s, const void* v, int64_t v_b, int64_t v_h, int64_t v_s, int64_t B, int64_t H,
+                           int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D, float scale, const int32_t* kv_lens,
+                           const uint8_t* key_mask, int64_t mask_b, void* out, int64_t o_b, int64_t o_h, int64_t o_s,
+                           void* workspace, int64_t workspace_bytes, vf4_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -38,6 +38,7 @@ int cast_device_error(int clear);
 int gemm_device_error(int clear);
 int attn_device_error(int clear);
 int fp8_device_error(int clear);
+int xattn_device_error(int clear);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -125,13 +125,13 @@ int vf4_version(void) { return 100; }
 const char* vf4_last_error_string(void) { return vf4::g_msg; }
 
 int vf4_device_error(int clear) {
-  cudaError_t e = cudaDeviceSynchronize();
-  if (e != cudaSuccess) return -1;
+  if (cudaDeviceSynchronize() != cudaSuccess) return -1;
   int a = vf4::cast_device_error(clear);
   int b = vf4::gemm_device_error(clear);
   int c = vf4::attn_device_error(clear);
   int d = vf4::fp8_device_error(clear);
-  return a ? a : (b ? b : (c ? c : d));
+  int e = vf4::xattn_device_error(clear);
+  return a ? a : (b ? b : (c ? c : (d ? d : e)));
 }
 
 }  // extern "C"

@@ -1,0 +1,861 @@
+// Cross attention: queries of one length over keys and values of another (an encoder's states), with
+// shared key / value heads, a key count per image and a mask of keys.
+//
+//   out[b, h, i] = sum_j p_j v[b, h / G, j] / sum_j p_j,   p_j = exp(scale q[b, h, i] . k[b, h / G, j])
+//
+// over the keys j that image b keeps (j < kv_lens[b] and key_mask[b, j]); a row that keeps none is 0.
+// Masked keys and values are never used, whatever they hold (NaN and infinities included).  No
+// counterpart in the reference, whose attention is self attention of a ViT (nvfp4/attention.py:53-86).
+//
+// The G query heads that share a key / value head and their Sq queries are the rows of one problem:
+// R = G * Sq rows against the same keys, so a decoder's single token still reads each key once.
+//
+//   R > 4   tcgen05: 128-row tiles, 128 keys at a time, online softmax (xattn_tc_kernel)
+//   R <= 4  plain FMAs: the keys stream through registers (xattn_rows_kernel)
+//
+// With fewer tiles than SMs the keys are cut into chunks: each CTA leaves its rows' maxima, sums and
+// unnormalised outputs in the workspace and xattn_join_kernel adds them up in order.
+#include <string.h>
+
+#include "vf4_common.cuh"
+#include "vf4_host.h"
+
+namespace vf4 {
+
+static __device__ int g_xattn_err;
+
+int xattn_device_error(int clear) {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, g_xattn_err, sizeof(int));
+  if (clear) {
+    int z = 0;
+    cudaMemcpyToSymbol(g_xattn_err, &z, sizeof(int));
+  }
+  return v;
+}
+
+struct XParams {
+  const __nv_bfloat16 *q, *k, *v;
+  int64_t qb, qh, qs, kb, kh, ks, vb, vh, vs;   // element strides
+  __nv_bfloat16* out;
+  int64_t ob, oh, os;
+  const int32_t* lens;     // (B,) or NULL
+  const uint8_t* mask;     // (B, Skv) bytes, non-zero = keep, or NULL; rows mask_b apart
+  int64_t mask_b;
+  int B, Hkv, G, Sq, Skv, D;
+  int R;                   // G * Sq
+  int negate;              // scale < 0: the queries are negated and c is its magnitude
+  float c;                 // |scale| * log2(e)
+  int chunk, chunks;       // keys per CTA and CTAs per row tile; chunks > 1: partial results to the workspace
+  float* part_o;           // [B * Hkv][chunks][R][D]
+  float2* part_ml;         // [B * Hkv][chunks][R]: {maximum of the scores, sum of the weights}
+  int tiles;               // 256-row tiles (tcgen05 kernel)
+};
+
+VF4_DEV int keys_of(const XParams& p, int b) {
+  return p.lens ? max(0, min(p.lens[b], p.Skv)) : p.Skv;
+}
+
+// Row r of head group hk: query element pointer offsets.
+VF4_DEV int64_t q_offset(const XParams& p, int b, int hk, int r) {
+  const int g = r / p.Sq, i = r - g * p.Sq;
+  return b * p.qb + (int64_t)(hk * p.G + g) * p.qh + i * p.qs;
+}
+VF4_DEV int64_t o_offset(const XParams& p, int b, int hk, int r) {
+  const int g = r / p.Sq, i = r - g * p.Sq;
+  return b * p.ob + (int64_t)(hk * p.G + g) * p.oh + i * p.os;
+}
+
+// ---------------------------------------------------------------------------------------
+// Up to 4 rows.  LPK lanes hold one key's D <= 8 LPK elements (16 bytes each), so a warp reads 32 / LPK keys
+// per load; every group of lanes keeps its own maximum, sum and output for the keys it sees, taking kU of
+// them at a time (loads of the next kU in flight), and the groups are joined at the end: lanes by shuffles,
+// warps through shared memory.  Bound by memory: each key and value is read once; 2 R FMAs per element.
+// ---------------------------------------------------------------------------------------
+constexpr int kRowWarps = 4;
+
+template <int LPK, int R>
+__global__ void __launch_bounds__(kRowWarps * 32) xattn_rows_kernel(const XParams p) {
+  constexpr int KPW = 32 / LPK, kU = 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int grp = lane / LPK, el = (lane % LPK) * 8;     // key group and first element of this lane
+  const int chunk = blockIdx.x % p.chunks, item = blockIdx.x / p.chunks;
+  const int b = item / p.Hkv, hk = item - b * p.Hkv;
+  const bool on = el < p.D;
+  const int k0 = chunk * p.chunk, k1 = min(keys_of(p, b), k0 + p.chunk);
+
+  float q[R][8], acc[R][8], m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (on && r < p.R) w = __ldg(reinterpret_cast<const uint4*>(p.q + q_offset(p, b, hk, r) + el));
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    const float f = p.negate ? -p.c : p.c;   // scores come out in units of log2
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      q[r][i] = __uint_as_float((i & 1) ? (u[i / 2] & 0xFFFF0000u) : (u[i / 2] << 16)) * f;
+      acc[r][i] = 0.f;
+    }
+  }
+  const __nv_bfloat16* kp = p.k + b * p.kb + hk * p.kh + el;
+  const __nv_bfloat16* vp = p.v + b * p.vb + hk * p.vh + el;
+  const uint8_t* mp = p.mask ? p.mask + b * p.mask_b : nullptr;
+  uint4 kw[kU], vw[kU];
+  bool keep[kU];
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int j = base + u * KPW + grp;
+      keep[u] = j < k1 && (!mp || mp[j] != 0);
+      kw[u] = vw[u] = make_uint4(0, 0, 0, 0);
+      if (keep[u] && on) {
+        kw[u] = __ldg(reinterpret_cast<const uint4*>(kp + (int64_t)j * p.ks));
+        vw[u] = __ldg(reinterpret_cast<const uint4*>(vp + (int64_t)j * p.vs));
+      }
+    }
+  };
+  constexpr int kStep = kRowWarps * KPW * kU;
+  const int first = k0 + warp * KPW * kU;
+  if (first < k1) fetch(first);
+  for (int base = first; base < k1; base += kStep) {
+    uint4 kc[kU], vc[kU];
+    bool kept[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      kc[u] = kw[u];
+      vc[u] = vw[u];
+      kept[u] = keep[u];
+    }
+    if (base + kStep < k1) fetch(base + kStep);
+    float s[kU][R];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const uint32_t w[4] = {kc[u].x, kc[u].y, kc[u].z, kc[u].w};
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[u][r] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = __uint_as_float((i & 1) ? (w[i / 2] & 0xFFFF0000u) : (w[i / 2] << 16));
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[u][r] = fmaf(q[r][i], x, s[u][r]);
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < LPK; o <<= 1)
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[u][r] += __shfl_xor_sync(0xFFFFFFFFu, s[u][r], o);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float mx = m[r];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        if (!kept[u]) s[u][r] = -INFINITY;
+        mx = fmaxf(mx, s[u][r]);
+      }
+      const float ms = mx == -INFINITY ? 0.f : mx;   // nothing kept so far: weights 2^-inf = 0
+      const float f = ex2_approx(m[r] - ms);
+      m[r] = mx;
+      l[r] *= f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[r][i] *= f;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        s[u][r] = ex2_approx(s[u][r] - ms);
+        l[r] += s[u][r];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const uint32_t w[4] = {vc[u].x, vc[u].y, vc[u].z, vc[u].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = __uint_as_float((i & 1) ? (w[i / 2] & 0xFFFF0000u) : (w[i / 2] << 16));
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[r][i] = fmaf(s[u][r], x, acc[r][i]);
+      }
+    }
+  }
+  // join the key groups of the warp, then the warps
+  __shared__ float red_o[kRowWarps][R][LPK * 8];
+  __shared__ float2 red_ml[kRowWarps][R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int o = LPK; o < 32; o <<= 1) {
+      const float m2 = __shfl_xor_sync(0xFFFFFFFFu, m[r], o), l2 = __shfl_xor_sync(0xFFFFFFFFu, l[r], o);
+      const float mx = fmaxf(m[r], m2), ms = mx == -INFINITY ? 0.f : mx;
+      const float f1 = ex2_approx(m[r] - ms), f2 = ex2_approx(m2 - ms);
+      // the same order of the two summands in both lanes, so that they agree to the last bit
+      l[r] = (lane & o) ? fmaf(l2, f2, l[r] * f1) : fmaf(l[r], f1, l2 * f2);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float a2 = __shfl_xor_sync(0xFFFFFFFFu, acc[r][i], o);
+        acc[r][i] = (lane & o) ? fmaf(a2, f2, acc[r][i] * f1) : fmaf(acc[r][i], f1, a2 * f2);
+      }
+      m[r] = mx;
+    }
+    if (grp == 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) red_o[warp][r][el + i] = acc[r][i];
+      if (lane == 0) red_ml[warp][r] = make_float2(m[r], l[r]);
+    }
+  }
+  __syncthreads();
+  for (int t = threadIdx.x; t < R * LPK; t += kRowWarps * 32) {
+    const int r = t / LPK, e = (t - r * LPK) * 8;
+    if (r >= p.R || e >= p.D) continue;
+    float mx = -INFINITY, ls = 0.f, o[8];
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) mx = fmaxf(mx, red_ml[w][r].x);
+    const float ms = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+      const float f = ex2_approx(red_ml[w][r].x - ms);
+      ls = fmaf(red_ml[w][r].y, f, ls);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = fmaf(red_o[w][r][e + i], f, o[i]);
+    }
+    if (p.chunks > 1) {
+      const int64_t row = ((int64_t)item * p.chunks + chunk) * p.R + r;
+      float4* dst = reinterpret_cast<float4*>(p.part_o + row * p.D + e);
+      dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+      dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+      if (e == 0) p.part_ml[row] = make_float2(mx, ls);
+    } else {
+      const float f = ls > 0.f ? __fdividef(1.f, ls) : (ls == 0.f ? 0.f : ls);   // nothing kept: 0; NaN stays
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = bf16x2_round(f32x2_pack(o[2 * i] * f, o[2 * i + 1] * f));
+      *reinterpret_cast<uint4*>(p.out + o_offset(p, b, hk, r) + e) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// One warp per row: the chunks' partial results in order.  Maxima are in units of log2.
+__global__ void __launch_bounds__(128) xattn_join_kernel(const XParams p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = blockIdx.x * 4ll + (threadIdx.x >> 5);
+  if (row >= (int64_t)p.B * p.Hkv * p.R) return;
+  const int item = (int)(row / p.R), r = (int)(row - (int64_t)item * p.R);
+  const int b = item / p.Hkv, hk = item - b * p.Hkv;
+  const int n = min(p.chunks, (keys_of(p, b) + p.chunk - 1) / p.chunk);   // chunks that hold keys
+  const int64_t at = (int64_t)item * p.chunks * p.R + r;
+  float mx = -INFINITY;
+  for (int c = lane; c < n; c += 32) mx = fmaxf(mx, p.part_ml[at + (int64_t)c * p.R].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+  const float ms = mx == -INFINITY ? 0.f : mx;
+  float ls = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  const int e = lane * 4;
+  for (int c = 0; c < n; ++c) {
+    const float2 ml = p.part_ml[at + (int64_t)c * p.R];
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;   // a chunk without kept keys
+    const float f = ex2_approx(ml.x - ms);
+    ls = fmaf(ml.y, f, ls);
+    if (e < p.D) {
+      const float4 o = *reinterpret_cast<const float4*>(p.part_o + (at + (int64_t)c * p.R) * p.D + e);
+      acc[0] = fmaf(o.x, f, acc[0]);
+      acc[1] = fmaf(o.y, f, acc[1]);
+      acc[2] = fmaf(o.z, f, acc[2]);
+      acc[3] = fmaf(o.w, f, acc[3]);
+    }
+  }
+  if (e < p.D) {
+    const float f = ls > 0.f ? __fdividef(1.f, ls) : (ls == 0.f ? 0.f : ls);
+    *reinterpret_cast<uint2*>(p.out + o_offset(p, b, hk, r) + e) =
+        make_uint2(bf16x2_round(f32x2_pack(acc[0] * f, acc[1] * f)), bf16x2_round(f32x2_pack(acc[2] * f, acc[3] * f)));
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// More rows: tcgen05.  A CTA takes up to 256 rows as two slots of 128 and runs "steps", one slot's 128
+// rows against one tile of 128 keys:
+//   two slots of rows (more than 128):  step i = slot i % 2, key tile i / 2 -- both slots use each tile
+//   one slot of rows:                   step i = slot i % 2, key tile i     -- the slots share the rows and
+//                                       take turns at the key tiles; joined at the end
+// so that one slot's softmax runs while the tensor core works for the other.  Per step:
+//   S = Q K^T (128 x 128, fp32, tensor memory) -> softmax warps: maximum, P = 2^(c s - c m) in bf16 over
+//   S's own columns in tensor memory -> O += P V (accumulated in tensor memory)
+// The running maximum m is only moved (and O and the sums rescaled) when it grows by more than 2^8: P stays
+// below 256, which bf16 and the fp32 sums hold as well as P <= 1.
+//
+//   warp 0      TMA of K and V tiles (128-byte swizzle, panels of 64 elements)
+//   warp 1      TMEM allocation, MMAs
+//   warp 2      masks: clears the masked rows of each V tile in shared memory, so that no NaN of theirs meets
+//               a weight of 0
+//   warps 4-7, 8-11  softmax of slot 0 and 1, a thread per row (holds the 128 scores in registers)
+// ---------------------------------------------------------------------------------------
+template <int DP>
+struct XCfg {
+  static constexpr int PANELS = DP / 64, PANEL = 128 * 128;    // bytes of 128 rows x 64 elements
+  static constexpr int TILE = PANELS * PANEL;
+  static constexpr int KV = DP == 64 ? 4 : 2;                  // tiles in flight of K and of V each
+  static constexpr int V_OFF = 0, K_OFF = KV * TILE, Q_OFF = 2 * KV * TILE;
+  static constexpr int RED_OFF = Q_OFF + 2 * TILE;             // {maximum, sum} per slot and row
+  static constexpr int BAR_OFF = RED_OFF + 2 * 128 * 8;
+  static constexpr int NBAR = 5 * KV + 1 + 2 * 3;
+  static constexpr int SMEM = 1024 + BAR_OFF + 8 * NBAR + 16;
+  static constexpr int THREADS = 384;
+  static constexpr int kLaunchRegs = 168, kControlRegs = 40, kSoftRegs = 232;
+  static_assert(128 * kControlRegs + 256 * kSoftRegs <= THREADS * kLaunchRegs, "register split");
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+  static_assert(2 * 128 * DP * 4 <= 2 * KV * TILE, "the joined outputs reuse the K and V tiles");
+};
+
+VF4_DEV void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+template <int DP>
+__global__ void __launch_bounds__(XCfg<DP>::THREADS, 1)
+    xattn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const int k_bm,
+                    const int k_hm, const int v_bm, const int v_hm, const XParams p) {
+  using C = XCfg<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw0 = smem_u32(smem_raw);
+  const uint32_t base = (raw0 + 1023u) & ~1023u;
+  uint8_t* gb = smem_raw + (base - raw0);
+  const uint32_t bar = base + C::BAR_OFF;
+  auto k_full = [&](int i) { return bar + 8u * i; };
+  auto k_free = [&](int i) { return bar + 8u * (C::KV + i); };
+  auto v_full = [&](int i) { return bar + 8u * (2 * C::KV + i); };
+  auto v_free = [&](int i) { return bar + 8u * (3 * C::KV + i); };
+  auto v_clean = [&](int i) { return bar + 8u * (4 * C::KV + i); };   // masked rows cleared
+  const uint32_t q_full = bar + 8u * (5 * C::KV);
+  auto s_full = [&](int s) { return q_full + 8u + 24u * s; };
+  auto p_full = [&](int s) { return q_full + 16u + 24u * s; };
+  auto o_full = [&](int s) { return q_full + 24u + 24u * s; };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + C::BAR_OFF + 8 * C::NBAR);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* err = &g_xattn_err;
+
+  // this CTA's rows and keys
+  const int chunk = blockIdx.x % p.chunks, tile = blockIdx.x / p.chunks % p.tiles, item = blockIdx.x / p.chunks / p.tiles;
+  const int b = item / p.Hkv, hk = item - b * p.Hkv;
+  const int row0 = tile * 256, rows = min(256, p.R - row0);
+  const bool two = rows > 128;                     // two slots of rows
+  const int k0 = chunk * p.chunk, k1 = min(keys_of(p, b), k0 + p.chunk);
+  const int tiles = k1 > k0 ? (k1 - k0 + 127) / 128 : 0;
+  const int steps = two ? 2 * tiles : tiles;
+  const bool masked = p.mask != nullptr || p.lens != nullptr;
+
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < C::KV; ++i) {
+      mbar_init(k_full(i), 1);
+      mbar_init(k_free(i), 1);
+      mbar_init(v_full(i), 1);
+      mbar_init(v_free(i), 1);
+      mbar_init(v_clean(i), 1);
+    }
+    mbar_init(q_full, two ? 256 : 128);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(s_full(s), 1);
+      mbar_init(p_full(s), 4);
+      mbar_init(o_full(s), 1);
+    }
+    fence_mbar_init();
+    tma_prefetch(&tmK);
+    tma_prefetch(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  fence_async_shared();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kControlRegs));
+    const bool elected = elect_one();
+    if (warp == 0) {
+      // K of tile t is needed by the first step that scores it, V one round of steps later: K0, (K1), V0, K1 / K2, ...
+      const int ahead = two ? 1 : 2;
+      auto load = [&](const CUtensorMap* m, uint32_t dst, uint32_t full, int t, int hm, int bm) {
+        if (elected) {
+          mbar_arrive_expect_tx(full, C::TILE);
+#pragma unroll
+          for (int c = 0; c < C::PANELS; ++c)
+            tma_load_4d(dst + c * C::PANEL, m, c * 64, k0 + t * 128, hk * hm, b * bm, full);
+        }
+        __syncwarp();
+      };
+      bool ok = true;
+      for (int i = -ahead; i < tiles && ok; ++i) {
+        if (i >= 0) {
+          const int s = i % C::KV, use = i / C::KV;
+          ok = __all_sync(0xFFFFFFFFu, use == 0 || mbar_wait(v_free(s), (uint32_t)(use - 1) & 1u, err, kDevErrTimeoutEmpty));
+          if (ok) load(&tmV, base + C::V_OFF + s * C::TILE, v_full(s), i, v_hm, v_bm);
+        }
+        const int t = i + ahead;
+        if (t < tiles && ok) {
+          const int s = t % C::KV, use = t / C::KV;
+          ok = __all_sync(0xFFFFFFFFu, use == 0 || mbar_wait(k_free(s), (uint32_t)(use - 1) & 1u, err, kDevErrTimeoutEmpty));
+          if (ok) load(&tmK, base + C::K_OFF + s * C::TILE, k_full(s), t, k_hm, k_bm);
+        }
+      }
+      // no copy may still be writing shared memory when the CTA goes on (to join, or to exit)
+      if (ok)
+        for (int t = max(0, tiles - C::KV); t < tiles; ++t) {
+          mbar_wait(k_full(t % C::KV), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull);
+          mbar_wait(v_full(t % C::KV), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull);
+        }
+    } else if (warp == 1) {
+      const int kd = (p.D + 15) / 16;
+      const uint32_t id_s = idesc_bf16(128, false), id_o = idesc_bf16((uint32_t)kd * 16u, true);
+      bool ok = steps == 0 || __all_sync(0xFFFFFFFFu, mbar_wait(q_full, 0, err, kDevErrTimeoutFull));
+      const uint64_t qd0 = smem_desc(base + C::Q_OFF, 16, 1024, 2), kd0 = smem_desc(base + C::K_OFF, 16, 1024, 2);
+      const uint64_t vd0 = smem_desc(base + C::V_OFF, C::PANEL, 1024, 2);
+      auto score = [&](int i) {   // S of step i
+        const int s = i & 1, t = two ? i >> 1 : i, st = t % C::KV;
+        if (!(two && s == 1))     // the second slot of a tile finds it loaded
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(k_full(st), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull));
+        if (!ok) return;
+        tc_fence_after();
+        if (elected) {
+          const uint64_t qd = qd0 + (uint32_t)((two ? s : 0) * (C::TILE >> 4)), kk0 = kd0 + (uint32_t)(st * (C::TILE >> 4));
+          for (int kk = 0; kk < kd; ++kk) {
+            const uint32_t off = (uint32_t)((kk >> 2) * (C::PANEL >> 4) + (kk & 3) * 2);
+            mma_f16(tmem + 128u * s, qd + off, kk0 + off, id_s, kk > 0 ? 1u : 0u);
+          }
+          tc_commit(s_full(s));
+          if (!two || s == 1) tc_commit(k_free(st));
+        }
+        __syncwarp();
+      };
+      if (ok && steps > 0) score(0);
+      if (ok && steps > 1) score(1);
+      for (int i = 0; i < steps && ok; ++i) {
+        const int s = i & 1, t = two ? i >> 1 : i, st = t % C::KV;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(masked ? v_clean(st) : v_full(st), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull) &&
+                                         mbar_wait(p_full(s), (uint32_t)(i >> 1) & 1u, err, kDevErrTimeoutTmem));
+        if (!ok) break;
+        tc_fence_after();
+        if (elected) {
+          const uint64_t vd = vd0 + (uint32_t)(st * (C::TILE >> 4));
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            mma_f16_tmem_a(tmem + 256u + 128u * s, tmem + 128u * s + 8u * kk, vd + (uint32_t)(kk * (2048 >> 4)), id_o,
+                           (i >= 2 || kk > 0) ? 1u : 0u);
+          tc_commit(o_full(s));
+          if (!two || s == 1) tc_commit(v_free(st));
+        }
+        __syncwarp();
+        if (i + 2 < steps) score(i + 2);
+      }
+      // the tensor core must be done with shared memory before it is reused
+      if (ok)
+        for (int s = 0; s < 2; ++s) {
+          const int n = (steps + 1 - s) / 2;   // steps of slot s
+          if (n > 0) mbar_wait(o_full(s), (uint32_t)(n - 1) & 1u, err, kDevErrTimeoutDrain);
+        }
+    } else if (warp == 2 && masked) {
+      const uint8_t* mp = p.mask ? p.mask + b * p.mask_b : nullptr;
+      for (int t = 0; t < tiles; ++t) {
+        const int st = t % C::KV, j0 = k0 + t * 128;
+        bool keep[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int j = j0 + 32 * w + lane;
+          keep[w] = j < k1 && (!mp || mp[j] != 0);
+        }
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(v_full(st), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull))) break;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t drop = ~__ballot_sync(0xFFFFFFFFu, keep[w]);
+          // four rows at a time, eight lanes of 16 bytes each
+          while (drop) {
+            uint32_t mine = 0;
+            bool any = false;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              if (drop) {
+                const uint32_t r = (uint32_t)__ffs((int)drop) - 1u;
+                drop &= drop - 1u;
+                if ((lane >> 3) == x) {
+                  mine = r;
+                  any = true;
+                }
+              }
+            }
+            if (any)
+#pragma unroll
+              for (int c = 0; c < C::PANELS; ++c)
+                *reinterpret_cast<uint4*>(gb + C::V_OFF + st * C::TILE + c * C::PANEL + (32 * w + mine) * 128 + (lane & 7) * 16) =
+                    make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_clean(st));
+      }
+    }
+    __syncwarp();
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
+    const int s = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;    // slot, row of the slot
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lane_base + 128u * s, t_o = tmem + lane_base + 256u + 128u * s;
+    const int row = row0 + (two ? s * 128 : 0) + r;
+    const bool valid = row < p.R;
+    const bool act = (two ? s * 128 : 0) + (warp & 3) * 32 < rows;   // any valid row in this warp
+    // Q: each thread copies its own row (rows past the last as zeros)
+    if (two || s == 0) {
+      const __nv_bfloat16* src = p.q + (valid ? q_offset(p, b, hk, row) : 0);
+      uint8_t* dst = gb + C::Q_OFF + s * C::TILE + r * 128;
+      const int pieces = (p.D + 15) / 16 * 2;
+      for (int j = 0; j < pieces; ++j) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (valid && j * 8 < p.D) w = __ldg(reinterpret_cast<const uint4*>(src) + j);
+        if (p.negate) {
+          w.x ^= 0x80008000u;
+          w.y ^= 0x80008000u;
+          w.z ^= 0x80008000u;
+          w.w ^= 0x80008000u;
+        }
+        *reinterpret_cast<uint4*>(dst + (j >> 3) * C::PANEL + (((j & 7) ^ (r & 7)) << 4)) = w;
+      }
+      fence_async_shared();
+      mbar_arrive(q_full);
+    }
+    const int n = (steps + 1 - s) / 2;   // steps of this slot
+    const uint8_t* mp = p.mask ? p.mask + b * p.mask_b : nullptr;
+    float m = -INFINITY, l = 0.f;
+    const float grow = p.c > 0.f ? 8.f / p.c : INFINITY;
+    bool ok = true;
+    for (int i = 0; i < n && ok; ++i) {
+      const int j0 = k0 + (two ? i : 2 * i + s) * 128;
+      // which of the tile's keys count, 32 per word (the same for every row)
+      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+      const bool part = mp || j0 + 128 > k1;
+      if (part) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int j = j0 + 32 * w + lane;
+          bits[w] = __ballot_sync(0xFFFFFFFFu, j < k1 && (!mp || mp[j] != 0));
+        }
+      }
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(s_full(s), (uint32_t)i & 1u, err, kDevErrTimeoutTmem));
+      if (!ok) break;
+      tc_fence_after();
+      if (act) {
+        uint32_t v[128];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) tmem_ld_32x32b_x32(t_s + 32 * w, v + 32 * w);
+        tmem_wait_ld();
+#pragma unroll
+        for (int w = 0; w < 8; ++w) reg_fence16(v + 16 * w);
+        if (part) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(bits[w] >> e & 1u)) v[32 * w + e] = 0xFF800000u;   // -inf, also in place of a NaN
+        }
+        float mx[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          mx[w] = __uint_as_float(v[32 * w]);
+#pragma unroll
+          for (int e = 1; e < 31; e += 2) mx[w] = max3f(mx[w], __uint_as_float(v[32 * w + e]), __uint_as_float(v[32 * w + e + 1]));
+          mx[w] = fmaxf(mx[w], __uint_as_float(v[32 * w + 31]));
+        }
+        const float top = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]);
+        if (i == 0) {
+          m = top;
+        } else {
+          const bool up = top > m + grow || (m == -INFINITY && top > m);
+          if (__any_sync(0xFFFFFFFFu, up)) {
+            // O holds the steps before this one once their products are done
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full(s), (uint32_t)(i - 1) & 1u, err, kDevErrTimeoutTmem));
+            if (!ok) break;
+            tc_fence_after();
+            const float f = !up ? 1.f : ex2_approx((m - top) * p.c);   // m = -inf: 0 (nothing was added yet)
+            if (up) m = top;
+            l *= f;
+            for (int c0 = 0; c0 < p.D; c0 += 16) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(t_o + c0, o);
+              tmem_wait_ld();
+              reg_fence16(o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st_32x32b_x16(t_o + c0, o);
+            }
+          }
+        }
+        const float nm = m == -INFINITY ? 0.f : -m * p.c;
+        const unsigned long long c2 = f32x2_pack(p.c, p.c), nm2 = f32x2_pack(nm, nm);
+        unsigned long long l2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x0, x1;
+            f32x2_unpack(fma_f32x2(f32x2_pack(__uint_as_float(v[32 * w + 2 * e]), __uint_as_float(v[32 * w + 2 * e + 1])), c2, nm2),
+                         &x0, &x1);
+            const unsigned long long pr = f32x2_pack(ex2_approx(x0), ex2_approx(x1));
+            l2[e & 1] = add_f32x2(l2[e & 1], pr);
+            pk[e] = bf16x2_round(pr);
+          }
+          tmem_st_32x32b_x16(t_s + 16 * w, pk);   // P over S: its 128 columns are in this thread's registers
+        }
+        float a0, a1, a2, a3;
+        f32x2_unpack(l2[0], &a0, &a1);
+        f32x2_unpack(l2[1], &a2, &a3);
+        l += (a0 + a1) + (a2 + a3);
+        tmem_wait_st();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full(s));
+    }
+    // the slot's output is complete when its last product is
+    if (n > 0 && ok) ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full(s), (uint32_t)(n - 1) & 1u, err, kDevErrTimeoutTmem));
+    tc_fence_after();
+    const int64_t part_row = ((int64_t)item * p.chunks + chunk) * p.R + row;
+    if (two) {
+      if (act && ok) {
+        const float f = p.chunks > 1 ? 1.f : l > 0.f ? __fdividef(1.f, l) : (l == 0.f ? 0.f : l);
+        for (int c0 = 0; c0 < p.D; c0 += 8) {
+          uint32_t o[8];
+          tmem_ld_32x32b_x8(t_o + c0, o);
+          tmem_wait_ld();
+          asm volatile("" : "+r"(o[0]), "+r"(o[1]), "+r"(o[2]), "+r"(o[3]), "+r"(o[4]), "+r"(o[5]), "+r"(o[6]), "+r"(o[7]));
+          if (n == 0)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = 0u;
+          if (!valid) continue;
+          if (p.chunks > 1) {
+            uint4* dst = reinterpret_cast<uint4*>(p.part_o + part_row * p.D + c0);
+            dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+          } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = l == 0.f ? 0u : bf16x2_round(f32x2_pack(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f));
+            *reinterpret_cast<uint4*>(p.out + o_offset(p, b, hk, row) + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        if (valid && p.chunks > 1) p.part_ml[part_row] = make_float2(m == -INFINITY ? m : m * p.c, l);
+      }
+    } else {
+      // both slots hold part of the same rows: into shared memory (the K and V tiles are done with)
+      float* so = reinterpret_cast<float*>(gb) + s * 128 * DP;
+      float2* ml = reinterpret_cast<float2*>(gb + C::RED_OFF) + s * 128;
+      named_bar_sync(1, 256);   // both slots' products are complete: nothing reads the tiles any more
+      if (act && ok) {
+        for (int c0 = 0; c0 < p.D; c0 += 8) {
+          uint32_t o[8];
+          tmem_ld_32x32b_x8(t_o + c0, o);
+          tmem_wait_ld();
+          asm volatile("" : "+r"(o[0]), "+r"(o[1]), "+r"(o[2]), "+r"(o[3]), "+r"(o[4]), "+r"(o[5]), "+r"(o[6]), "+r"(o[7]));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) so[(c0 + e) * 128 + r] = n == 0 ? 0.f : __uint_as_float(o[e]);
+        }
+        ml[r] = make_float2(m == -INFINITY ? m : m * p.c, l);
+      }
+      named_bar_sync(1, 256);
+      const float2 *ml0 = reinterpret_cast<const float2*>(gb + C::RED_OFF), *ml1 = ml0 + 128;
+      const float* so0 = reinterpret_cast<const float*>(gb);
+      const int et = threadIdx.x - 128, er = et & 127;
+      if (er < rows && ok) {
+        const float2 x = ml0[er], y = ml1[er];
+        const float mx = fmaxf(x.x, y.x), ms = mx == -INFINITY ? 0.f : mx;
+        const float f0 = ex2_approx(x.x - ms), f1 = ex2_approx(y.x - ms);
+        const float ls = fmaf(x.y, f0, y.y * f1);
+        const float f = p.chunks > 1 ? 1.f : ls > 0.f ? __fdividef(1.f, ls) : (ls == 0.f ? 0.f : ls);
+        const int64_t prow = ((int64_t)item * p.chunks + chunk) * p.R + row0 + er;
+        for (int c0 = (et >> 7) * 8; c0 < p.D; c0 += 16) {
+          float o[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int at = (c0 + e) * 128 + er;
+            // a slot without kept keys holds 0 * f
+            o[e] = (fmaf(so0[at], f0, so0[128 * DP + at] * f1)) * f;
+          }
+          if (p.chunks > 1) {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + prow * p.D + c0);
+            dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+            dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+          } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = bf16x2_round(f32x2_pack(o[2 * e], o[2 * e + 1]));
+            *reinterpret_cast<uint4*>(p.out + o_offset(p, b, hk, row0 + er) + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        if (p.chunks > 1 && et < 128) p.part_ml[prow] = make_float2(mx, ls);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// K or V as (elements, keys, heads, images); a dimension of stride 0 (or of one entry) is given extent 1 and its
+// coordinate multiplied by 0.
+static int make_kv_map(CUtensorMap* m, const void* ptr, const XParams& p, int64_t sb, int64_t sh, int64_t ss, int* bm, int* hm) {
+  EncodeTiledFn enc = encode_tiled();
+  if (!enc) return fail(VF4_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  *bm = p.B > 1 && sb != 0;
+  *hm = p.Hkv > 1 && sh != 0;
+  const bool one_key = p.Skv == 1;
+  cuuint64_t dims[4] = {(cuuint64_t)p.D, (cuuint64_t)p.Skv, (cuuint64_t)(*hm ? p.Hkv : 1), (cuuint64_t)(*bm ? p.B : 1)};
+  cuuint64_t strides[3] = {(cuuint64_t)(one_key ? 16 : ss * 2), (cuuint64_t)(*hm ? sh * 2 : 16), (cuuint64_t)(*bm ? sb * 2 : 16)};
+  cuuint32_t box[4] = {64u, 128u, 1u, 1u};
+  cuuint32_t es[4] = {1u, 1u, 1u, 1u};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, strides, box, es,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(VF4_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return VF4_OK;
+}
+
+// Rows that the plain kernel takes: it reads each key once for all of them but pays 4 FMAs per element and row
+// pair; from 5 rows on the tensor core is faster.
+constexpr int kPlainRows = 4;
+
+// How many keys a CTA takes, and how many CTAs share a row tile (1: no workspace).
+static void plan_chunks(int64_t B, int64_t Hkv, int64_t R, int64_t Skv, int sms, int* chunk, int* chunks) {
+  const int64_t items = B * Hkv * (R <= kPlainRows ? 1 : (R + 255) / 256);
+  // plain kernel: 8 CTAs of 128 threads per SM, at least 256 keys each; tcgen05: one CTA per SM, at least 512
+  const int64_t want = R <= kPlainRows ? (int64_t)sms * 8 : sms, least = R <= kPlainRows ? 256 : 512;
+  int64_t n = want / items;
+  if (n > (Skv + least - 1) / least) n = (Skv + least - 1) / least;
+  if (n < 1) n = 1;
+  int64_t c = ((Skv + n - 1) / n + 127) / 128 * 128;
+  if (c < 128) c = 128;
+  *chunk = (int)c;
+  *chunks = (int)((Skv + c - 1) / c);
+  if (*chunks < 1) *chunks = 1;
+}
+
+template <int DP>
+static int launch_tc(const XParams& p, cudaStream_t s) {
+  using C = XCfg<DP>;
+  CUtensorMap tk, tv;
+  int kbm, khm, vbm, vhm;
+  if (int st = make_kv_map(&tk, p.k, p, p.kb, p.kh, p.ks, &kbm, &khm)) return st;
+  if (int st = make_kv_map(&tv, p.v, p, p.vb, p.vh, p.vs, &vbm, &vhm)) return st;
+  auto kern = xattn_tc_kernel<DP>;
+  if (int st = smem_optin(kern, C::SMEM)) return st;
+  static const int regs = [] {   // the register split of the kernel relies on what its launch allocates
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, xattn_tc_kernel<DP>) == cudaSuccess ? a.numRegs : 0;
+  }();
+  if (regs != C::kLaunchRegs) return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: built with %d registers", regs);
+  const int64_t grid = (int64_t)p.B * p.Hkv * p.tiles * p.chunks;
+  if (grid > INT32_MAX) return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: sizes too large");
+  kern<<<(unsigned)grid, C::THREADS, C::SMEM, s>>>(tk, tv, kbm, khm, vbm, vhm, p);
+  return launch_status("vf4_cross_attn");
+}
+
+template <int LPK>
+static int launch_rows(const XParams& p, cudaStream_t s) {
+  const int64_t grid = (int64_t)p.B * p.Hkv * p.chunks;
+  if (grid > INT32_MAX) return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: sizes too large");
+  if (p.R == 1) xattn_rows_kernel<LPK, 1><<<(unsigned)grid, kRowWarps * 32, 0, s>>>(p);
+  else if (p.R == 2) xattn_rows_kernel<LPK, 2><<<(unsigned)grid, kRowWarps * 32, 0, s>>>(p);
+  else xattn_rows_kernel<LPK, 4><<<(unsigned)grid, kRowWarps * 32, 0, s>>>(p);
+  return launch_status("vf4_cross_attn");
+}
+
+static bool sizes_ok(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D) {
+  return B >= 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && Sq >= 0 && Skv >= 0 && D > 0;
+}
+
+}  // namespace vf4
+
+using namespace vf4;
+
+extern "C" {
+
+int64_t vf4_cross_attn_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D) {
+  if (!sizes_ok(B, H, Hkv, Sq, Skv, D) || B == 0 || Sq == 0 || Skv == 0) return 0;
+  if (B > (1 << 24) || H > (1 << 16) || Sq > (1 << 24) || Skv > (1 << 30) || D > 128) return 0;   // refused by the call
+  int chunk, chunks;
+  plan_chunks(B, Hkv, H / Hkv * Sq, Skv, num_sms(), &chunk, &chunks);
+  return chunks == 1 ? 0 : B * H * Sq * (int64_t)chunks * (D * 4 + 8);
+}
+
+int vf4_cross_attn(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const void* k, int64_t k_b, int64_t k_h,
+                   int64_t k_s, const void* v, int64_t v_b, int64_t v_h, int64_t v_s, int64_t B, int64_t H, int64_t Hkv,
+                   int64_t Sq, int64_t Skv, int64_t D, float scale, const int32_t* kv_lens, const uint8_t* key_mask,
+                   int64_t mask_b, void* out, int64_t o_b, int64_t o_h, int64_t o_s, void* workspace,
+                   int64_t workspace_bytes, vf4_stream_t stream) {
+  if (int st = check_device()) return st;
+  if (!sizes_ok(B, H, Hkv, Sq, Skv, D))
+    return fail(VF4_ERR_ARG, "vf4_cross_attn: bad sizes (B=%lld H=%lld Hkv=%lld Sq=%lld Skv=%lld D=%lld)", (long long)B,
+                (long long)H, (long long)Hkv, (long long)Sq, (long long)Skv, (long long)D);
+  if (D % 8 || D > 128) return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: head dims that are multiples of 8 up to 128 (D=%lld)", (long long)D);
+  if (B > (1 << 24) || H > (1 << 16) || Sq > (1 << 24) || Skv > (1 << 30) || H / Hkv * Sq > (1 << 28))
+    return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: sizes too large");
+  if (B == 0 || Sq == 0) return VF4_OK;
+  if (!q || !out || (Skv > 0 && (!k || !v))) return fail(VF4_ERR_ARG, "vf4_cross_attn: null operand");
+  const int64_t strides[] = {q_b, q_h, q_s, k_b, k_h, k_s, v_b, v_h, v_s, o_b, o_h, o_s};
+  for (int64_t x : strides)
+    if (x % 8 || x < 0) return fail(VF4_ERR_ALIGN, "vf4_cross_attn: strides must be non-negative multiples of 8 elements");
+  if (Skv > 1 && (k_s < D || v_s < D)) return fail(VF4_ERR_ARG, "vf4_cross_attn: keys or values overlap");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(workspace) ||
+      reinterpret_cast<uintptr_t>(kv_lens) % 4)
+    return fail(VF4_ERR_ALIGN, "vf4_cross_attn: operands must be 16-byte aligned");
+  if (!(scale > -INFINITY && scale < INFINITY)) return fail(VF4_ERR_ARG, "vf4_cross_attn: scale is not finite");
+  XParams p{};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.k = static_cast<const __nv_bfloat16*>(k);
+  p.v = static_cast<const __nv_bfloat16*>(v);
+  p.qb = q_b; p.qh = q_h; p.qs = q_s;
+  p.kb = k_b; p.kh = k_h; p.ks = k_s;
+  p.vb = v_b; p.vh = v_h; p.vs = v_s;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.ob = o_b; p.oh = o_h; p.os = o_s;
+  p.lens = kv_lens;
+  p.mask = key_mask;
+  p.mask_b = mask_b;
+  p.B = (int)B; p.Hkv = (int)Hkv; p.G = (int)(H / Hkv); p.Sq = (int)Sq; p.Skv = (int)Skv; p.D = (int)D;
+  p.R = p.G * p.Sq;
+  p.negate = scale < 0.f;
+  p.c = (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
+  if (p.c < 1e-30f) p.c = 1e-30f;   // a scale of 0: every finite score weighs 1, and c * -inf stays -inf
+  p.tiles = (p.R + 255) / 256;
+  plan_chunks(B, Hkv, p.R, Skv, num_sms(), &p.chunk, &p.chunks);
+  if (p.chunks > 1) {
+    const int64_t rows = B * H * Sq * (int64_t)p.chunks;
+    if (!workspace || workspace_bytes < rows * (D * 4 + 8))
+      return fail(VF4_ERR_ARG, "vf4_cross_attn: workspace of %lld bytes needed, got %lld", (long long)(rows * (D * 4 + 8)),
+                  (long long)workspace_bytes);
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * D);
+  }
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  int st = VF4_OK;
+  if (Skv == 0) p.chunks = 0;   // without keys the rows are 0, which joining no chunks writes
+  else if (p.R <= kPlainRows)
+    st = D <= 32 ? launch_rows<4>(p, s) : D <= 64 ? launch_rows<8>(p, s) : launch_rows<16>(p, s);
+  else
+    st = D <= 64 ? launch_tc<64>(p, s) : launch_tc<128>(p, s);
+  if (st || p.chunks == 1) return st;
+  const int64_t rows = B * H * Sq;
+  xattn_join_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
+  return launch_status("vf4_cross_attn (join)");
+}
+
+}  // extern "C"

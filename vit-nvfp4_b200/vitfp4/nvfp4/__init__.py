@@ -10,6 +10,7 @@ from .gemm import (nvfp4_gemm, nvfp4_linear, register_backend, available_backend
 from .fp8 import fp8_e4m3_quant_dequant
 from .fp8_block import quantize_to_fp8_block, dequantize_fp8_block, fp8_block_gemm, fp8_block_linear
 from .norm import gated_residual_norm
+from .cross_attention import cross_sdpa
 from .attention import quant_sdpa
 
 __all__ = [
@@ -19,5 +20,5 @@ __all__ = [
     "cast_nvfp4", "linear_packed",
     "fp8_e4m3_quant_dequant", "quant_sdpa",
     "quantize_to_fp8_block", "dequantize_fp8_block", "fp8_block_gemm", "fp8_block_linear",
-    "gated_residual_norm",
+    "gated_residual_norm", "cross_sdpa",
 ]

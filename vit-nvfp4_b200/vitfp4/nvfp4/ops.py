@@ -645,6 +645,39 @@ def attention_packed_qkv(qkv: torch.Tensor, num_heads: int, scale: float, head_g
     return out
 
 
+def _attn_view(t: torch.Tensor) -> torch.Tensor:
+    """(B, H, S, D) with the strides the cross attention kernels read in place (copied otherwise)."""
+    st = t.stride()
+    if st[3] == 1 and not (st[0] | st[1] | st[2]) % 8 and not t.data_ptr() % 16 and (st[2] >= t.shape[3] or t.shape[2] <= 1):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
+                    kv_lens: torch.Tensor | None = None, key_mask: torch.Tensor | None = None) -> torch.Tensor:
+    """q (B, H, Sq, D) over k, v (B, Hkv, Skv, D) bf16 -> (B, H, Sq, D) bf16, laid out as (B, Sq, H, D).
+
+    ``kv_lens`` (B,) int32, ``key_mask`` (B, Skv) bool with unit column stride.  The workspace is allocated per
+    call (by torch's caching allocator), so concurrent calls and captured graphs never share one."""
+    with _on_device_of(q, k, v, kv_lens, key_mask):
+        q, k, v = _attn_view(q), _attn_view(k), _attn_view(v)
+        B, H, Sq, D = q.shape
+        Hkv, Skv = k.shape[1], k.shape[2]
+        out = torch.empty((B, Sq, H, D), dtype=torch.bfloat16, device=q.device)
+        if out.numel() == 0:
+            return out.transpose(1, 2)
+        n = _lib.lib().vf4_cross_attn_workspace_size(B, H, Hkv, Sq, Skv, D)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+        with _Timed(f"cross_attn_{B * H}x{Sq}x{Skv}x{D}", 4.0 * B * H * Sq * Skv * D):
+            _lib.call("vf4_cross_attn", q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr() or None, ks[0], ks[1], ks[2],
+                      v.data_ptr() or None, vs[0], vs[1], vs[2], B, H, Hkv, Sq, Skv, D, scale, _ptr(kv_lens),
+                      _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), out.data_ptr(), Sq * H * D, D,
+                      H * D, _ptr(ws), n, _stream())
+        _launched(2 if n else 1)
+    return out.transpose(1, 2)
+
+
 def ln_cast(x: torch.Tensor, ln_w: torch.Tensor, ln_b: torch.Tensor, eps: float, gs: torch.Tensor | None = None,
             y: torch.Tensor | None = None, gamma: torch.Tensor | None = None, x_out: torch.Tensor | None = None):
     """LayerNorm fused into the NVFP4 cast, optionally after x' = x + y * gamma (written to x_out).
