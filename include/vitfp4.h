@@ -355,6 +355,17 @@ VF4_API int vf4_gemm_fp8_block(const uint8_t* a, int64_t lda, const float* a_sca
                                int64_t M, int64_t N, int64_t K, const void* bias, int bias_dtype, void* out,
                                int64_t ldo, int out_dtype, vf4_stream_t stream);
 
+/* Linear layer with an FP8 block weight: vf4_cast_fp8_block of the rows x (M, K), then vf4_gemm_fp8_block, in one
+ * call: out = x W^T + bias in x's dtype.  Up to 4 rows (K up to 24576
+ * for one row, 12288 for two, 6144 beyond) take one launch that
+ * casts the rows itself.  workspace: vf4_linear_fp8_block_workspace_size(M, K) bytes (0: none needed), 16-byte
+ * aligned, used until the call's work is done. */
+VF4_API int64_t vf4_linear_fp8_block_workspace_size(int64_t M, int64_t K);
+VF4_API int vf4_linear_fp8_block(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w, int64_t ldw,
+                                 const float* w_scale, int64_t ws_n, int64_t ws_k, int64_t N, const void* bias,
+                                 int bias_dtype, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes,
+                                 vf4_stream_t stream);
+
 /* Norms before and after a block, fused with its gate and residual scale (sandwich / adaLN-gated blocks; a timm
  * or DINOv2 block's LayerScale is the gate with one group and no post-norm):
  *   x' = x + residual_scale * gate (.) N_post(y)        h = N_pre(x')

@@ -5,6 +5,7 @@
 //
 // No counterpart in the reference, whose formats are bf16 and NVFP4; the framework's layers that stay
 // out of NVFP4 (heads, first and last blocks, projections of a cross attention) take this one.
+#include <cuda_fp16.h>
 #include <string.h>
 
 #include "vf4_fp8_block.cuh"
@@ -655,6 +656,160 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
   }
 }
 
+// ---------------------------------------------------------------------------------------
+// Linear layer of up to 4 rows (a decoder's token, a class token): cast and product in one launch.  Bound by
+// reading the weight once.  Every CTA casts the rows for itself into shared memory (decoded: code * scale, in
+// the order in which the lanes read them), while its warps' first weights are on their way; then a warp takes
+// two weight rows at a time, 512 columns (16 per lane) by 512.  The tensor core would pad the rows to 16 and
+// needs a cast kernel before it and a reduction after it.
+// ---------------------------------------------------------------------------------------
+constexpr int kVecRows = 4, kVecWarps = 8;
+
+struct F8Vec {
+  const void* x;
+  int64_t ldx;
+  const uint8_t* b;
+  int64_t ldb;
+  int K, chunks;       // chunks of 512 columns
+  int x_vec;           // x rows may be read 4 elements at a time
+};
+
+// Codes k .. k + 15 of a row (0 past K, whatever the row's padding holds).
+VF4_DEV uint4 load_codes(const uint8_t* row, int k, int K) {
+  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  for (int i = 0; k + i < K && i < 16; ++i) w[i >> 2] |= (uint32_t)__ldg(row + k + i) << (8 * (i & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+VF4_DEV float2 e4m3x2_to_f32x2(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xFFFFu), __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+template <typename T, int R>
+__global__ void __launch_bounds__(kVecWarps * 32, 2) fp8_linear_rows_kernel(const F8Vec a, const F8Params p) {
+  extern __shared__ __align__(16) float xs[];   // [R][chunk][4][32 lanes][4]: lane's columns 16 lane + 4 j ..
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wid = blockIdx.x * kVecWarps + warp, total = gridDim.x * kVecWarps;
+  const int row_floats = a.chunks * 512;
+  // two weight rows n and n + total, chunk by chunk
+  uint4 w[2];
+  auto fetch = [&](int n, int c, uint4* d) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = n + i * total;
+      d[i] = r < p.N ? load_codes(a.b + (int64_t)r * a.ldb, c * 512 + lane * 16, a.K) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  fetch(wid, 0, w);
+  // the cast: a warp per block of 128 columns, 4 per lane
+  for (int i = warp; i < R * a.chunks * 4; i += kVecWarps) {
+    const int m = i / (a.chunks * 4), g = i - m * (a.chunks * 4), k = g * 128 + lane * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (m < p.M && k < a.K) {
+      const T* src = static_cast<const T*>(a.x) + m * a.ldx + k;
+      if (a.x_vec && k + 4 <= a.K) {
+        if constexpr (sizeof(T) == 2) {
+          const uint2 u = __ldg(reinterpret_cast<const uint2*>(src));
+          v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xFFFF0000u);
+          v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xFFFF0000u);
+        } else {
+          const float4 u = __ldg(reinterpret_cast<const float4*>(src));
+          v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (k + e < a.K) v[e] = (float)src[e];
+      }
+    }
+    uint32_t top = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const Fp8Block q = fp8_block(top);
+    const float2 lo = e4m3x2_to_f32x2(e4m3x2(fp8_quotient(v[0], q), fp8_quotient(v[1], q)));
+    const float2 hi = e4m3x2_to_f32x2(e4m3x2(fp8_quotient(v[2], q), fp8_quotient(v[3], q)));
+    const int in = (k & 511) >> 4, j = (k & 15) >> 2;   // the lane that will read these 4, and its piece
+    *reinterpret_cast<float4*>(xs + m * row_floats + ((((k >> 9) * 4 + j) * 32 + in) << 2)) =
+        make_float4(lo.x * q.scale, lo.y * q.scale, hi.x * q.scale, hi.y * q.scale);
+  }
+  __syncthreads();
+  for (int n = wid; n < p.N; n += 2 * total) {
+    float acc[2][R];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int m = 0; m < R; ++m) acc[i][m] = 0.f;
+    for (int c = 0; c < a.chunks; ++c) {
+      const uint4 now[2] = {w[0], w[1]};
+      const bool last = c + 1 == a.chunks;
+      if (!last || n + 2 * total < p.N) fetch(last ? n + 2 * total : n, last ? 0 : c + 1, w);
+      const int g = min(c * 4 + (lane >> 3), p.kb - 1);   // this lane's block (past K its codes are 0)
+      float4 x[R][4];
+#pragma unroll
+      for (int m = 0; m < R; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[m][j] = *reinterpret_cast<const float4*>(xs + m * row_floats + (((c * 4 + j) * 32 + lane) << 2));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float s = __ldg(p.sb + (int64_t)(min(n + i * total, p.N - 1) >> 7) * p.sb_n + g * p.sb_k);
+        const uint32_t u[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
+        float d[R];
+#pragma unroll
+        for (int m = 0; m < R; ++m) d[m] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 lo = e4m3x2_to_f32x2(u[j]), hi = e4m3x2_to_f32x2(u[j] >> 16);
+#pragma unroll
+          for (int m = 0; m < R; ++m) {
+            d[m] = fmaf(lo.x, x[m][j].x, d[m]);
+            d[m] = fmaf(lo.y, x[m][j].y, d[m]);
+            d[m] = fmaf(hi.x, x[m][j].z, d[m]);
+            d[m] = fmaf(hi.y, x[m][j].w, d[m]);
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < R; ++m) acc[i][m] = fmaf(d[m], s, acc[i][m]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int m = 0; m < R; ++m) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) acc[i][m] += __shfl_xor_sync(0xFFFFFFFFu, acc[i][m], o);
+        if (lane == 0) store1<sizeof(T) == 4>(p, m, n + i * total, acc[i][m]);
+      }
+  }
+}
+
+// What the kernel above takes: its rows' decoded values fit shared memory twice per SM.
+static int rows_held(int64_t M) { return M == 3 ? 4 : (int)M; }
+static bool few_rows(int64_t M, int64_t K) {
+  return M <= kVecRows && rows_held(M) * ((K + 511) / 512) * 2048 <= 96 * 1024;
+}
+
+template <typename T>
+static int launch_rows(const F8Vec& a, const F8Params& p, cudaStream_t s) {
+  const int R = rows_held(p.M);
+  const size_t smem = (size_t)R * a.chunks * 2048;
+  const int sms = num_sms();
+  int64_t grid = ((int64_t)p.N + 2 * kVecWarps - 1) / (2 * kVecWarps);   // two rows per warp, if that fills the machine
+  if (grid < sms) grid = ((int64_t)p.N + kVecWarps - 1) / kVecWarps;
+  if (grid > 2 * sms) grid = 2 * sms;
+  auto run = [&](auto kern) {
+    if (smem > 48 * 1024) {
+      if (int st = smem_optin(kern, 96 * 1024)) return st;
+    }
+    kern<<<(unsigned)grid, kVecWarps * 32, smem, s>>>(a, p);
+    return launch_status("vf4_linear_fp8_block");
+  };
+  if (R == 1) return run(fp8_linear_rows_kernel<T, 1>);
+  if (R == 2) return run(fp8_linear_rows_kernel<T, 2>);
+  return run(fp8_linear_rows_kernel<T, 4>);
+}
+
 static int make_code_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t K, int64_t ld, int box_rows) {
   EncodeTiledFn enc = encode_tiled();
   if (!enc) return fail(VF4_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
@@ -841,6 +996,55 @@ int vf4_gemm_fp8_block(const uint8_t* a, int64_t lda, const float* a_scale, int6
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const F8Operand x{a, M, lda}, w{b, N, ldb};
   return out_dtype == VF4_F32 ? dispatch_fp8_gemm<true>(x, w, K, p, s) : dispatch_fp8_gemm<false>(x, w, K, p, s);
+}
+
+// workspace of vf4_linear_fp8_block: the rows' codes, then their scales, column block by column block
+int64_t vf4_linear_fp8_block_workspace_size(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0 || M > (1 << 30) || K > (1 << 20) || few_rows(M, K)) return 0;
+  return M * ((K + 15) / 16 * 16) + M * ((K + 127) / 128) * 4;
+}
+
+int vf4_linear_fp8_block(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w, int64_t ldw,
+                         const float* w_scale, int64_t ws_n, int64_t ws_k, int64_t N, const void* bias, int bias_dtype,
+                         void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, vf4_stream_t stream) {
+  if (int st = check_device()) return st;
+  const int64_t need = vf4_linear_fp8_block_workspace_size(M, K);
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    return fail(VF4_ERR_ARG, "vf4_linear_fp8_block: %lld bytes of 16-byte aligned workspace needed, got %lld", (long long)need,
+                (long long)workspace_bytes);
+  if (M > 0 && few_rows(M, K)) {
+    if (K <= 0 || N <= 0 || ldx < K || ldo < N || N > (1 << 24))
+      return fail(VF4_ERR_ARG, "vf4_linear_fp8_block: bad sizes M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
+    if ((dtype != VF4_BF16 && dtype != VF4_F32) || (bias && bias_dtype != VF4_BF16 && bias_dtype != VF4_F32))
+      return fail(VF4_ERR_ARG, "vf4_linear_fp8_block: bad dtype");
+    if (!x || !w || !w_scale || !out) return fail(VF4_ERR_ARG, "vf4_linear_fp8_block: null operand");
+    const int esz = dtype == VF4_BF16 ? 2 : 4;
+    if (!aligned16(w) || ldw % 16 || ldw < K)
+      return fail(VF4_ERR_ALIGN, "vf4_linear_fp8_block: code rows need 16-byte aligned starts of at least K bytes (ldw=%lld)", (long long)ldw);
+    if (reinterpret_cast<uintptr_t>(x) % esz || reinterpret_cast<uintptr_t>(out) % esz || reinterpret_cast<uintptr_t>(w_scale) % 4 ||
+        (bias && reinterpret_cast<uintptr_t>(bias) % (bias_dtype == VF4_BF16 ? 2 : 4)))
+      return fail(VF4_ERR_ALIGN, "vf4_linear_fp8_block: a pointer is misaligned for its type");
+    F8Vec a{x, ldx, w, ldw, (int)K, (int)((K + 511) / 512), reinterpret_cast<uintptr_t>(x) % (4 * esz) == 0 && (M == 1 || ldx % 4 == 0)};
+    F8Params p{};
+    p.sb = w_scale;
+    p.sb_n = ws_n;
+    p.sb_k = ws_k;
+    p.M = (int)M;
+    p.N = (int)N;
+    p.kb = (int)((K + 127) / 128);
+    p.bias = bias;
+    p.bias_f32 = bias_dtype == VF4_F32;
+    p.out = out;
+    p.ldo = ldo;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    return dtype == VF4_BF16 ? launch_rows<__nv_bfloat16>(a, p, s) : launch_rows<float>(a, p, s);
+  }
+  const int64_t ldc = (K + 15) / 16 * 16;
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  float* scale = reinterpret_cast<float*>(codes + M * ldc);
+  if (int st = vf4_cast_fp8_block(x, dtype, M, K, ldx, 1, codes, ldc, scale, 1, M, stream)) return st;
+  return vf4_gemm_fp8_block(codes, ldc, scale, 1, M, w, ldw, w_scale, ws_n, ws_k, M, N, K, bias, bias_dtype, out, ldo,
+                            dtype, stream);
 }
 
 }  // extern "C"

@@ -60,6 +60,8 @@ SIGNATURES: dict[str, list] = {
     "vf4_attn_workspace_size_modes": [_L, _L, _L, _L, _I, _I, _I],
     "vf4_cast_fp8_block": [_P, _I, _L, _L, _L, _I, _P, _L, _P, _L, _L, _P],
     "vf4_gemm_fp8_block": [_P, _L, _P, _L, _L, _P, _L, _P, _L, _L, _L, _L, _L, _P, _I, _P, _L, _I, _P],
+    "vf4_linear_fp8_block_workspace_size": [_L, _L],
+    "vf4_linear_fp8_block": [_P, _I, _L, _L, _L, _P, _L, _P, _L, _L, _L, _P, _I, _P, _L, _P, _L, _P],
     "vf4_gated_residual_norm": [_P, _L, _P, _L, _I, _L, _L, _P, _L, ctypes.c_float, _I, _P, _P, _I, _P, _P, _I,
                                 ctypes.c_float, _P, _P, _I, _L, _P, _L, _L, _P],
     "vf4_cross_attn_workspace_size": [_L, _L, _L, _L, _L, _L],
@@ -69,7 +71,8 @@ SIGNATURES: dict[str, list] = {
 }
 _RESTYPE = {"vf4_last_error_string": ctypes.c_char_p, "vf4_attn_workspace_size": ctypes.c_int64,
             "vf4_attn_workspace_size_ex": ctypes.c_int64, "vf4_attn_workspace_size_modes": ctypes.c_int64,
-            "vf4_b_scale_image_bytes": ctypes.c_int64, "vf4_cross_attn_workspace_size": ctypes.c_int64}
+            "vf4_b_scale_image_bytes": ctypes.c_int64, "vf4_cross_attn_workspace_size": ctypes.c_int64,
+            "vf4_linear_fp8_block_workspace_size": ctypes.c_int64}
 
 
 class VitFp4Error(RuntimeError):

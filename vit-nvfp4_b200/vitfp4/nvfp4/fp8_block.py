@@ -25,18 +25,19 @@ def _check_operand(name: str, codes: torch.Tensor, scale: torch.Tensor, block_ro
     if codes.dtype != torch.float8_e4m3fn or codes.dim() != 2:
         raise _lib.VitFp4Error(f"{name}: (rows, K) float8_e4m3fn codes needed, got {tuple(codes.shape)} {codes.dtype}")
     rows, K = codes.shape
-    want = (-(-rows // block_rows), -(-K // _BLOCK))
-    if scale.dtype != torch.float32 or tuple(scale.shape) != want:
-        raise _lib.VitFp4Error(f"{name}: scales of {codes.shape} codes are {want} fp32, got {tuple(scale.shape)} "
+    want = ((rows + block_rows - 1) // block_rows, (K + _BLOCK - 1) // _BLOCK)
+    if scale.dtype != torch.float32 or scale.shape != want:
+        raise _lib.VitFp4Error(f"{name}: scales of {tuple(codes.shape)} codes are {want} fp32, got {tuple(scale.shape)} "
                                f"{scale.dtype}")
 
 
 def _check_weight(w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None) -> None:
     _check_operand("weight", w, w_scale, _BLOCK)
-    if w.shape[0] < 1 or w.shape[1] < 1:
+    N, K = w.shape
+    if N < 1 or K < 1:
         raise _lib.VitFp4Error(f"weight: at least one row and one column needed, got {tuple(w.shape)}")
-    if bias is not None and (tuple(bias.shape) != (w.shape[0],) or bias.stride(0) != 1 and w.shape[0] > 1):
-        raise _lib.VitFp4Error(f"bias: a contiguous ({w.shape[0]},) vector needed, got {tuple(bias.shape)}")
+    if bias is not None and (bias.shape != (N,) or bias.stride(0) != 1 and N > 1):
+        raise _lib.VitFp4Error(f"bias: a contiguous ({N},) vector needed, got {tuple(bias.shape)}")
 
 
 @torch.library.custom_op("vitfp4::cast_fp8_block", mutates_args=())
@@ -65,12 +66,28 @@ def _(a, a_scale, b, b_scale, bias, fp32_out):
     return a.new_empty((a.shape[0], b.shape[0]), dtype=torch.float32 if fp32_out else torch.bfloat16)
 
 
+@torch.library.custom_op("vitfp4::linear_fp8_block", mutates_args=())
+def linear_fp8_block_op(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                        bias: torch.Tensor | None) -> torch.Tensor:
+    return ops.linear_fp8_block(x, w, w_scale, bias)
+
+
+@linear_fp8_block_op.register_fake
+def _(x, w, w_scale, bias):
+    return x.new_empty((x.shape[0], w.shape[0]))
+
+
 def _traced(*ts: torch.Tensor | None) -> bool:
     """Whether a call has to go through its torch.library op: under torch.compile, or where gradients are
     recorded (the op has no backward and says so).  Plain calls skip the dispatcher, which costs more host time
     than the small kernels run."""
-    return torch.compiler.is_compiling() or (torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                                                             for t in ts))
+    if torch.compiler.is_compiling():
+        return True
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def quantize_to_fp8_block(x: torch.Tensor, block_rows: int = 1):
@@ -120,10 +137,5 @@ def fp8_block_linear(x, w, w_scale, *, bias=None):
     if x.shape[-1] != w.shape[1]:
         raise _lib.VitFp4Error(f"x has {x.shape[-1]} columns, the weight {w.shape[1]}")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if _traced(x, w_scale, bias):
-        codes, scale = cast_fp8_block_op(x2, 1)
-        y = gemm_fp8_block_op(codes, scale, w, w_scale, bias, x.dtype == torch.float32)
-    else:
-        codes, scale = ops.cast_fp8_block(x2, 1)
-        y = ops.gemm_fp8_block(codes, scale, w, w_scale, bias, x.dtype)
+    y = (linear_fp8_block_op if _traced(x, w_scale, bias) else ops.linear_fp8_block)(x2, w, w_scale, bias)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], w.shape[0])

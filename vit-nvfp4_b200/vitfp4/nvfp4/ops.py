@@ -55,7 +55,8 @@ class _Timed:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """Torch's current stream on the current device (the raw handle: building a Stream object costs 3 us)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -215,31 +216,34 @@ def gptq_block(w: torch.Tensor, hinv: torch.Tensor, block_scale: torch.Tensor, g
     _launched()
 
 
-def _on_device_of(*ts: torch.Tensor | None):
-    """All tensors on one CUDA device (else an error); a context that makes it the current one, so the
-    launch and the stream it goes to are that device's."""
+def _elsewhere(*ts: torch.Tensor | None) -> bool:
+    """Whether a call's tensors (all on one CUDA device, else an error) live on another device than the current
+    one; ``_there`` then runs the call with that device current, so that launch and stream are that device's."""
     dev = None
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            _need_cuda(t)
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise _lib.VitFp4Error(f"tensors on two devices: {dev} and {t.device}")
-    return _same_device if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+        if t is not None:
+            i = t.get_device()
+            if i < 0:
+                _need_cuda(t)
+            if dev is None:
+                dev = i
+            elif i != dev:
+                raise _lib.VitFp4Error(f"tensors on two devices: cuda:{dev} and cuda:{i}")
+    return dev != torch._C._cuda_getDevice()
 
 
-class _SameDevice:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *a):
-        return None
+def _there(fn, first: torch.Tensor, *args):
+    with torch.cuda.device(first.device):
+        return fn(first, *args)
 
 
-_same_device = _SameDevice()
+def _timed(kind: str, sizes: tuple, work: float, name: str, *args) -> None:
+    """One launch under the probe's events (the label is only built when it is on)."""
+    if probe.timing:
+        with _Timed(f"{kind}_{'x'.join(map(str, sizes))}", work):
+            _lib.call(name, *args)
+    else:
+        _lib.call(name, *args)
 
 
 def _rows_2d(x: torch.Tensor) -> torch.Tensor:
@@ -259,24 +263,21 @@ def cast_fp8_block(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, 
     """FP8 block cast of (M, K) bf16 / fp32 rows: codes float8_e4m3fn (M, K), in rows padded to 16 bytes,
     and fp32 scales (ceil(M / block_rows), ceil(K / 128)); block_rows is 1 (activations) or 128 (weights).
     The activation scales are stored column block by column block, the order the product reads them in."""
-    with _on_device_of(x):
-        code = _dtype_code(x)
-        x2 = _rows_2d(x)
-        M, K = x2.shape
-        if K < 1:
-            raise _lib.VitFp4Error("the FP8 block cast needs at least one column")
-        ldc, kb = (K + 15) // 16 * 16, (K + 127) // 128
-        codes = torch.empty((M, ldc), dtype=torch.float8_e4m3fn, device=x.device)
-        if block_rows == 1:
-            scale = torch.empty((kb, M), dtype=torch.float32, device=x.device)
-            s_m, s_k, scale = 1, M, scale.t()
-        else:
-            scale = torch.empty(((M + block_rows - 1) // block_rows, kb), dtype=torch.float32, device=x.device)
-            s_m, s_k = kb, 1
-        with _Timed(f"cast_fp8_block_{M}x{K}", M * K * (x2.element_size() + 1) + scale.numel() * 4):
-            _lib.call("vf4_cast_fp8_block", x2.data_ptr(), code, M, K, _ld(x2), block_rows, codes.data_ptr(), ldc,
-                      scale.data_ptr(), s_m, s_k, _stream())
-        _launched()
+    if _elsewhere(x):
+        return _there(cast_fp8_block, x, block_rows)
+    code = _dtype_code(x)
+    x2 = _rows_2d(x)
+    M, K = x2.shape
+    if K < 1:
+        raise _lib.VitFp4Error("the FP8 block cast needs at least one column")
+    ldc, kb, dev = (K + 15) // 16 * 16, (K + 127) // 128, x.device
+    codes = torch.empty_strided((M, ldc), (ldc, 1), dtype=torch.float8_e4m3fn, device=dev)
+    rows = M if block_rows == 1 else (M + block_rows - 1) // block_rows
+    s_m, s_k = (1, M) if block_rows == 1 else (kb, 1)
+    scale = torch.empty_strided((rows, kb), (s_m, s_k), dtype=torch.float32, device=dev)
+    _timed("cast_fp8_block", (M, K), M * K * (x2.element_size() + 1) + rows * kb * 4, "vf4_cast_fp8_block",
+           x2.data_ptr(), code, M, K, _ld(x2), block_rows, codes.data_ptr(), ldc, scale.data_ptr(), s_m, s_k, _stream())
+    probe.launches += 1
     return (codes if ldc == K else codes[:, :K]), scale
 
 
@@ -293,16 +294,37 @@ def _code_rows(t: torch.Tensor) -> torch.Tensor:
 def gemm_fp8_block(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
                    bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """(M, K) x (N, K) FP8 block operands -> (M, N) bf16 or fp32 (+ bias)."""
-    with _on_device_of(a, a_scale, b, b_scale, bias):
-        a, b = _code_rows(a), _code_rows(b)
-        (M, K), N = a.shape, b.shape[0]
-        out = torch.empty((M, N), dtype=out_dtype, device=a.device)
-        with _Timed(f"gemm_fp8_block_{M}x{N}x{K}", 2.0 * M * N * K):
-            _lib.call("vf4_gemm_fp8_block", a.data_ptr(), _ld(a), a_scale.data_ptr(), a_scale.stride(0),
-                      a_scale.stride(1), b.data_ptr(), _ld(b), b_scale.data_ptr(), b_scale.stride(0),
-                      b_scale.stride(1), M, N, K, _ptr(bias), 0 if bias is None else _dtype_code(bias),
-                      out.data_ptr(), N, _dtype_code(out), _stream())
-        _launched()
+    if _elsewhere(a, a_scale, b, b_scale, bias):
+        return _there(gemm_fp8_block, a, a_scale, b, b_scale, bias, out_dtype)
+    a, b = _code_rows(a), _code_rows(b)
+    (M, K), N = a.shape, b.shape[0]
+    out = torch.empty_strided((M, N), (N, 1), dtype=out_dtype, device=a.device)
+    as_m, as_k = a_scale.stride()
+    bs_n, bs_k = b_scale.stride()
+    _timed("gemm_fp8_block", (M, N, K), 2.0 * M * N * K, "vf4_gemm_fp8_block", a.data_ptr(), _ld(a), a_scale.data_ptr(),
+           as_m, as_k, b.data_ptr(), _ld(b), b_scale.data_ptr(), bs_n, bs_k, M, N, K, _ptr(bias),
+           0 if bias is None else _dtype_code(bias), out.data_ptr(), N, 1 if out_dtype == torch.float32 else 0, _stream())
+    probe.launches += 1
+    return out
+
+
+def linear_fp8_block(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                     bias: torch.Tensor | None = None) -> torch.Tensor:
+    """Cast of the rows x (M, K) and product with the FP8 block weight w (N, K) in one call -> (M, N) in x's type.
+    The rows' codes live in a workspace allocated per call."""
+    if _elsewhere(x, w, w_scale, bias):
+        return _there(linear_fp8_block, x, w, w_scale, bias)
+    code = _dtype_code(x)
+    x, w = _rows_2d(x), _code_rows(w)
+    (M, K), N, dev = x.shape, w.shape[0], x.device
+    out = torch.empty_strided((M, N), (N, 1), dtype=x.dtype, device=dev)
+    n = _lib.lib().vf4_linear_fp8_block_workspace_size(M, K)
+    ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=dev) if n else None
+    ws_n, ws_k = w_scale.stride()
+    _timed("linear_fp8_block", (M, N, K), 2.0 * M * N * K, "vf4_linear_fp8_block", x.data_ptr(), code, M, K, _ld(x),
+           w.data_ptr(), _ld(w), w_scale.data_ptr(), ws_n, ws_k, N, _ptr(bias), 0 if bias is None else _dtype_code(bias),
+           out.data_ptr(), N, _ptr(ws), n, _stream())
+    probe.launches += 2 if n else 1
     return out
 
 
@@ -316,32 +338,32 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor | None, gate: torch.Ten
 
     Returns (x' or None without y, h or None without pre, scales or None): h is (M, K) in x's dtype, or E4M3
     codes with their scales.  The parameters share one dtype, bf16 or fp32."""
-    with _on_device_of(x, y, gate, post_w, post_b, pre_w, pre_b):
-        x2 = _rows_2d(x)
-        y2 = None if y is None else _rows_2d(y)
-        M, K = x2.shape
-        x_out = None if y is None else torch.empty((M, K), dtype=x.dtype, device=x.device)
-        h = scale = None
-        ldc = s_m = s_k = 0
-        if pre is not None and fp8_out:
-            ldc = (K + 15) // 16 * 16
-            h = torch.empty((M, ldc), dtype=torch.float8_e4m3fn, device=x.device)
-            scale = torch.empty(((K + 127) // 128, M), dtype=torch.float32, device=x.device).t()
-            s_m, s_k = 1, M
-        elif pre is not None:
-            h = torch.empty((M, K), dtype=x.dtype, device=x.device)
-        param = next((t for t in (gate, post_w, post_b, pre_w, pre_b) if t is not None), x)
-        groups = 1 if gate is None or gate.dim() == 1 else gate.shape[0]
-        esz = x.element_size()
-        if M == 0:   # empty tensors have no address, which would read as "not given"
-            return x_out, h if h is None else h[:, :K], scale
-        with _Timed(f"gated_norm_{M}x{K}", M * K * (esz * (1 if y is None else 3) +
-                                                   (0 if h is None else 1 if fp8_out else esz))):
-            _lib.call("vf4_gated_residual_norm", x2.data_ptr(), _ld(x2), _ptr(y2), 0 if y2 is None else _ld(y2),
-                      _dtype_code(x), M, K, _ptr(gate), groups, residual_scale, NORM_KINDS[post], _ptr(post_w),
-                      _ptr(post_b), NORM_KINDS[pre], _ptr(pre_w), _ptr(pre_b), _dtype_code(param), eps,
-                      _ptr(x_out), _ptr(h), int(fp8_out), ldc, _ptr(scale), s_m, s_k, _stream())
-        _launched()
+    if _elsewhere(x, y, gate, post_w, post_b, pre_w, pre_b):
+        return _there(gated_residual_norm, x, y, gate, residual_scale, post, post_w, post_b, pre, pre_w, pre_b, eps, fp8_out)
+    x2 = _rows_2d(x)
+    y2 = None if y is None else _rows_2d(y)
+    (M, K), dev = x2.shape, x.device
+    x_out = None if y is None else torch.empty_strided((M, K), (K, 1), dtype=x.dtype, device=dev)
+    h = scale = None
+    ldc = s_m = s_k = 0
+    if pre is not None and fp8_out:
+        ldc, kb = (K + 15) // 16 * 16, (K + 127) // 128
+        h = torch.empty_strided((M, ldc), (ldc, 1), dtype=torch.float8_e4m3fn, device=dev)
+        scale = torch.empty_strided((M, kb), (1, M), dtype=torch.float32, device=dev)
+        s_m, s_k = 1, M
+    elif pre is not None:
+        h = torch.empty_strided((M, K), (K, 1), dtype=x.dtype, device=dev)
+    param = gate if gate is not None else post_w if post_w is not None else post_b if post_b is not None else \
+        pre_w if pre_w is not None else pre_b if pre_b is not None else x
+    groups = 1 if gate is None or gate.dim() == 1 else gate.shape[0]
+    if M == 0:   # empty tensors have no address, which would read as "not given"
+        return x_out, h if h is None else h[:, :K], scale
+    esz = x.element_size()
+    _timed("gated_norm", (M, K), M * K * (esz * (1 if y is None else 3) + (0 if h is None else 1 if fp8_out else esz)),
+           "vf4_gated_residual_norm", x2.data_ptr(), _ld(x2), _ptr(y2), 0 if y2 is None else _ld(y2), _dtype_code(x), M, K,
+           _ptr(gate), groups, residual_scale, NORM_KINDS[post], _ptr(post_w), _ptr(post_b), NORM_KINDS[pre], _ptr(pre_w),
+           _ptr(pre_b), _dtype_code(param), eps, _ptr(x_out), _ptr(h), int(fp8_out), ldc, _ptr(scale), s_m, s_k, _stream())
+    probe.launches += 1
     if h is not None and ldc and ldc != K:
         h = h[:, :K]
     return x_out, h, scale
@@ -659,23 +681,25 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
 
     ``kv_lens`` (B,) int32, ``key_mask`` (B, Skv) bool with unit column stride.  The workspace is allocated per
     call (by torch's caching allocator), so concurrent calls and captured graphs never share one."""
-    with _on_device_of(q, k, v, kv_lens, key_mask):
-        q, k, v = _attn_view(q), _attn_view(k), _attn_view(v)
-        B, H, Sq, D = q.shape
-        Hkv, Skv = k.shape[1], k.shape[2]
-        out = torch.empty((B, Sq, H, D), dtype=torch.bfloat16, device=q.device)
-        if out.numel() == 0:
-            return out.transpose(1, 2)
-        n = _lib.lib().vf4_cross_attn_workspace_size(B, H, Hkv, Sq, Skv, D)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        qs, ks, vs = q.stride(), k.stride(), v.stride()
-        with _Timed(f"cross_attn_{B * H}x{Sq}x{Skv}x{D}", 4.0 * B * H * Sq * Skv * D):
-            _lib.call("vf4_cross_attn", q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr() or None, ks[0], ks[1], ks[2],
-                      v.data_ptr() or None, vs[0], vs[1], vs[2], B, H, Hkv, Sq, Skv, D, scale, _ptr(kv_lens),
-                      _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), out.data_ptr(), Sq * H * D, D,
-                      H * D, _ptr(ws), n, _stream())
-        _launched(2 if n else 1)
-    return out.transpose(1, 2)
+    if _elsewhere(q, k, v, kv_lens, key_mask):
+        return _there(cross_attention, q, k, v, scale, kv_lens, key_mask)
+    q, k, v = _attn_view(q), _attn_view(k), _attn_view(v)
+    B, H, Sq, D = q.shape
+    Hkv, Skv = k.shape[1], k.shape[2]
+    out = torch.empty_strided((B, H, Sq, D), (Sq * H * D, D, H * D, 1), dtype=torch.bfloat16, device=q.device)
+    if B == 0 or Sq == 0:
+        return out
+    n = _lib.lib().vf4_cross_attn_workspace_size(B, H, Hkv, Sq, Skv, D)
+    ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=q.device) if n else None
+    qb, qh, qs, _ = q.stride()
+    kb, kh, ks, _ = k.stride()
+    vb, vh, vs, _ = v.stride()
+    _timed("cross_attn", (B * H, Sq, Skv, D), 4.0 * B * H * Sq * Skv * D, "vf4_cross_attn", q.data_ptr(), qb, qh, qs,
+           k.data_ptr() or None, kb, kh, ks, v.data_ptr() or None, vb, vh, vs, B, H, Hkv, Sq, Skv, D, scale, _ptr(kv_lens),
+           _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), out.data_ptr(), Sq * H * D, D, H * D, _ptr(ws), n,
+           _stream())
+    probe.launches += 2 if n else 1
+    return out
 
 
 def ln_cast(x: torch.Tensor, ln_w: torch.Tensor, ln_b: torch.Tensor, eps: float, gs: torch.Tensor | None = None,
