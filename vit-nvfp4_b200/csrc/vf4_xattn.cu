@@ -10,8 +10,8 @@
 // The G query heads that share a key / value head and their Sq queries are the rows of one problem:
 // R = G * Sq rows against the same keys, so a decoder's single token still reads each key once.
 //
-//   R > 4   tcgen05: 128-row tiles, 128 keys at a time, online softmax (xattn_tc_kernel)
-//   R <= 4  plain FMAs: the keys stream through registers (xattn_rows_kernel)
+//   xattn_tc_kernel    tcgen05: 128-row tiles, 128 keys at a time, online softmax
+//   xattn_rows_kernel  up to 4 rows over short keys, plain FMAs: the keys stream through registers
 //
 // With fewer tiles than SMs the keys are cut into chunks: each CTA leaves its rows' maxima, sums and
 // unnormalised outputs in the workspace and xattn_join_kernel adds them up in order.
@@ -49,7 +49,7 @@ struct XParams {
   int chunk, chunks;       // keys per CTA and CTAs per row tile; chunks > 1: partial results to the workspace
   float* part_o;           // [B * Hkv][chunks][R][D]
   float2* part_ml;         // [B * Hkv][chunks][R]: {maximum of the scores, sum of the weights}
-  int tiles;               // 256-row tiles (tcgen05 kernel)
+  int tiles;               // 128-row tiles (tcgen05 kernel)
 };
 
 VF4_DEV int keys_of(const XParams& p, int b) {
@@ -274,38 +274,44 @@ __global__ void __launch_bounds__(128) xattn_join_kernel(const XParams p) {
 }
 
 // ---------------------------------------------------------------------------------------
-// More rows: tcgen05.  A CTA takes up to 256 rows as two slots of 128 and runs "steps", one slot's 128
-// rows against one tile of 128 keys:
-//   two slots of rows (more than 128):  step i = slot i % 2, key tile i / 2 -- both slots use each tile
-//   one slot of rows:                   step i = slot i % 2, key tile i     -- the slots share the rows and
-//                                       take turns at the key tiles; joined at the end
-// so that one slot's softmax runs while the tensor core works for the other.  Per step:
-//   S = Q K^T (128 x 128, fp32, tensor memory) -> softmax warps: maximum, P = 2^(c s - c m) in bf16 over
-//   S's own columns in tensor memory -> O += P V (accumulated in tensor memory)
+// Many rows or many keys: tcgen05.  A CTA takes 128 rows and runs over its keys in tiles of 128:
+//   S = Q K^T (128 x 128, fp32, tensor memory) -> softmax warps: maximum, P = 2^(c s - c m) in bf16, back to
+//   tensor memory -> O += P V (accumulated in tensor memory)
+// Two CTAs share an SM (half of its shared and tensor memory each), so that one's softmax runs while the
+// tensor core works for the other, and one's first and last steps hide behind the other's middle ones.
+// Up to 64 elements per head P has columns of its own, and the next tile's S is computed while this one's P
+// is; beyond, P takes S's place and the next S follows O += P V.
+//
 // The running maximum m is only moved (and O and the sums rescaled) when it grows by more than 2^8: P stays
 // below 256, which bf16 and the fp32 sums hold as well as P <= 1.
 //
 //   warp 0      TMA of K and V tiles (128-byte swizzle, panels of 64 elements)
 //   warp 1      TMEM allocation, MMAs
-//   warp 2      masks: clears the masked rows of each V tile in shared memory, so that no NaN of theirs meets
-//               a weight of 0
-//   warps 4-7, 8-11  softmax of slot 0 and 1, a thread per row (holds the 128 scores in registers)
+//   warp 2      masks (with a mask or key counts): spreads each tile's kept keys to words for the softmax warps,
+//               and clears the dropped rows of V in shared memory, so that no NaN of theirs meets a weight of 0
+//   warps 4-7   softmax, a thread per row, which holds the row's 128 scores in registers
+//
+// Bound by the exponentials: 16 per clock and SM on the special-function unit is 1024 clocks per 128 x 128
+// scores (the products take 512 at 64 elements per head), so one in kPolyEvery pairs is computed by a polynomial
+// on the FMA pipes instead.
 // ---------------------------------------------------------------------------------------
 template <int DP>
 struct XCfg {
   static constexpr int PANELS = DP / 64, PANEL = 128 * 128;    // bytes of 128 rows x 64 elements
   static constexpr int TILE = PANELS * PANEL;
-  static constexpr int KV = DP == 64 ? 4 : 2;                  // tiles in flight of K and of V each
+  static constexpr int KV = DP == 64 ? 2 : 1;                  // tiles in flight of K and of V each
+  static constexpr bool kOwnP = DP == 64;
+  static constexpr uint32_t P_COL = kOwnP ? 128 : 0, O_COL = kOwnP ? 192 : 128;
   static constexpr int V_OFF = 0, K_OFF = KV * TILE, Q_OFF = 2 * KV * TILE;
-  static constexpr int RED_OFF = Q_OFF + 2 * TILE;             // {maximum, sum} per slot and row
-  static constexpr int BAR_OFF = RED_OFF + 2 * 128 * 8;
-  static constexpr int NBAR = 5 * KV + 1 + 2 * 3;
+  static constexpr int MASK_OFF = Q_OFF + TILE;                // per tile in flight: 128 words and a flag (all kept)
+  static constexpr int MASK = 128 * 4 + 16;
+  static constexpr int BAR_OFF = MASK_OFF + KV * MASK;
+  static constexpr int NBAR = 5 * KV + 5;
   static constexpr int SMEM = 1024 + BAR_OFF + 8 * NBAR + 16;
-  static constexpr int THREADS = 384;
-  static constexpr int kLaunchRegs = 168, kControlRegs = 40, kSoftRegs = 232;
-  static_assert(128 * kControlRegs + 256 * kSoftRegs <= THREADS * kLaunchRegs, "register split");
-  static_assert(SMEM <= 227 * 1024, "shared memory");
-  static_assert(2 * 128 * DP * 4 <= 2 * KV * TILE, "the joined outputs reuse the K and V tiles");
+  static constexpr int THREADS = 256;
+  static constexpr int kLaunchRegs = 128, kControlRegs = 40, kSoftRegs = 216;
+  static_assert(128 * kControlRegs + 128 * kSoftRegs <= THREADS * kLaunchRegs, "register split");
+  static_assert(SMEM <= 113 * 1024, "two CTAs share an SM");
 };
 
 VF4_DEV void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t* r) {
@@ -317,8 +323,38 @@ VF4_DEV void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
+// max(a, b, c), NaN if any is: a NaN score has to reach its row's maximum, whose whole row it makes NaN
+VF4_DEV float max3nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of a pair on the FMA pipes: x = j + f with j the nearest integer (by adding 1.5 * 2^23) and |f| <= 1/2,
+// 2^f by the degree-4 polynomial of least relative error (2.6e-6, fitted on that interval), j added to the
+// exponent.  x below -126 counts as -126; a NaN's row is NaN already through its maximum.
+VF4_DEV unsigned long long ex2_poly_x2(unsigned long long x) {
+  float x0, x1;
+  f32x2_unpack(x, &x0, &x1);
+  const unsigned long long v = f32x2_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const unsigned long long big = f32x2_pack(12582912.f, 12582912.f), nbig = f32x2_pack(-12582912.f, -12582912.f);
+  const unsigned long long t = add_f32x2(v, big), j = add_f32x2(t, nbig);
+  const unsigned long long f = fma_f32x2(j, f32x2_pack(-1.f, -1.f), v);
+  unsigned long long y = fma_f32x2(f, f32x2_pack(0.0095701f, 0.0095701f), f32x2_pack(0.05591786f, 0.05591786f));
+  y = fma_f32x2(y, f, f32x2_pack(0.24024745f, 0.24024745f));
+  y = fma_f32x2(y, f, f32x2_pack(0.69312181f, 0.69312181f));
+  y = fma_f32x2(y, f, f32x2_pack(0.99999926f, 0.99999926f));
+  float y0, y1, t0, t1;
+  f32x2_unpack(y, &y0, &y1);
+  f32x2_unpack(t, &t0, &t1);
+  return f32x2_pack(__uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23)),
+                    __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23)));
+}
+
+constexpr int kPolyEvery = 4;
+
 template <int DP>
-__global__ void __launch_bounds__(XCfg<DP>::THREADS, 1)
+__global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
     xattn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const int k_bm,
                     const int k_hm, const int v_bm, const int v_hm, const XParams p) {
   using C = XCfg<DP>;
@@ -331,11 +367,9 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 1)
   auto k_free = [&](int i) { return bar + 8u * (C::KV + i); };
   auto v_full = [&](int i) { return bar + 8u * (2 * C::KV + i); };
   auto v_free = [&](int i) { return bar + 8u * (3 * C::KV + i); };
-  auto v_clean = [&](int i) { return bar + 8u * (4 * C::KV + i); };   // masked rows cleared
-  const uint32_t q_full = bar + 8u * (5 * C::KV);
-  auto s_full = [&](int s) { return q_full + 8u + 24u * s; };
-  auto p_full = [&](int s) { return q_full + 16u + 24u * s; };
-  auto o_full = [&](int s) { return q_full + 24u + 24u * s; };
+  auto v_clean = [&](int i) { return bar + 8u * (4 * C::KV + i); };   // mask words written, dropped rows cleared
+  const uint32_t q_full = bar + 8u * (5 * C::KV), s_full = q_full + 8, s_free = q_full + 16, p_full = q_full + 24,
+                 o_full = q_full + 32;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + C::BAR_OFF + 8 * C::NBAR);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* err = &g_xattn_err;
@@ -343,12 +377,10 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 1)
   // this CTA's rows and keys
   const int chunk = blockIdx.x % p.chunks, tile = blockIdx.x / p.chunks % p.tiles, item = blockIdx.x / p.chunks / p.tiles;
   const int b = item / p.Hkv, hk = item - b * p.Hkv;
-  const int row0 = tile * 256, rows = min(256, p.R - row0);
-  const bool two = rows > 128;                     // two slots of rows
+  const int row0 = tile * 128, rows = min(128, p.R - row0);
   const int k0 = chunk * p.chunk, k1 = min(keys_of(p, b), k0 + p.chunk);
-  const int tiles = k1 > k0 ? (k1 - k0 + 127) / 128 : 0;
-  const int steps = two ? 2 * tiles : tiles;
-  const bool masked = p.mask != nullptr || p.lens != nullptr;
+  const int n = k1 > k0 ? (k1 - k0 + 127) / 128 : 0;   // key tiles
+  const bool masked = p.mask != nullptr || (k1 - k0) % 128 != 0;
 
   if (warp == 0 && lane == 0) {
     for (int i = 0; i < C::KV; ++i) {
@@ -358,18 +390,17 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 1)
       mbar_init(v_free(i), 1);
       mbar_init(v_clean(i), 1);
     }
-    mbar_init(q_full, two ? 256 : 128);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(s_full(s), 1);
-      mbar_init(p_full(s), 4);
-      mbar_init(o_full(s), 1);
-    }
+    mbar_init(q_full, 128);
+    mbar_init(s_full, 1);
+    mbar_init(s_free, 4);
+    mbar_init(p_full, 4);
+    mbar_init(o_full, 1);
     fence_mbar_init();
     tma_prefetch(&tmK);
     tma_prefetch(&tmV);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_alloc(smem_u32(tmem_slot), 256);
     tmem_relinquish();
   }
   fence_async_shared();
@@ -382,9 +413,11 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kControlRegs));
     const bool elected = elect_one();
     if (warp == 0) {
-      // K of tile t is needed by the first step that scores it, V one round of steps later: K0, (K1), V0, K1 / K2, ...
-      const int ahead = two ? 1 : 2;
-      auto load = [&](const CUtensorMap* m, uint32_t dst, uint32_t full, int t, int hm, int bm) {
+      // in the order of use: K0, K1, V0, K2, V1, ...
+      auto load = [&](const CUtensorMap* m, uint32_t dst, uint32_t full, uint32_t free_, int t, int hm, int bm) {
+        const int use = t / C::KV;
+        if (!__all_sync(0xFFFFFFFFu, use == 0 || mbar_wait(free_, (uint32_t)(use - 1) & 1u, err, kDevErrTimeoutEmpty)))
+          return false;
         if (elected) {
           mbar_arrive_expect_tx(full, C::TILE);
 #pragma unroll
@@ -392,113 +425,124 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 1)
             tma_load_4d(dst + c * C::PANEL, m, c * 64, k0 + t * 128, hk * hm, b * bm, full);
         }
         __syncwarp();
+        return true;
       };
       bool ok = true;
-      for (int i = -ahead; i < tiles && ok; ++i) {
-        if (i >= 0) {
-          const int s = i % C::KV, use = i / C::KV;
-          ok = __all_sync(0xFFFFFFFFu, use == 0 || mbar_wait(v_free(s), (uint32_t)(use - 1) & 1u, err, kDevErrTimeoutEmpty));
-          if (ok) load(&tmV, base + C::V_OFF + s * C::TILE, v_full(s), i, v_hm, v_bm);
-        }
-        const int t = i + ahead;
-        if (t < tiles && ok) {
-          const int s = t % C::KV, use = t / C::KV;
-          ok = __all_sync(0xFFFFFFFFu, use == 0 || mbar_wait(k_free(s), (uint32_t)(use - 1) & 1u, err, kDevErrTimeoutEmpty));
-          if (ok) load(&tmK, base + C::K_OFF + s * C::TILE, k_full(s), t, k_hm, k_bm);
-        }
+      for (int t = -1; t < n && ok; ++t) {
+        const int u = t + 1;
+        if (C::KV > 1 && u < n) ok = load(&tmK, base + C::K_OFF + u % C::KV * C::TILE, k_full(u % C::KV), k_free(u % C::KV), u, k_hm, k_bm);
+        if (ok && t >= 0) ok = load(&tmV, base + C::V_OFF + t % C::KV * C::TILE, v_full(t % C::KV), v_free(t % C::KV), t, v_hm, v_bm);
+        // one tile of each: K0, V0, K1, V1, ... (K1 waits for the scores of tile 0 only)
+        if (C::KV == 1 && u < n && ok) ok = load(&tmK, base + C::K_OFF, k_full(0), k_free(0), u, k_hm, k_bm);
       }
-      // no copy may still be writing shared memory when the CTA goes on (to join, or to exit)
+      // no copy may still be writing shared memory when the CTA exits
       if (ok)
-        for (int t = max(0, tiles - C::KV); t < tiles; ++t) {
+        for (int t = max(0, n - C::KV); t < n; ++t) {
           mbar_wait(k_full(t % C::KV), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull);
           mbar_wait(v_full(t % C::KV), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull);
         }
     } else if (warp == 1) {
       const int kd = (p.D + 15) / 16;
       const uint32_t id_s = idesc_bf16(128, false), id_o = idesc_bf16((uint32_t)kd * 16u, true);
-      bool ok = steps == 0 || __all_sync(0xFFFFFFFFu, mbar_wait(q_full, 0, err, kDevErrTimeoutFull));
-      const uint64_t qd0 = smem_desc(base + C::Q_OFF, 16, 1024, 2), kd0 = smem_desc(base + C::K_OFF, 16, 1024, 2);
+      const uint64_t qd = smem_desc(base + C::Q_OFF, 16, 1024, 2), kd0 = smem_desc(base + C::K_OFF, 16, 1024, 2);
       const uint64_t vd0 = smem_desc(base + C::V_OFF, C::PANEL, 1024, 2);
-      auto score = [&](int i) {   // S of step i
-        const int s = i & 1, t = two ? i >> 1 : i, st = t % C::KV;
-        if (!(two && s == 1))     // the second slot of a tile finds it loaded
-          ok = __all_sync(0xFFFFFFFFu, mbar_wait(k_full(st), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull));
+      bool ok = n == 0 || __all_sync(0xFFFFFFFFu, mbar_wait(q_full, 0, err, kDevErrTimeoutFull));
+      auto score = [&](int t) {   // S of tile t
+        const int st = t % C::KV;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(k_full(st), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull));
         if (!ok) return;
         tc_fence_after();
         if (elected) {
-          const uint64_t qd = qd0 + (uint32_t)((two ? s : 0) * (C::TILE >> 4)), kk0 = kd0 + (uint32_t)(st * (C::TILE >> 4));
+          const uint64_t kk0 = kd0 + (uint32_t)(st * (C::TILE >> 4));
           for (int kk = 0; kk < kd; ++kk) {
             const uint32_t off = (uint32_t)((kk >> 2) * (C::PANEL >> 4) + (kk & 3) * 2);
-            mma_f16(tmem + 128u * s, qd + off, kk0 + off, id_s, kk > 0 ? 1u : 0u);
+            mma_f16(tmem, qd + off, kk0 + off, id_s, kk > 0 ? 1u : 0u);
           }
-          tc_commit(s_full(s));
-          if (!two || s == 1) tc_commit(k_free(st));
+          tc_commit(s_full);
+          tc_commit(k_free(st));
         }
         __syncwarp();
       };
-      if (ok && steps > 0) score(0);
-      if (ok && steps > 1) score(1);
-      for (int i = 0; i < steps && ok; ++i) {
-        const int s = i & 1, t = two ? i >> 1 : i, st = t % C::KV;
+      if (ok && n > 0) score(0);
+      for (int t = 0; t < n && ok; ++t) {
+        const int st = t % C::KV;
+        if (C::kOwnP && t + 1 < n) {   // S may be overwritten once the softmax warps hold it
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(s_free, (uint32_t)t & 1u, err, kDevErrTimeoutTmem));
+          if (ok) score(t + 1);
+          if (!ok) break;
+        }
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(masked ? v_clean(st) : v_full(st), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull) &&
-                                         mbar_wait(p_full(s), (uint32_t)(i >> 1) & 1u, err, kDevErrTimeoutTmem));
+                                         mbar_wait(p_full, (uint32_t)t & 1u, err, kDevErrTimeoutTmem));
         if (!ok) break;
         tc_fence_after();
         if (elected) {
           const uint64_t vd = vd0 + (uint32_t)(st * (C::TILE >> 4));
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            mma_f16_tmem_a(tmem + 256u + 128u * s, tmem + 128u * s + 8u * kk, vd + (uint32_t)(kk * (2048 >> 4)), id_o,
-                           (i >= 2 || kk > 0) ? 1u : 0u);
-          tc_commit(o_full(s));
-          if (!two || s == 1) tc_commit(v_free(st));
+            mma_f16_tmem_a(tmem + C::O_COL, tmem + C::P_COL + 8u * kk, vd + (uint32_t)(kk * (2048 >> 4)), id_o,
+                           (t > 0 || kk > 0) ? 1u : 0u);
+          tc_commit(o_full);
+          tc_commit(v_free(st));
         }
         __syncwarp();
-        if (i + 2 < steps) score(i + 2);
+        if (!C::kOwnP && t + 1 < n) score(t + 1);
       }
-      // the tensor core must be done with shared memory before it is reused
-      if (ok)
-        for (int s = 0; s < 2; ++s) {
-          const int n = (steps + 1 - s) / 2;   // steps of slot s
-          if (n > 0) mbar_wait(o_full(s), (uint32_t)(n - 1) & 1u, err, kDevErrTimeoutDrain);
-        }
+      // the tensor core must be done with shared memory before the CTA exits
+      if (ok && n > 0) mbar_wait(o_full, (uint32_t)(n - 1) & 1u, err, kDevErrTimeoutDrain);
     } else if (warp == 2 && masked) {
       const uint8_t* mp = p.mask ? p.mask + b * p.mask_b : nullptr;
-      for (int t = 0; t < tiles; ++t) {
-        const int st = t % C::KV, j0 = k0 + t * 128;
-        bool keep[4];
+      bool keep[4], next[4];
+      auto kept = [&](int t, bool* d) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const int j = j0 + 32 * w + lane;
-          keep[w] = j < k1 && (!mp || mp[j] != 0);
+          const int j = k0 + t * 128 + 32 * w + lane;
+          d[w] = j < k1 && (!mp || mp[j] != 0);
         }
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(v_full(st), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull))) break;
+      };
+      kept(0, next);
+      for (int t = 0; t < n; ++t) {
+        const int st = t % C::KV;
+        bool all = true;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          uint32_t drop = ~__ballot_sync(0xFFFFFFFFu, keep[w]);
-          // four rows at a time, eight lanes of 16 bytes each
-          while (drop) {
-            uint32_t mine = 0;
-            bool any = false;
+          keep[w] = next[w];
+          all = all && keep[w];
+        }
+        if (t + 1 < n) kept(t + 1, next);
+        // V's arrival says that the tile before it in this place is done with, its mask words too
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(v_full(st), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull))) break;
+        uint32_t* words = reinterpret_cast<uint32_t*>(gb + C::MASK_OFF + st * C::MASK);
+        all = __all_sync(0xFFFFFFFFu, all);
+        if (lane == 0) words[128] = all;
+        if (!all) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              if (drop) {
-                const uint32_t r = (uint32_t)__ffs((int)drop) - 1u;
-                drop &= drop - 1u;
-                if ((lane >> 3) == x) {
-                  mine = r;
-                  any = true;
+          for (int w = 0; w < 4; ++w) {
+            words[32 * w + lane] = keep[w] ? ~0u : 0u;
+            uint32_t drop = ~__ballot_sync(0xFFFFFFFFu, keep[w]);
+            // four rows at a time, eight lanes of 16 bytes each
+            while (drop) {
+              uint32_t mine = 0;
+              bool any = false;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                if (drop) {
+                  const uint32_t r = (uint32_t)__ffs((int)drop) - 1u;
+                  drop &= drop - 1u;
+                  if ((lane >> 3) == x) {
+                    mine = r;
+                    any = true;
+                  }
                 }
               }
-            }
-            if (any)
+              if (any)
 #pragma unroll
-              for (int c = 0; c < C::PANELS; ++c)
-                *reinterpret_cast<uint4*>(gb + C::V_OFF + st * C::TILE + c * C::PANEL + (32 * w + mine) * 128 + (lane & 7) * 16) =
-                    make_uint4(0, 0, 0, 0);
+                for (int c = 0; c < C::PANELS; ++c)
+                  *reinterpret_cast<uint4*>(gb + C::V_OFF + st * C::TILE + c * C::PANEL + (32 * w + mine) * 128 + (lane & 7) * 16) =
+                      make_uint4(0, 0, 0, 0);
+            }
           }
+          fence_async_shared();
         }
-        fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(v_clean(st));
       }
@@ -506,49 +550,32 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 1)
     __syncwarp();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
-    const int s = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;    // slot, row of the slot
-    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lane_base + 128u * s, t_o = tmem + lane_base + 256u + 128u * s;
-    const int row = row0 + (two ? s * 128 : 0) + r;
-    const bool valid = row < p.R;
-    const bool act = (two ? s * 128 : 0) + (warp & 3) * 32 < rows;   // any valid row in this warp
-    // Q: each thread copies its own row (rows past the last as zeros)
-    if (two || s == 0) {
+    const int r = (warp & 3) * 32 + lane;    // row of the tile
+    const uint32_t t_s = tmem + ((uint32_t)((warp & 3) * 32) << 16), t_p = t_s + C::P_COL, t_o = t_s + C::O_COL;
+    const int row = row0 + r;
+    const bool valid = r < rows, act = (warp & 3) * 32 < rows;   // this row; any row of this warp
+    {  // Q: each thread copies its own row (rows past the last as zeros)
       const __nv_bfloat16* src = p.q + (valid ? q_offset(p, b, hk, row) : 0);
-      uint8_t* dst = gb + C::Q_OFF + s * C::TILE + r * 128;
+      uint8_t* dst = gb + C::Q_OFF + r * 128;
       const int pieces = (p.D + 15) / 16 * 2;
+      const uint32_t sign = p.negate ? 0x80008000u : 0u;
       for (int j = 0; j < pieces; ++j) {
         uint4 w = make_uint4(0, 0, 0, 0);
         if (valid && j * 8 < p.D) w = __ldg(reinterpret_cast<const uint4*>(src) + j);
-        if (p.negate) {
-          w.x ^= 0x80008000u;
-          w.y ^= 0x80008000u;
-          w.z ^= 0x80008000u;
-          w.w ^= 0x80008000u;
-        }
-        *reinterpret_cast<uint4*>(dst + (j >> 3) * C::PANEL + (((j & 7) ^ (r & 7)) << 4)) = w;
+        *reinterpret_cast<uint4*>(dst + (j >> 3) * C::PANEL + (((j & 7) ^ (r & 7)) << 4)) =
+            make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
       }
       fence_async_shared();
       mbar_arrive(q_full);
     }
-    const int n = (steps + 1 - s) / 2;   // steps of this slot
-    const uint8_t* mp = p.mask ? p.mask + b * p.mask_b : nullptr;
     float m = -INFINITY, l = 0.f;
-    const float grow = p.c > 0.f ? 8.f / p.c : INFINITY;
+    const float grow = 8.f / p.c;
+    const unsigned long long c2 = f32x2_pack(p.c, p.c);
     bool ok = true;
-    for (int i = 0; i < n && ok; ++i) {
-      const int j0 = k0 + (two ? i : 2 * i + s) * 128;
-      // which of the tile's keys count, 32 per word (the same for every row)
-      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
-      const bool part = mp || j0 + 128 > k1;
-      if (part) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int j = j0 + 32 * w + lane;
-          bits[w] = __ballot_sync(0xFFFFFFFFu, j < k1 && (!mp || mp[j] != 0));
-        }
-      }
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait(s_full(s), (uint32_t)i & 1u, err, kDevErrTimeoutTmem));
+    for (int t = 0; t < n && ok; ++t) {
+      const int st = t % C::KV;
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(s_full, (uint32_t)t & 1u, err, kDevErrTimeoutTmem) &&
+                                       (!masked || mbar_wait(v_clean(st), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull)));
       if (!ok) break;
       tc_fence_after();
       if (act) {
@@ -558,31 +585,47 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 1)
         tmem_wait_ld();
 #pragma unroll
         for (int w = 0; w < 8; ++w) reg_fence16(v + 16 * w);
-        if (part) {
+        if (C::kOwnP) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free);
+        }
+        if (masked) {
+          const uint32_t* words = reinterpret_cast<const uint32_t*>(gb + C::MASK_OFF + st * C::MASK);
+          if (words[128] == 0) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(bits[w] >> e & 1u)) v[32 * w + e] = 0xFF800000u;   // -inf, also in place of a NaN
+            for (int e = 0; e < 128; e += 4) {   // dropped keys: -inf, also in place of a NaN
+              const uint4 k = *reinterpret_cast<const uint4*>(words + e);
+              v[e] = (v[e] & k.x) | (~k.x & 0xFF800000u);
+              v[e + 1] = (v[e + 1] & k.y) | (~k.y & 0xFF800000u);
+              v[e + 2] = (v[e + 2] & k.z) | (~k.z & 0xFF800000u);
+              v[e + 3] = (v[e + 3] & k.w) | (~k.w & 0xFF800000u);
+            }
+          }
         }
         float mx[4];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          mx[w] = __uint_as_float(v[32 * w]);
+          mx[w] = max3nan(__uint_as_float(v[32 * w]), __uint_as_float(v[32 * w + 1]), __uint_as_float(v[32 * w + 31]));
 #pragma unroll
-          for (int e = 1; e < 31; e += 2) mx[w] = max3f(mx[w], __uint_as_float(v[32 * w + e]), __uint_as_float(v[32 * w + e + 1]));
-          mx[w] = fmaxf(mx[w], __uint_as_float(v[32 * w + 31]));
+          for (int e = 2; e < 30; e += 2) mx[w] = max3nan(mx[w], __uint_as_float(v[32 * w + e]), __uint_as_float(v[32 * w + e + 1]));
+          mx[w] = max3nan(mx[w], mx[w], __uint_as_float(v[32 * w + 30]));
         }
-        const float top = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]);
-        if (i == 0) {
-          m = top;
-        } else {
-          const bool up = top > m + grow || (m == -INFINITY && top > m);
-          if (__any_sync(0xFFFFFFFFu, up)) {
-            // O holds the steps before this one once their products are done
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full(s), (uint32_t)(i - 1) & 1u, err, kDevErrTimeoutTmem));
+        const float top = max3nan(max3nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+        // P's columns (and, to rescale it, O) are free once the product before is done
+        if (t > 0) {
+          if (C::kOwnP) {
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full, (uint32_t)(t - 1) & 1u, err, kDevErrTimeoutTmem));
             if (!ok) break;
             tc_fence_after();
+          }
+          const bool up = !(top <= m + grow);   // also for a NaN, and from -inf
+          if (__any_sync(0xFFFFFFFFu, up)) {
+            if (!C::kOwnP) {
+              ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full, (uint32_t)(t - 1) & 1u, err, kDevErrTimeoutTmem));
+              if (!ok) break;
+              tc_fence_after();
+            }
             const float f = !up ? 1.f : ex2_approx((m - top) * p.c);   // m = -inf: 0 (nothing was added yet)
             if (up) m = top;
             l *= f;
@@ -596,118 +639,81 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 1)
               tmem_st_32x32b_x16(t_o + c0, o);
             }
           }
+        } else {
+          m = top;
         }
         const float nm = m == -INFINITY ? 0.f : -m * p.c;
-        const unsigned long long c2 = f32x2_pack(p.c, p.c), nm2 = f32x2_pack(nm, nm);
+        const unsigned long long nm2 = f32x2_pack(nm, nm);
         unsigned long long l2[2] = {0ull, 0ull};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            float x0, x1;
-            f32x2_unpack(fma_f32x2(f32x2_pack(__uint_as_float(v[32 * w + 2 * e]), __uint_as_float(v[32 * w + 2 * e + 1])), c2, nm2),
-                         &x0, &x1);
-            const unsigned long long pr = f32x2_pack(ex2_approx(x0), ex2_approx(x1));
+            const unsigned long long x = fma_f32x2(
+                f32x2_pack(__uint_as_float(v[32 * w + 2 * e]), __uint_as_float(v[32 * w + 2 * e + 1])), c2, nm2);
+            unsigned long long pr;
+            if (e % kPolyEvery == kPolyEvery - 1) {
+              pr = ex2_poly_x2(x);
+            } else {
+              float x0, x1;
+              f32x2_unpack(x, &x0, &x1);
+              pr = f32x2_pack(ex2_approx(x0), ex2_approx(x1));
+            }
             l2[e & 1] = add_f32x2(l2[e & 1], pr);
             pk[e] = bf16x2_round(pr);
           }
-          tmem_st_32x32b_x16(t_s + 16 * w, pk);   // P over S: its 128 columns are in this thread's registers
+          tmem_st_32x32b_x16(t_p + 16 * w, pk);
         }
         float a0, a1, a2, a3;
         f32x2_unpack(l2[0], &a0, &a1);
         f32x2_unpack(l2[1], &a2, &a3);
         l += (a0 + a1) + (a2 + a3);
         tmem_wait_st();
+      } else if (C::kOwnP) {
+        if (lane == 0) mbar_arrive(s_free);
+        // not ahead of the warps with rows: their P of tile t - 1 must not be counted from this warp's tile t
+        ok = t == 0 || __all_sync(0xFFFFFFFFu, mbar_wait(o_full, (uint32_t)(t - 1) & 1u, err, kDevErrTimeoutTmem));
+        if (!ok) break;
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full(s));
+      if (lane == 0) mbar_arrive(p_full);
     }
-    // the slot's output is complete when its last product is
-    if (n > 0 && ok) ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full(s), (uint32_t)(n - 1) & 1u, err, kDevErrTimeoutTmem));
+    // O is complete when its last product is
+    if (n > 0 && ok) ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full, (uint32_t)(n - 1) & 1u, err, kDevErrTimeoutTmem));
     tc_fence_after();
-    const int64_t part_row = ((int64_t)item * p.chunks + chunk) * p.R + row;
-    if (two) {
-      if (act && ok) {
-        const float f = p.chunks > 1 ? 1.f : l > 0.f ? __fdividef(1.f, l) : (l == 0.f ? 0.f : l);
-        for (int c0 = 0; c0 < p.D; c0 += 8) {
-          uint32_t o[8];
-          tmem_ld_32x32b_x8(t_o + c0, o);
-          tmem_wait_ld();
-          asm volatile("" : "+r"(o[0]), "+r"(o[1]), "+r"(o[2]), "+r"(o[3]), "+r"(o[4]), "+r"(o[5]), "+r"(o[6]), "+r"(o[7]));
-          if (n == 0)
+    if (act && ok) {
+      const int64_t part_row = ((int64_t)item * p.chunks + chunk) * p.R + row;
+      const bool parts = p.chunks > 1;
+      const float f = l > 0.f ? __fdividef(1.f, l) : (l == 0.f ? 0.f : l);   // nothing kept: 0; NaN stays
+      __nv_bfloat16* dst = p.out + (valid ? o_offset(p, b, hk, row) : 0);
+      for (int c0 = 0; c0 < p.D; c0 += 8) {
+        uint32_t o[8];
+        tmem_ld_32x32b_x8(t_o + c0, o);
+        tmem_wait_ld();
+        asm volatile("" : "+r"(o[0]), "+r"(o[1]), "+r"(o[2]), "+r"(o[3]), "+r"(o[4]), "+r"(o[5]), "+r"(o[6]), "+r"(o[7]));
+        if (!valid) continue;
+        if (parts) {
+          if (n == 0) continue;   // the join does not read a chunk without keys
+          uint4* d = reinterpret_cast<uint4*>(p.part_o + part_row * p.D + c0);
+          d[0] = make_uint4(o[0], o[1], o[2], o[3]);
+          d[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        } else {
+          uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = 0u;
-          if (!valid) continue;
-          if (p.chunks > 1) {
-            uint4* dst = reinterpret_cast<uint4*>(p.part_o + part_row * p.D + c0);
-            dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
-          } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = l == 0.f ? 0u : bf16x2_round(f32x2_pack(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f));
-            *reinterpret_cast<uint4*>(p.out + o_offset(p, b, hk, row) + c0) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          for (int e = 0; e < 4; ++e)
+            w[e] = l == 0.f ? 0u : bf16x2_round(f32x2_pack(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f));
+          *reinterpret_cast<uint4*>(dst + c0) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        if (valid && p.chunks > 1) p.part_ml[part_row] = make_float2(m == -INFINITY ? m : m * p.c, l);
       }
-    } else {
-      // both slots hold part of the same rows: into shared memory (the K and V tiles are done with)
-      float* so = reinterpret_cast<float*>(gb) + s * 128 * DP;
-      float2* ml = reinterpret_cast<float2*>(gb + C::RED_OFF) + s * 128;
-      named_bar_sync(1, 256);   // both slots' products are complete: nothing reads the tiles any more
-      if (act && ok) {
-        for (int c0 = 0; c0 < p.D; c0 += 8) {
-          uint32_t o[8];
-          tmem_ld_32x32b_x8(t_o + c0, o);
-          tmem_wait_ld();
-          asm volatile("" : "+r"(o[0]), "+r"(o[1]), "+r"(o[2]), "+r"(o[3]), "+r"(o[4]), "+r"(o[5]), "+r"(o[6]), "+r"(o[7]));
-#pragma unroll
-          for (int e = 0; e < 8; ++e) so[(c0 + e) * 128 + r] = n == 0 ? 0.f : __uint_as_float(o[e]);
-        }
-        ml[r] = make_float2(m == -INFINITY ? m : m * p.c, l);
-      }
-      named_bar_sync(1, 256);
-      const float2 *ml0 = reinterpret_cast<const float2*>(gb + C::RED_OFF), *ml1 = ml0 + 128;
-      const float* so0 = reinterpret_cast<const float*>(gb);
-      const int et = threadIdx.x - 128, er = et & 127;
-      if (er < rows && ok) {
-        const float2 x = ml0[er], y = ml1[er];
-        const float mx = fmaxf(x.x, y.x), ms = mx == -INFINITY ? 0.f : mx;
-        const float f0 = ex2_approx(x.x - ms), f1 = ex2_approx(y.x - ms);
-        const float ls = fmaf(x.y, f0, y.y * f1);
-        const float f = p.chunks > 1 ? 1.f : ls > 0.f ? __fdividef(1.f, ls) : (ls == 0.f ? 0.f : ls);
-        const int64_t prow = ((int64_t)item * p.chunks + chunk) * p.R + row0 + er;
-        for (int c0 = (et >> 7) * 8; c0 < p.D; c0 += 16) {
-          float o[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int at = (c0 + e) * 128 + er;
-            // a slot without kept keys holds 0 * f
-            o[e] = (fmaf(so0[at], f0, so0[128 * DP + at] * f1)) * f;
-          }
-          if (p.chunks > 1) {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + prow * p.D + c0);
-            dst[0] = make_float4(o[0], o[1], o[2], o[3]);
-            dst[1] = make_float4(o[4], o[5], o[6], o[7]);
-          } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = bf16x2_round(f32x2_pack(o[2 * e], o[2 * e + 1]));
-            *reinterpret_cast<uint4*>(p.out + o_offset(p, b, hk, row0 + er) + c0) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-        if (p.chunks > 1 && et < 128) p.part_ml[prow] = make_float2(mx, ls);
-      }
+      if (valid && parts) p.part_ml[part_row] = make_float2(m == -INFINITY ? m : m * p.c, l);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  if (warp == 1) tmem_dealloc(tmem, 256);
 }
 
 // K or V as (elements, keys, heads, images); a dimension of stride 0 (or of one entry) is given extent 1 and its
@@ -729,15 +735,18 @@ static int make_kv_map(CUtensorMap* m, const void* ptr, const XParams& p, int64_
   return VF4_OK;
 }
 
-// Rows that the plain kernel takes: it reads each key once for all of them but pays 4 FMAs per element and row
-// pair; from 5 rows on the tensor core is faster.
-constexpr int kPlainRows = 4;
+// The plain kernel takes up to 4 rows over short keys, where a CTA of the tensor-core kernel would spend most of
+// its time starting and ending; with long keys the tensor copies read faster than its lanes do.
+constexpr int kPlainRows = 4, kPlainKeys = 1024;
+static bool plain_rows(int64_t R, int64_t Skv) { return R <= kPlainRows && Skv <= kPlainKeys; }
 
 // How many keys a CTA takes, and how many CTAs share a row tile (1: no workspace).
-static void plan_chunks(int64_t B, int64_t Hkv, int64_t R, int64_t Skv, int sms, int* chunk, int* chunks) {
-  const int64_t items = B * Hkv * (R <= kPlainRows ? 1 : (R + 255) / 256);
-  // plain kernel: 8 CTAs of 128 threads per SM, at least 256 keys each; tcgen05: one CTA per SM, at least 512
-  const int64_t want = R <= kPlainRows ? (int64_t)sms * 8 : sms, least = R <= kPlainRows ? 256 : 512;
+static void plan_chunks(int64_t B, int64_t Hkv, int64_t R, int64_t Skv, bool ragged, int sms, int* chunk, int* chunks) {
+  const bool plain = plain_rows(R, Skv);
+  const int64_t items = B * Hkv * (plain ? 1 : (R + 127) / 128);
+  // plain kernel: 4 CTAs of 128 threads per SM, at least 256 keys each; tcgen05: two CTAs per SM, at least 512 keys,
+  // and chunks of a third of that share where the images' key counts differ
+  const int64_t want = plain ? (int64_t)sms * 4 : (int64_t)sms * (ragged ? 6 : 2), least = plain ? 256 : 512;
   int64_t n = want / items;
   if (n > (Skv + least - 1) / least) n = (Skv + least - 1) / least;
   if (n < 1) n = 1;
@@ -788,11 +797,11 @@ using namespace vf4;
 
 extern "C" {
 
-int64_t vf4_cross_attn_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D) {
+int64_t vf4_cross_attn_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D, int ragged) {
   if (!sizes_ok(B, H, Hkv, Sq, Skv, D) || B == 0 || Sq == 0 || Skv == 0) return 0;
   if (B > (1 << 24) || H > (1 << 16) || Sq > (1 << 24) || Skv > (1 << 30) || D > 128) return 0;   // refused by the call
   int chunk, chunks;
-  plan_chunks(B, Hkv, H / Hkv * Sq, Skv, num_sms(), &chunk, &chunks);
+  plan_chunks(B, Hkv, H / Hkv * Sq, Skv, ragged != 0, num_sms(), &chunk, &chunks);
   return chunks == 1 ? 0 : B * H * Sq * (int64_t)chunks * (D * 4 + 8);
 }
 
@@ -835,8 +844,8 @@ int vf4_cross_attn(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const v
   p.negate = scale < 0.f;
   p.c = (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
   if (p.c < 1e-30f) p.c = 1e-30f;   // a scale of 0: every finite score weighs 1, and c * -inf stays -inf
-  p.tiles = (p.R + 255) / 256;
-  plan_chunks(B, Hkv, p.R, Skv, num_sms(), &p.chunk, &p.chunks);
+  p.tiles = (p.R + 127) / 128;
+  plan_chunks(B, Hkv, p.R, Skv, kv_lens != nullptr, num_sms(), &p.chunk, &p.chunks);
   if (p.chunks > 1) {
     const int64_t rows = B * H * Sq * (int64_t)p.chunks;
     if (!workspace || workspace_bytes < rows * (D * 4 + 8))
@@ -848,7 +857,7 @@ int vf4_cross_attn(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const v
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int st = VF4_OK;
   if (Skv == 0) p.chunks = 0;   // without keys the rows are 0, which joining no chunks writes
-  else if (p.R <= kPlainRows)
+  else if (plain_rows(p.R, Skv))
     st = D <= 32 ? launch_rows<4>(p, s) : D <= 64 ? launch_rows<8>(p, s) : launch_rows<16>(p, s);
   else
     st = D <= 64 ? launch_tc<64>(p, s) : launch_tc<128>(p, s);
