@@ -518,27 +518,13 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             words[32 * w + lane] = keep[w] ? ~0u : 0u;
-            uint32_t drop = ~__ballot_sync(0xFFFFFFFFu, keep[w]);
-            // four rows at a time, eight lanes of 16 bytes each
-            while (drop) {
-              uint32_t mine = 0;
-              bool any = false;
+            if (!keep[w]) {   // the lane clears its own row, starting at a piece of its own: no bank conflicts
 #pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                if (drop) {
-                  const uint32_t r = (uint32_t)__ffs((int)drop) - 1u;
-                  drop &= drop - 1u;
-                  if ((lane >> 3) == x) {
-                    mine = r;
-                    any = true;
-                  }
-                }
-              }
-              if (any)
+              for (int c = 0; c < C::PANELS; ++c)
 #pragma unroll
-                for (int c = 0; c < C::PANELS; ++c)
-                  *reinterpret_cast<uint4*>(gb + C::V_OFF + st * C::TILE + c * C::PANEL + (32 * w + mine) * 128 + (lane & 7) * 16) =
-                      make_uint4(0, 0, 0, 0);
+                for (int x = 0; x < 8; ++x)
+                  *reinterpret_cast<uint4*>(gb + C::V_OFF + st * C::TILE + c * C::PANEL + (32 * w + lane) * 128 +
+                                            ((x + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
           }
           fence_async_shared();
