@@ -287,31 +287,37 @@ __global__ void __launch_bounds__(128) xattn_join_kernel(const XParams p) {
 //
 //   warp 0      TMA of K and V tiles (128-byte swizzle, panels of 64 elements)
 //   warp 1      TMEM allocation, MMAs
-//   warp 2      masks (with a mask or key counts): spreads each tile's kept keys to words for the softmax warps,
-//               and clears the dropped rows of V in shared memory, so that no NaN of theirs meets a weight of 0
+//   warps 2, 3  masks (with a mask or key counts): clear the dropped rows of each K and V tile in shared memory, so
+//               that none of their NaNs reaches a score or meets a weight of 0, and set the tile's extra column:
+//               S gets one more step of its product, with 1 in every query's column and 0 or -3.4e38 in each
+//               key's, so a dropped key's score is -3.4e38 without a thread of the softmax looking at the mask
+//               (which took it as long as its maximum)
 //   warps 4-7   softmax, a thread per row, which holds the row's 128 scores in registers
 //
 // Bound by the exponentials: 16 per clock and SM on the special-function unit is 1024 clocks per 128 x 128
 // scores (the products take 512 at 64 elements per head), so one in kPolyEvery pairs is computed by a polynomial
 // on the FMA pipes instead.
 // ---------------------------------------------------------------------------------------
-template <int DP>
+// kDeep: one CTA per SM with as many tiles in flight as fit, for few rows of more than 64 elements: bound by
+// memory, and half an SM holds only one tile of K and V each.
+template <int DP, bool kDeep>
 struct XCfg {
   static constexpr int PANELS = DP / 64, PANEL = 128 * 128;    // bytes of 128 rows x 64 elements
   static constexpr int TILE = PANELS * PANEL;
-  static constexpr int KV = DP == 64 ? 2 : 1;                  // tiles in flight of K and of V each
+  static constexpr int NK = kDeep ? 3 : DP == 64 ? 2 : 1, NV = kDeep ? 2 : NK;   // tiles in flight of K and of V
+  static_assert(!kDeep || DP == 128, "up to 64 elements two tiles of each fit half an SM");
   static constexpr bool kOwnP = DP == 64;
   static constexpr uint32_t P_COL = kOwnP ? 128 : 0, O_COL = kOwnP ? 192 : 128;
-  static constexpr int V_OFF = 0, K_OFF = KV * TILE, Q_OFF = 2 * KV * TILE;
-  static constexpr int MASK_OFF = Q_OFF + TILE;                // per tile in flight: 128 words and a flag (all kept)
-  static constexpr int MASK = 128 * 4 + 16;
-  static constexpr int BAR_OFF = MASK_OFF + KV * MASK;
-  static constexpr int NBAR = 5 * KV + 5;
+  static constexpr int EXT = 128 * 32;                         // the extra step: 128 rows x 16 elements, not swizzled
+  static constexpr int V_OFF = 0, K_OFF = NV * TILE, Q_OFF = (NV + NK) * TILE;
+  static constexpr int QX_OFF = Q_OFF + TILE, KX_OFF = QX_OFF + EXT;
+  static constexpr int BAR_OFF = KX_OFF + NK * EXT;
+  static constexpr int NBAR = 3 * (NK + NV) + 6;
   static constexpr int SMEM = 1024 + BAR_OFF + 8 * NBAR + 16;
-  static constexpr int THREADS = 256;
-  static constexpr int kLaunchRegs = 128, kControlRegs = 40, kSoftRegs = 216;
-  static_assert(128 * kControlRegs + 128 * kSoftRegs <= THREADS * kLaunchRegs, "register split");
-  static_assert(SMEM <= 113 * 1024, "two CTAs share an SM");
+  static constexpr int THREADS = 256, CTAS = kDeep ? 1 : 2;
+  static constexpr int kLaunchRegs = kDeep ? 232 : 128, kControlRegs = 40, kSoftRegs = 216;
+  static_assert(128 * kControlRegs + 128 * kSoftRegs <= THREADS * 128, "register split");
+  static_assert(SMEM <= (kDeep ? 227 : 113) * 1024, "shared memory");
 };
 
 VF4_DEV void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t* r) {
@@ -353,23 +359,24 @@ VF4_DEV unsigned long long ex2_poly_x2(unsigned long long x) {
 
 constexpr int kPolyEvery = 4;
 
-template <int DP>
-__global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
+template <int DP, bool kDeep>
+__global__ void __launch_bounds__(256, kDeep ? 1 : 2)
     xattn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const int k_bm,
                     const int k_hm, const int v_bm, const int v_hm, const XParams p) {
-  using C = XCfg<DP>;
+  using C = XCfg<DP, kDeep>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw0 = smem_u32(smem_raw);
   const uint32_t base = (raw0 + 1023u) & ~1023u;
   uint8_t* gb = smem_raw + (base - raw0);
   const uint32_t bar = base + C::BAR_OFF;
   auto k_full = [&](int i) { return bar + 8u * i; };
-  auto k_free = [&](int i) { return bar + 8u * (C::KV + i); };
-  auto v_full = [&](int i) { return bar + 8u * (2 * C::KV + i); };
-  auto v_free = [&](int i) { return bar + 8u * (3 * C::KV + i); };
-  auto v_clean = [&](int i) { return bar + 8u * (4 * C::KV + i); };   // mask words written, dropped rows cleared
-  const uint32_t q_full = bar + 8u * (5 * C::KV), s_full = q_full + 8, s_free = q_full + 16, p_full = q_full + 24,
-                 o_full = q_full + 32;
+  auto k_free = [&](int i) { return bar + 8u * (C::NK + i); };
+  auto k_clean = [&](int i) { return bar + 8u * (2 * C::NK + i); };   // dropped rows cleared, extra column set
+  auto v_full = [&](int i) { return bar + 8u * (3 * C::NK + i); };
+  auto v_free = [&](int i) { return bar + 8u * (3 * C::NK + C::NV + i); };
+  auto v_clean = [&](int i) { return bar + 8u * (3 * C::NK + 2 * C::NV + i); };
+  const uint32_t q_full = bar + 8u * (3 * (C::NK + C::NV)), s_full = q_full + 8, s_free = q_full + 16, p_full = q_full + 24,
+                 o_full = q_full + 32, p_half = q_full + 40;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + C::BAR_OFF + 8 * C::NBAR);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* err = &g_xattn_err;
@@ -383,9 +390,12 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
   const bool masked = p.mask != nullptr || (k1 - k0) % 128 != 0;
 
   if (warp == 0 && lane == 0) {
-    for (int i = 0; i < C::KV; ++i) {
+    for (int i = 0; i < C::NK; ++i) {
       mbar_init(k_full(i), 1);
       mbar_init(k_free(i), 1);
+      mbar_init(k_clean(i), 1);
+    }
+    for (int i = 0; i < C::NV; ++i) {
       mbar_init(v_full(i), 1);
       mbar_init(v_free(i), 1);
       mbar_init(v_clean(i), 1);
@@ -394,6 +404,7 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
     mbar_init(s_full, 1);
     mbar_init(s_free, 4);
     mbar_init(p_full, 4);
+    mbar_init(p_half, 4);
     mbar_init(o_full, 1);
     fence_mbar_init();
     tma_prefetch(&tmK);
@@ -410,12 +421,11 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kControlRegs));
+    if constexpr (!kDeep) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kControlRegs));
     const bool elected = elect_one();
     if (warp == 0) {
-      // in the order of use: K0, K1, V0, K2, V1, ...
-      auto load = [&](const CUtensorMap* m, uint32_t dst, uint32_t full, uint32_t free_, int t, int hm, int bm) {
-        const int use = t / C::KV;
+      // in the order of use: K0 (K1, K2), V0, K next, V1, ...; with one place for K its next tile follows V
+      auto load = [&](const CUtensorMap* m, uint32_t dst, uint32_t full, uint32_t free_, int use, int t, int hm, int bm) {
         if (!__all_sync(0xFFFFFFFFu, use == 0 || mbar_wait(free_, (uint32_t)(use - 1) & 1u, err, kDevErrTimeoutEmpty)))
           return false;
         if (elected) {
@@ -427,29 +437,39 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
         __syncwarp();
         return true;
       };
+      auto load_k = [&](int t) {
+        const int i = t % C::NK;
+        return load(&tmK, base + C::K_OFF + i * C::TILE, k_full(i), k_free(i), t / C::NK, t, k_hm, k_bm);
+      };
+      auto load_v = [&](int t) {
+        const int i = t % C::NV;
+        return load(&tmV, base + C::V_OFF + i * C::TILE, v_full(i), v_free(i), t / C::NV, t, v_hm, v_bm);
+      };
       bool ok = true;
-      for (int t = -1; t < n && ok; ++t) {
-        const int u = t + 1;
-        if (C::KV > 1 && u < n) ok = load(&tmK, base + C::K_OFF + u % C::KV * C::TILE, k_full(u % C::KV), k_free(u % C::KV), u, k_hm, k_bm);
-        if (ok && t >= 0) ok = load(&tmV, base + C::V_OFF + t % C::KV * C::TILE, v_full(t % C::KV), v_free(t % C::KV), t, v_hm, v_bm);
-        // one tile of each: K0, V0, K1, V1, ... (K1 waits for the scores of tile 0 only)
-        if (C::KV == 1 && u < n && ok) ok = load(&tmK, base + C::K_OFF, k_full(0), k_free(0), u, k_hm, k_bm);
+      int kt = 0;
+      while (kt < n && kt < C::NK && ok) ok = load_k(kt++);
+      for (int t = 0; t < n && ok; ++t) {
+        ok = load_v(t);
+        if (kt < n && ok) ok = load_k(kt++);   // K of tile t + NK, free once the scores of tile t are there
       }
       // no copy may still be writing shared memory when the CTA exits
-      if (ok)
-        for (int t = max(0, n - C::KV); t < n; ++t) {
-          mbar_wait(k_full(t % C::KV), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull);
-          mbar_wait(v_full(t % C::KV), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull);
-        }
+      if (ok) {
+        for (int t = max(0, n - C::NK); t < n; ++t)
+          mbar_wait(k_full(t % C::NK), (uint32_t)(t / C::NK) & 1u, err, kDevErrTimeoutFull);
+        for (int t = max(0, n - C::NV); t < n; ++t)
+          mbar_wait(v_full(t % C::NV), (uint32_t)(t / C::NV) & 1u, err, kDevErrTimeoutFull);
+      }
     } else if (warp == 1) {
       const int kd = (p.D + 15) / 16;
       const uint32_t id_s = idesc_bf16(128, false), id_o = idesc_bf16((uint32_t)kd * 16u, true);
       const uint64_t qd = smem_desc(base + C::Q_OFF, 16, 1024, 2), kd0 = smem_desc(base + C::K_OFF, 16, 1024, 2);
       const uint64_t vd0 = smem_desc(base + C::V_OFF, C::PANEL, 1024, 2);
+      // not swizzled: 8 rows x 16 bytes per core matrix, the step's two of them 128 bytes apart, 8-row groups 256
+      const uint64_t qx = smem_desc(base + C::QX_OFF, 128, 256, 0), kx0 = smem_desc(base + C::KX_OFF, 128, 256, 0);
       bool ok = n == 0 || __all_sync(0xFFFFFFFFu, mbar_wait(q_full, 0, err, kDevErrTimeoutFull));
       auto score = [&](int t) {   // S of tile t
-        const int st = t % C::KV;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(k_full(st), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull));
+        const int st = t % C::NK;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(masked ? k_clean(st) : k_full(st), (uint32_t)(t / C::NK) & 1u, err, kDevErrTimeoutFull));
         if (!ok) return;
         tc_fence_after();
         if (elected) {
@@ -458,6 +478,7 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
             const uint32_t off = (uint32_t)((kk >> 2) * (C::PANEL >> 4) + (kk & 3) * 2);
             mma_f16(tmem, qd + off, kk0 + off, id_s, kk > 0 ? 1u : 0u);
           }
+          if (masked) mma_f16(tmem, qx, kx0 + (uint32_t)(st * (C::EXT >> 4)), id_s, 1u);
           tc_commit(s_full);
           tc_commit(k_free(st));
         }
@@ -465,22 +486,31 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
       };
       if (ok && n > 0) score(0);
       for (int t = 0; t < n && ok; ++t) {
-        const int st = t % C::KV;
+        const int st = t % C::NV;
         if (C::kOwnP && t + 1 < n) {   // S may be overwritten once the softmax warps hold it
           ok = __all_sync(0xFFFFFFFFu, mbar_wait(s_free, (uint32_t)t & 1u, err, kDevErrTimeoutTmem));
           if (ok) score(t + 1);
           if (!ok) break;
         }
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(masked ? v_clean(st) : v_full(st), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull) &&
-                                         mbar_wait(p_full, (uint32_t)t & 1u, err, kDevErrTimeoutTmem));
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(masked ? v_clean(st) : v_full(st), (uint32_t)(t / C::NV) & 1u, err, kDevErrTimeoutFull) &&
+                                         mbar_wait(p_half, (uint32_t)t & 1u, err, kDevErrTimeoutTmem));
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t vd = vd0 + (uint32_t)(st * (C::TILE >> 4));
+        if (elected) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f16_tmem_a(tmem + C::O_COL, tmem + C::P_COL + 8u * kk, vd + (uint32_t)(kk * (2048 >> 4)), id_o,
+                           (t > 0 || kk > 0) ? 1u : 0u);
+        }
+        __syncwarp();
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(p_full, (uint32_t)t & 1u, err, kDevErrTimeoutTmem));
         if (!ok) break;
         tc_fence_after();
         if (elected) {
-          const uint64_t vd = vd0 + (uint32_t)(st * (C::TILE >> 4));
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            mma_f16_tmem_a(tmem + C::O_COL, tmem + C::P_COL + 8u * kk, vd + (uint32_t)(kk * (2048 >> 4)), id_o,
-                           (t > 0 || kk > 0) ? 1u : 0u);
+          for (int kk = 4; kk < 8; ++kk)
+            mma_f16_tmem_a(tmem + C::O_COL, tmem + C::P_COL + 8u * kk, vd + (uint32_t)(kk * (2048 >> 4)), id_o, 1u);
           tc_commit(o_full);
           tc_commit(v_free(st));
         }
@@ -489,67 +519,71 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
       }
       // the tensor core must be done with shared memory before the CTA exits
       if (ok && n > 0) mbar_wait(o_full, (uint32_t)(n - 1) & 1u, err, kDevErrTimeoutDrain);
-    } else if (warp == 2 && masked) {
+    } else if (masked) {
+      const bool is_k = warp == 2;   // warp 2: K and its extra column, warp 3: V
       const uint8_t* mp = p.mask ? p.mask + b * p.mask_b : nullptr;
-      bool keep[4], next[4];
-      auto kept = [&](int t, bool* d) {
+      bool next[4];
+      auto kept = [&](int t) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int j = k0 + t * 128 + 32 * w + lane;
-          d[w] = j < k1 && (!mp || mp[j] != 0);
+          next[w] = j < k1 && (!mp || mp[j] != 0);
         }
       };
-      kept(0, next);
+      if (is_k)   // the extra step's other columns are 0: the second core matrix of every 8-row group
+        for (int i = lane; i < C::NK * 128; i += 32)
+          *reinterpret_cast<uint4*>(gb + C::KX_OFF + (i >> 3) * 256 + 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+      kept(0);
       for (int t = 0; t < n; ++t) {
-        const int st = t % C::KV;
-        bool all = true;
+        const int use = is_k ? t / C::NK : t / C::NV, st = is_k ? t % C::NK : t % C::NV;
+        bool keep[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) keep[w] = next[w];
+        if (t + 1 < n) kept(t + 1);
+        // a tile's arrival also says that the one before it in this place is done with
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(is_k ? k_full(st) : v_full(st), (uint32_t)use & 1u, err, kDevErrTimeoutFull))) break;
+        uint8_t* at = gb + (is_k ? C::K_OFF : C::V_OFF) + st * C::TILE;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          keep[w] = next[w];
-          all = all && keep[w];
-        }
-        if (t + 1 < n) kept(t + 1, next);
-        // V's arrival says that the tile before it in this place is done with, its mask words too
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(v_full(st), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull))) break;
-        uint32_t* words = reinterpret_cast<uint32_t*>(gb + C::MASK_OFF + st * C::MASK);
-        all = __all_sync(0xFFFFFFFFu, all);
-        if (lane == 0) words[128] = all;
-        if (!all) {
+          const int j = 32 * w + lane;
+          if (is_k)   // 0xFF7F: -3.39e38, the lowest bf16
+            *reinterpret_cast<uint4*>(gb + C::KX_OFF + st * C::EXT + (j >> 3) * 256 + (j & 7) * 16) =
+                make_uint4(keep[w] ? 0u : 0xFF7Fu, 0, 0, 0);
+          if (!keep[w]) {   // the lane clears its own row, starting at a piece of its own: no bank conflicts
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            words[32 * w + lane] = keep[w] ? ~0u : 0u;
-            if (!keep[w]) {   // the lane clears its own row, starting at a piece of its own: no bank conflicts
+            for (int c = 0; c < C::PANELS; ++c)
 #pragma unroll
-              for (int c = 0; c < C::PANELS; ++c)
-#pragma unroll
-                for (int x = 0; x < 8; ++x)
-                  *reinterpret_cast<uint4*>(gb + C::V_OFF + st * C::TILE + c * C::PANEL + (32 * w + lane) * 128 +
-                                            ((x + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
+              for (int x = 0; x < 8; ++x)
+                *reinterpret_cast<uint4*>(at + c * C::PANEL + j * 128 + ((x + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
-          fence_async_shared();
         }
+        fence_async_shared();
         __syncwarp();
-        if (lane == 0) mbar_arrive(v_clean(st));
+        if (lane == 0) mbar_arrive(is_k ? k_clean(st) : v_clean(st));
       }
     }
     __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
+    if constexpr (!kDeep) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
     const int r = (warp & 3) * 32 + lane;    // row of the tile
     const uint32_t t_s = tmem + ((uint32_t)((warp & 3) * 32) << 16), t_p = t_s + C::P_COL, t_o = t_s + C::O_COL;
     const int row = row0 + r;
     const bool valid = r < rows, act = (warp & 3) * 32 < rows;   // this row; any row of this warp
-    {  // Q: each thread copies its own row (rows past the last as zeros)
-      const __nv_bfloat16* src = p.q + (valid ? q_offset(p, b, hk, row) : 0);
+    {  // Q: each thread copies its own row (rows past the last, and elements up to a multiple of 16, as zeros)
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + (valid ? q_offset(p, b, hk, row) : 0));
       uint8_t* dst = gb + C::Q_OFF + r * 128;
-      const int pieces = (p.D + 15) / 16 * 2;
       const uint32_t sign = p.negate ? 0x80008000u : 0u;
-      for (int j = 0; j < pieces; ++j) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (valid && j * 8 < p.D) w = __ldg(reinterpret_cast<const uint4*>(src) + j);
+      uint4 w[8 * C::PANELS];
+#pragma unroll
+      for (int j = 0; j < 8 * C::PANELS; ++j) w[j] = valid && j * 8 < p.D ? __ldg(src + j) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 8 * C::PANELS; ++j)
         *reinterpret_cast<uint4*>(dst + (j >> 3) * C::PANEL + (((j & 7) ^ (r & 7)) << 4)) =
-            make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
+            make_uint4(w[j].x ^ sign, w[j].y ^ sign, w[j].z ^ sign, w[j].w ^ sign);
+      if (masked) {   // the extra step: 1 in the first column
+        uint8_t* x = gb + C::QX_OFF + (r >> 3) * 256 + (r & 7) * 16;
+        *reinterpret_cast<uint4*>(x) = make_uint4(0x3F80u, 0, 0, 0);
+        *reinterpret_cast<uint4*>(x + 128) = make_uint4(0, 0, 0, 0);
       }
       fence_async_shared();
       mbar_arrive(q_full);
@@ -559,9 +593,7 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
     const unsigned long long c2 = f32x2_pack(p.c, p.c);
     bool ok = true;
     for (int t = 0; t < n && ok; ++t) {
-      const int st = t % C::KV;
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait(s_full, (uint32_t)t & 1u, err, kDevErrTimeoutTmem) &&
-                                       (!masked || mbar_wait(v_clean(st), (uint32_t)(t / C::KV) & 1u, err, kDevErrTimeoutFull)));
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(s_full, (uint32_t)t & 1u, err, kDevErrTimeoutTmem));
       if (!ok) break;
       tc_fence_after();
       if (act) {
@@ -576,19 +608,6 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
           __syncwarp();
           if (lane == 0) mbar_arrive(s_free);
         }
-        if (masked) {
-          const uint32_t* words = reinterpret_cast<const uint32_t*>(gb + C::MASK_OFF + st * C::MASK);
-          if (words[128] == 0) {
-#pragma unroll
-            for (int e = 0; e < 128; e += 4) {   // dropped keys: -inf, also in place of a NaN
-              const uint4 k = *reinterpret_cast<const uint4*>(words + e);
-              v[e] = (v[e] & k.x) | (~k.x & 0xFF800000u);
-              v[e + 1] = (v[e + 1] & k.y) | (~k.y & 0xFF800000u);
-              v[e + 2] = (v[e + 2] & k.z) | (~k.z & 0xFF800000u);
-              v[e + 3] = (v[e + 3] & k.w) | (~k.w & 0xFF800000u);
-            }
-          }
-        }
         float mx[4];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -597,21 +616,23 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
           for (int e = 2; e < 30; e += 2) mx[w] = max3nan(mx[w], __uint_as_float(v[32 * w + e]), __uint_as_float(v[32 * w + e + 1]));
           mx[w] = max3nan(mx[w], mx[w], __uint_as_float(v[32 * w + 30]));
         }
-        const float top = max3nan(max3nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-        // P's columns (and, to rescale it, O) are free once the product before is done
-        if (t > 0) {
-          if (C::kOwnP) {
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full, (uint32_t)(t - 1) & 1u, err, kDevErrTimeoutTmem));
-            if (!ok) break;
-            tc_fence_after();
-          }
+        float top = max3nan(max3nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+        if (top < -1e38f) top = -INFINITY;   // every key so far is dropped
+        bool ready = t == 0;                 // the product of the tile before is done: O and P's columns are free
+        auto finish_previous = [&]() {
+          if (ready) return true;
+          ready = true;
+          const bool done = __all_sync(0xFFFFFFFFu, mbar_wait(o_full, (uint32_t)(t - 1) & 1u, err, kDevErrTimeoutTmem));
+          tc_fence_after();
+          return done;
+        };
+        if (t == 0) {
+          m = top;
+        } else {
           const bool up = !(top <= m + grow);   // also for a NaN, and from -inf
           if (__any_sync(0xFFFFFFFFu, up)) {
-            if (!C::kOwnP) {
-              ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full, (uint32_t)(t - 1) & 1u, err, kDevErrTimeoutTmem));
-              if (!ok) break;
-              tc_fence_after();
-            }
+            ok = finish_previous();
+            if (!ok) break;
             const float f = !up ? 1.f : ex2_approx((m - top) * p.c);   // m = -inf: 0 (nothing was added yet)
             if (up) m = top;
             l *= f;
@@ -625,19 +646,16 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
               tmem_st_32x32b_x16(t_o + c0, o);
             }
           }
-        } else {
-          m = top;
         }
         const float nm = m == -INFINITY ? 0.f : -m * p.c;
         const unsigned long long nm2 = f32x2_pack(nm, nm);
         unsigned long long l2[2] = {0ull, 0ull};
+        // P in place of the scores: pair i of the registers becomes word i
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t pk[16];
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const unsigned long long x = fma_f32x2(
-                f32x2_pack(__uint_as_float(v[32 * w + 2 * e]), __uint_as_float(v[32 * w + 2 * e + 1])), c2, nm2);
+          for (int e = 32 * h; e < 32 * h + 32; ++e) {
+            const unsigned long long x = fma_f32x2(f32x2_pack(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), c2, nm2);
             unsigned long long pr;
             if (e % kPolyEvery == kPolyEvery - 1) {
               pr = ex2_poly_x2(x);
@@ -647,10 +665,22 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
               pr = f32x2_pack(ex2_approx(x0), ex2_approx(x1));
             }
             l2[e & 1] = add_f32x2(l2[e & 1], pr);
-            pk[e] = bf16x2_round(pr);
+            v[e] = bf16x2_round(pr);
           }
-          tmem_st_32x32b_x16(t_p + 16 * w, pk);
+          if (h == 0) {
+            if (C::kOwnP) ok = finish_previous();
+            if (!ok) break;
+          }
+          tmem_st_32x32b_x16(t_p + 32 * h, v + 32 * h);
+          tmem_st_32x32b_x16(t_p + 32 * h + 16, v + 32 * h + 16);
+          if (h == 0) {   // the first half of the product starts while the second half of P is computed
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_half);
+          }
         }
+        if (!ok) break;
         float a0, a1, a2, a3;
         f32x2_unpack(l2[0], &a0, &a1);
         f32x2_unpack(l2[1], &a2, &a3);
@@ -661,6 +691,9 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
         // not ahead of the warps with rows: their P of tile t - 1 must not be counted from this warp's tile t
         ok = t == 0 || __all_sync(0xFFFFFFFFu, mbar_wait(o_full, (uint32_t)(t - 1) & 1u, err, kDevErrTimeoutTmem));
         if (!ok) break;
+        if (lane == 0) mbar_arrive(p_half);
+      } else {
+        if (lane == 0) mbar_arrive(p_half);
       }
       tc_fence_before();
       __syncwarp();
@@ -674,23 +707,29 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
       const bool parts = p.chunks > 1;
       const float f = l > 0.f ? __fdividef(1.f, l) : (l == 0.f ? 0.f : l);   // nothing kept: 0; NaN stays
       __nv_bfloat16* dst = p.out + (valid ? o_offset(p, b, hk, row) : 0);
-      for (int c0 = 0; c0 < p.D; c0 += 8) {
-        uint32_t o[8];
-        tmem_ld_32x32b_x8(t_o + c0, o);
-        tmem_wait_ld();
-        asm volatile("" : "+r"(o[0]), "+r"(o[1]), "+r"(o[2]), "+r"(o[3]), "+r"(o[4]), "+r"(o[5]), "+r"(o[6]), "+r"(o[7]));
-        if (!valid) continue;
-        if (parts) {
-          if (n == 0) continue;   // the join does not read a chunk without keys
-          uint4* d = reinterpret_cast<uint4*>(p.part_o + part_row * p.D + c0);
-          d[0] = make_uint4(o[0], o[1], o[2], o[3]);
-          d[1] = make_uint4(o[4], o[5], o[6], o[7]);
-        } else {
-          uint32_t w[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = l == 0.f ? 0u : bf16x2_round(f32x2_pack(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f));
-          *reinterpret_cast<uint4*>(dst + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int c0 = 0; c0 < DP; c0 += 32) {
+        if (c0 >= p.D) break;
+        uint32_t o[32];   // columns past D hold products with the tile's zero padding, or nothing
+        tmem_ld_32x32b_x32(t_o + c0, o);
+        tmem_wait_ld();
+        reg_fence16(o);
+        reg_fence16(o + 16);
+        if (!valid || (parts && n == 0)) continue;   // the join does not read a chunk without keys
+#pragma unroll
+        for (int c = 0; c < 32; c += 8) {
+          if (c0 + c >= p.D) break;
+          if (parts) {
+            uint4* d = reinterpret_cast<uint4*>(p.part_o + part_row * p.D + c0 + c);
+            d[0] = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+            d[1] = make_uint4(o[c + 4], o[c + 5], o[c + 6], o[c + 7]);
+          } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = l == 0.f ? 0u : bf16x2_round(f32x2_pack(__uint_as_float(o[c + 2 * e]) * f, __uint_as_float(o[c + 2 * e + 1]) * f));
+            *reinterpret_cast<uint4*>(dst + c0 + c) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
         }
       }
       if (valid && parts) p.part_ml[part_row] = make_float2(m == -INFINITY ? m : m * p.c, l);
@@ -726,13 +765,19 @@ static int make_kv_map(CUtensorMap* m, const void* ptr, const XParams& p, int64_
 constexpr int kPlainRows = 4, kPlainKeys = 1024;
 static bool plain_rows(int64_t R, int64_t Skv) { return R <= kPlainRows && Skv <= kPlainKeys; }
 
+// Rows so few that the keys' bytes, not their scores, bound the work: one CTA per SM with more tiles in flight.
+constexpr int kDeepRows = 32;
+static bool deep(int64_t R, int64_t D) { return D > 64 && R <= kDeepRows; }
+
 // How many keys a CTA takes, and how many CTAs share a row tile (1: no workspace).
-static void plan_chunks(int64_t B, int64_t Hkv, int64_t R, int64_t Skv, bool ragged, int sms, int* chunk, int* chunks) {
+static void plan_chunks(int64_t B, int64_t Hkv, int64_t R, int64_t Skv, int64_t D, bool ragged, int sms, int* chunk,
+                        int* chunks) {
   const bool plain = plain_rows(R, Skv);
   const int64_t items = B * Hkv * (plain ? 1 : (R + 127) / 128);
-  // plain kernel: 4 CTAs of 128 threads per SM, at least 256 keys each; tcgen05: two CTAs per SM, at least 512 keys,
-  // and chunks of a third of that share where the images' key counts differ
-  const int64_t want = plain ? (int64_t)sms * 4 : (int64_t)sms * (ragged ? 6 : 2), least = plain ? 256 : 512;
+  // plain kernel: 4 CTAs of 128 threads per SM, at least 256 keys each; tcgen05: as many CTAs as are resident at
+  // once, at least 512 keys each, and twice as many where the images' key counts differ
+  const int64_t want = plain ? (int64_t)sms * 4 : (int64_t)sms * (deep(R, D) ? 1 : 2) * (ragged ? 2 : 1);
+  const int64_t least = plain ? 256 : 512;
   int64_t n = want / items;
   if (n > (Skv + least - 1) / least) n = (Skv + least - 1) / least;
   if (n < 1) n = 1;
@@ -743,20 +788,20 @@ static void plan_chunks(int64_t B, int64_t Hkv, int64_t R, int64_t Skv, bool rag
   if (*chunks < 1) *chunks = 1;
 }
 
-template <int DP>
+template <int DP, bool kDeep>
 static int launch_tc(const XParams& p, cudaStream_t s) {
-  using C = XCfg<DP>;
+  using C = XCfg<DP, kDeep>;
   CUtensorMap tk, tv;
   int kbm, khm, vbm, vhm;
   if (int st = make_kv_map(&tk, p.k, p, p.kb, p.kh, p.ks, &kbm, &khm)) return st;
   if (int st = make_kv_map(&tv, p.v, p, p.vb, p.vh, p.vs, &vbm, &vhm)) return st;
-  auto kern = xattn_tc_kernel<DP>;
+  auto kern = xattn_tc_kernel<DP, kDeep>;
   if (int st = smem_optin(kern, C::SMEM)) return st;
   static const int regs = [] {   // the register split of the kernel relies on what its launch allocates
     cudaFuncAttributes a;
-    return cudaFuncGetAttributes(&a, xattn_tc_kernel<DP>) == cudaSuccess ? a.numRegs : 0;
+    return cudaFuncGetAttributes(&a, xattn_tc_kernel<DP, kDeep>) == cudaSuccess ? a.numRegs : 0;
   }();
-  if (regs != C::kLaunchRegs) return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: built with %d registers", regs);
+  if (!kDeep && regs != C::kLaunchRegs) return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: built with %d registers", regs);
   const int64_t grid = (int64_t)p.B * p.Hkv * p.tiles * p.chunks;
   if (grid > INT32_MAX) return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: sizes too large");
   kern<<<(unsigned)grid, C::THREADS, C::SMEM, s>>>(tk, tv, kbm, khm, vbm, vhm, p);
@@ -787,7 +832,7 @@ int64_t vf4_cross_attn_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t
   if (!sizes_ok(B, H, Hkv, Sq, Skv, D) || B == 0 || Sq == 0 || Skv == 0) return 0;
   if (B > (1 << 24) || H > (1 << 16) || Sq > (1 << 24) || Skv > (1 << 30) || D > 128) return 0;   // refused by the call
   int chunk, chunks;
-  plan_chunks(B, Hkv, H / Hkv * Sq, Skv, ragged != 0, num_sms(), &chunk, &chunks);
+  plan_chunks(B, Hkv, H / Hkv * Sq, Skv, D, ragged != 0, num_sms(), &chunk, &chunks);
   return chunks == 1 ? 0 : B * H * Sq * (int64_t)chunks * (D * 4 + 8);
 }
 
@@ -831,7 +876,7 @@ int vf4_cross_attn(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const v
   p.c = (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
   if (p.c < 1e-30f) p.c = 1e-30f;   // a scale of 0: every finite score weighs 1, and c * -inf stays -inf
   p.tiles = (p.R + 127) / 128;
-  plan_chunks(B, Hkv, p.R, Skv, kv_lens != nullptr, num_sms(), &p.chunk, &p.chunks);
+  plan_chunks(B, Hkv, p.R, Skv, D, kv_lens != nullptr, num_sms(), &p.chunk, &p.chunks);
   if (p.chunks > 1) {
     const int64_t rows = B * H * Sq * (int64_t)p.chunks;
     if (!workspace || workspace_bytes < rows * (D * 4 + 8))
@@ -846,7 +891,7 @@ int vf4_cross_attn(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const v
   else if (plain_rows(p.R, Skv))
     st = D <= 32 ? launch_rows<4>(p, s) : D <= 64 ? launch_rows<8>(p, s) : launch_rows<16>(p, s);
   else
-    st = D <= 64 ? launch_tc<64>(p, s) : launch_tc<128>(p, s);
+    st = D <= 64 ? launch_tc<64, false>(p, s) : deep(p.R, D) ? launch_tc<128, true>(p, s) : launch_tc<128, false>(p, s);
   if (st || p.chunks == 1) return st;
   const int64_t rows = B * H * Sq;
   xattn_join_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
