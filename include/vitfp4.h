@@ -392,11 +392,10 @@ VF4_API int vf4_gated_residual_norm(const void* x, int64_t ldx, const void* y, i
  *   kv_lens: NULL or (B,) int32 device values, keys j >= kv_lens[b] are not used (clamped to 0 .. Skv).
  *   key_mask: NULL or (B, Skv) bytes with rows mask_b apart, 0 = not used.  Unused keys and values may hold
  *   anything (NaN included).  A query whose keys are all unused gives 0.
- * workspace: vf4_cross_attn_workspace_size bytes (ragged: whether kv_lens is given; asked with the device current
- * that the call runs on; 0: none needed), 16-byte aligned, used
+ * workspace: vf4_cross_attn_workspace_size bytes (asked with the device current that the call runs on; 0: none
+ * needed), 16-byte aligned, used
  * until the call's work is done; calls that may overlap need one each.  Deterministic. */
-VF4_API int64_t vf4_cross_attn_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D,
-                                              int ragged);
+VF4_API int64_t vf4_cross_attn_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D);
 VF4_API int vf4_cross_attn(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const void* k, int64_t k_b, int64_t k_h,
                            int64_t k_s, const void* v, int64_t v_b, int64_t v_h, int64_t v_s, int64_t B, int64_t H,
                            int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D, float scale, const int32_t* kv_lens,

@@ -195,7 +195,7 @@ def test_workspace_is_checked():
     from vitfp4 import _lib
     q, k, v = _inputs(1, 2, 2, 1, 6000, 64)
     o = torch.full((1, 1, 2, 64), 7.0, device="cuda", dtype=torch.bfloat16)
-    n = _lib.lib().vf4_cross_attn_workspace_size(1, 2, 2, 1, 6000, 64, 0)
+    n = _lib.lib().vf4_cross_attn_workspace_size(1, 2, 2, 1, 6000, 64)
     assert n > 0
     ws = torch.empty(n, dtype=torch.uint8, device="cuda")
     args = lambda bytes_: (q.data_ptr(), *q.stride()[:3], k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], 1, 2, 2, 1, 6000,

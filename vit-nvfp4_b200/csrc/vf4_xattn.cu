@@ -298,14 +298,11 @@ __global__ void __launch_bounds__(128) xattn_join_kernel(const XParams p) {
 // scores (the products take 512 at 64 elements per head), so one in kPolyEvery pairs is computed by a polynomial
 // on the FMA pipes instead.
 // ---------------------------------------------------------------------------------------
-// kDeep: one CTA per SM with as many tiles in flight as fit, for few rows of more than 64 elements: bound by
-// memory, and half an SM holds only one tile of K and V each.
-template <int DP, bool kDeep>
+template <int DP>
 struct XCfg {
   static constexpr int PANELS = DP / 64, PANEL = 128 * 128;    // bytes of 128 rows x 64 elements
   static constexpr int TILE = PANELS * PANEL;
-  static constexpr int NK = kDeep ? 3 : DP == 64 ? 2 : 1, NV = kDeep ? 2 : NK;   // tiles in flight of K and of V
-  static_assert(!kDeep || DP == 128, "up to 64 elements two tiles of each fit half an SM");
+  static constexpr int NK = DP == 64 ? 2 : 1, NV = NK;         // tiles in flight of K and of V
   static constexpr bool kOwnP = DP == 64;
   static constexpr uint32_t P_COL = kOwnP ? 128 : 0, O_COL = kOwnP ? 192 : 128;
   static constexpr int EXT = 128 * 32;                         // the extra step: 128 rows x 16 elements, not swizzled
@@ -314,10 +311,10 @@ struct XCfg {
   static constexpr int BAR_OFF = KX_OFF + NK * EXT;
   static constexpr int NBAR = 3 * (NK + NV) + 6;
   static constexpr int SMEM = 1024 + BAR_OFF + 8 * NBAR + 16;
-  static constexpr int THREADS = 256, CTAS = kDeep ? 1 : 2;
-  static constexpr int kLaunchRegs = kDeep ? 232 : 128, kControlRegs = 40, kSoftRegs = 216;
-  static_assert(128 * kControlRegs + 128 * kSoftRegs <= THREADS * 128, "register split");
-  static_assert(SMEM <= (kDeep ? 227 : 113) * 1024, "shared memory");
+  static constexpr int THREADS = 256;
+  static constexpr int kLaunchRegs = 128, kControlRegs = 40, kSoftRegs = 216;
+  static_assert(128 * kControlRegs + 128 * kSoftRegs <= THREADS * kLaunchRegs, "register split");
+  static_assert(SMEM <= 113 * 1024, "two CTAs share an SM");
 };
 
 VF4_DEV void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t* r) {
@@ -359,11 +356,11 @@ VF4_DEV unsigned long long ex2_poly_x2(unsigned long long x) {
 
 constexpr int kPolyEvery = 4;
 
-template <int DP, bool kDeep>
-__global__ void __launch_bounds__(256, kDeep ? 1 : 2)
+template <int DP>
+__global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
     xattn_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const int k_bm,
                     const int k_hm, const int v_bm, const int v_hm, const XParams p) {
-  using C = XCfg<DP, kDeep>;
+  using C = XCfg<DP>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw0 = smem_u32(smem_raw);
   const uint32_t base = (raw0 + 1023u) & ~1023u;
@@ -421,7 +418,7 @@ __global__ void __launch_bounds__(256, kDeep ? 1 : 2)
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
 
   if (warp < 4) {
-    if constexpr (!kDeep) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kControlRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kControlRegs));
     const bool elected = elect_one();
     if (warp == 0) {
       // in the order of use: K0 (K1, K2), V0, K next, V1, ...; with one place for K its next tile follows V
@@ -564,7 +561,7 @@ __global__ void __launch_bounds__(256, kDeep ? 1 : 2)
     }
     __syncwarp();
   } else {
-    if constexpr (!kDeep) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
     const int r = (warp & 3) * 32 + lane;    // row of the tile
     const uint32_t t_s = tmem + ((uint32_t)((warp & 3) * 32) << 16), t_p = t_s + C::P_COL, t_o = t_s + C::O_COL;
     const int row = row0 + r;
@@ -765,19 +762,14 @@ static int make_kv_map(CUtensorMap* m, const void* ptr, const XParams& p, int64_
 constexpr int kPlainRows = 4, kPlainKeys = 1024;
 static bool plain_rows(int64_t R, int64_t Skv) { return R <= kPlainRows && Skv <= kPlainKeys; }
 
-// Rows so few that the keys' bytes, not their scores, bound the work: one CTA per SM with more tiles in flight.
-constexpr int kDeepRows = 32;
-static bool deep(int64_t R, int64_t D) { return D > 64 && R <= kDeepRows; }
-
 // How many keys a CTA takes, and how many CTAs share a row tile (1: no workspace).
-static void plan_chunks(int64_t B, int64_t Hkv, int64_t R, int64_t Skv, int64_t D, bool ragged, int sms, int* chunk,
-                        int* chunks) {
+static void plan_chunks(int64_t B, int64_t Hkv, int64_t R, int64_t Skv, int sms, int* chunk, int* chunks) {
   const bool plain = plain_rows(R, Skv);
   const int64_t items = B * Hkv * (plain ? 1 : (R + 127) / 128);
   // plain kernel: 4 CTAs of 128 threads per SM, at least 256 keys each; tcgen05: as many CTAs as are resident at
-  // once, at least 512 keys each, and twice as many where the images' key counts differ
-  const int64_t want = plain ? (int64_t)sms * 4 : (int64_t)sms * (deep(R, D) ? 1 : 2) * (ragged ? 2 : 1);
-  const int64_t least = plain ? 256 : 512;
+  // once, at least 512 keys each (with key counts that differ, shorter chunks would even the CTAs out, but measured
+  // slower: 4 images of up to 16391 keys, 32 heads over 8 of 128 elements: 45 us, 53 with twice as many)
+  const int64_t want = plain ? (int64_t)sms * 4 : (int64_t)sms * 2, least = plain ? 256 : 512;
   int64_t n = want / items;
   if (n > (Skv + least - 1) / least) n = (Skv + least - 1) / least;
   if (n < 1) n = 1;
@@ -788,20 +780,20 @@ static void plan_chunks(int64_t B, int64_t Hkv, int64_t R, int64_t Skv, int64_t 
   if (*chunks < 1) *chunks = 1;
 }
 
-template <int DP, bool kDeep>
+template <int DP>
 static int launch_tc(const XParams& p, cudaStream_t s) {
-  using C = XCfg<DP, kDeep>;
+  using C = XCfg<DP>;
   CUtensorMap tk, tv;
   int kbm, khm, vbm, vhm;
   if (int st = make_kv_map(&tk, p.k, p, p.kb, p.kh, p.ks, &kbm, &khm)) return st;
   if (int st = make_kv_map(&tv, p.v, p, p.vb, p.vh, p.vs, &vbm, &vhm)) return st;
-  auto kern = xattn_tc_kernel<DP, kDeep>;
+  auto kern = xattn_tc_kernel<DP>;
   if (int st = smem_optin(kern, C::SMEM)) return st;
   static const int regs = [] {   // the register split of the kernel relies on what its launch allocates
     cudaFuncAttributes a;
-    return cudaFuncGetAttributes(&a, xattn_tc_kernel<DP, kDeep>) == cudaSuccess ? a.numRegs : 0;
+    return cudaFuncGetAttributes(&a, xattn_tc_kernel<DP>) == cudaSuccess ? a.numRegs : 0;
   }();
-  if (!kDeep && regs != C::kLaunchRegs) return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: built with %d registers", regs);
+  if (regs != C::kLaunchRegs) return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: built with %d registers", regs);
   const int64_t grid = (int64_t)p.B * p.Hkv * p.tiles * p.chunks;
   if (grid > INT32_MAX) return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: sizes too large");
   kern<<<(unsigned)grid, C::THREADS, C::SMEM, s>>>(tk, tv, kbm, khm, vbm, vhm, p);
@@ -828,11 +820,11 @@ using namespace vf4;
 
 extern "C" {
 
-int64_t vf4_cross_attn_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D, int ragged) {
+int64_t vf4_cross_attn_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D) {
   if (!sizes_ok(B, H, Hkv, Sq, Skv, D) || B == 0 || Sq == 0 || Skv == 0) return 0;
   if (B > (1 << 24) || H > (1 << 16) || Sq > (1 << 24) || Skv > (1 << 30) || D > 128) return 0;   // refused by the call
   int chunk, chunks;
-  plan_chunks(B, Hkv, H / Hkv * Sq, Skv, D, ragged != 0, num_sms(), &chunk, &chunks);
+  plan_chunks(B, Hkv, H / Hkv * Sq, Skv, num_sms(), &chunk, &chunks);
   return chunks == 1 ? 0 : B * H * Sq * (int64_t)chunks * (D * 4 + 8);
 }
 
@@ -876,7 +868,7 @@ int vf4_cross_attn(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const v
   p.c = (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
   if (p.c < 1e-30f) p.c = 1e-30f;   // a scale of 0: every finite score weighs 1, and c * -inf stays -inf
   p.tiles = (p.R + 127) / 128;
-  plan_chunks(B, Hkv, p.R, Skv, D, kv_lens != nullptr, num_sms(), &p.chunk, &p.chunks);
+  plan_chunks(B, Hkv, p.R, Skv, num_sms(), &p.chunk, &p.chunks);
   if (p.chunks > 1) {
     const int64_t rows = B * H * Sq * (int64_t)p.chunks;
     if (!workspace || workspace_bytes < rows * (D * 4 + 8))
@@ -891,7 +883,7 @@ int vf4_cross_attn(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const v
   else if (plain_rows(p.R, Skv))
     st = D <= 32 ? launch_rows<4>(p, s) : D <= 64 ? launch_rows<8>(p, s) : launch_rows<16>(p, s);
   else
-    st = D <= 64 ? launch_tc<64, false>(p, s) : deep(p.R, D) ? launch_tc<128, true>(p, s) : launch_tc<128, false>(p, s);
+    st = D <= 64 ? launch_tc<64>(p, s) : launch_tc<128>(p, s);
   if (st || p.chunks == 1) return st;
   const int64_t rows = B * H * Sq;
   xattn_join_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);

@@ -689,7 +689,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
     out = torch.empty_strided((B, H, Sq, D), (Sq * H * D, D, H * D, 1), dtype=torch.bfloat16, device=q.device)
     if B == 0 or Sq == 0:
         return out
-    n = _lib.lib().vf4_cross_attn_workspace_size(B, H, Hkv, Sq, Skv, D, kv_lens is not None)
+    n = _lib.lib().vf4_cross_attn_workspace_size(B, H, Hkv, Sq, Skv, D)
     ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=q.device) if n else None
     qb, qh, qs, _ = q.stride()
     kb, kh, ks, _ = k.stride()
