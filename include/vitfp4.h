@@ -371,7 +371,8 @@ VF4_API int vf4_linear_fp8_block(const void* x, int dtype, int64_t M, int64_t K,
  *   x' = x + residual_scale * gate (.) N_post(y)        h = N_pre(x')
  * x, y: (M, K) rows of ldx / ldy elements, both of dtype (VF4_BF16 or VF4_F32); K <= 16384.  post / pre: 0 none,
  * 1 LayerNorm, 2 RMSNorm, with optional (K,) weight and bias; gate: (gate_groups, K), row m using group
- * m / (M / gate_groups), or NULL; gate, weights and biases all of param_dtype.  All arithmetic in fp32; x'
+ * m / (M / gate_groups), or NULL; gate, weights and biases all of param_dtype
+ * (VF4_F32, or dtype).  All arithmetic in fp32; x'
  * (M, K) is rounded once to dtype and enters N_pre before that rounding.  h: (M, K) in dtype, or (h_fp8) codes
  * in rows of ldc bytes with scales at m * stride_m + (column / 128) * stride_k as vf4_cast_fp8_block writes them,
  * cast from the fp32 values.  y NULL: h = N_pre(x) alone (x_out unused).  pre 0: x' alone.  x_out may be x

@@ -11,6 +11,7 @@
 // A row lives in the registers of its threads (8 consecutive columns per thread and step, so that 16 lanes
 // hold a block of 128).  Each thread takes the mean and the squared deviations of its own values, one pass
 // over the threads joins them, all in fp32; x' enters the second norm before it is rounded for storage.
+// Bound by memory for fp32 rows (65792 x 1024: 5.1 TB/s); bf16 rows by their instructions as much (106 us, 5.1 TB/s).
 #include "vf4_fp8_block.cuh"
 #include "vf4_host.h"
 
@@ -22,7 +23,7 @@ struct NormParams {
   const void *x, *y, *gate, *w2, *b2, *w1, *b1;   // w2 / b2: post-norm, w1 / b1: pre-norm; NULL: 1 / 0
   int64_t M, ldx, ldy;
   uint32_t rows_per_gate;
-  int K, post, pre, p_f32;     // p_f32: the parameters' type (gate, weights, biases)
+  int K, post, pre;
   float rs, eps;
   void *x_out, *h;
   int64_t ldc;                 // FP8 output: bytes per code row
@@ -30,142 +31,195 @@ struct NormParams {
   int64_t s_m, s_k;
 };
 
-// Eight parameter values from column col (nv valid), of either type.
-template <bool kVec>
-VF4_DEV void param8(const void* base, int64_t at, int f32, int nv, float* v) {
-  if (f32) load8<float, kVec>(static_cast<const float*>(base) + at, nv, v);
-  else load8<__nv_bfloat16, kVec>(static_cast<const __nv_bfloat16*>(base) + at, nv, v);
+// Eight consecutive values as four pairs: the arithmetic below runs on pairs (one issue slot for two
+// elements; in scalars the bf16 rows were bound by instruction issue, not by memory).
+using Pair = unsigned long long;
+VF4_DEV Pair both(float a) { return f32x2_pack(a, a); }
+
+template <typename T, bool kVec>
+VF4_DEV void pairs8(const Raw8<T, kVec>& r, Pair* v) {
+  if constexpr (kVec && sizeof(T) == 2) {
+    v[0] = bf16x2_to_f32x2(r.w.x);
+    v[1] = bf16x2_to_f32x2(r.w.y);
+    v[2] = bf16x2_to_f32x2(r.w.z);
+    v[3] = bf16x2_to_f32x2(r.w.w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = f32x2_pack(r.v[2 * i], r.v[2 * i + 1]);
+  }
+}
+
+// Eight parameter values from element `at` on (nv valid).
+template <typename P, bool kVec>
+VF4_DEV void param8(const void* base, int64_t at, int nv, Pair* v) {
+  Raw8<P, kVec> r;
+  r.load(static_cast<const P*>(base) + at, nv);
+  pairs8(r, v);
 }
 
 template <typename T, bool kVec>
-VF4_DEV void store_row8(T* p, int nv, const float* v) {
+VF4_DEV void store_row8(T* p, int nv, const Pair* v) {
   if (kVec && nv == 8) {
     if constexpr (sizeof(T) == 2) {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = bf16x2_round(f32x2_pack(v[2 * i], v[2 * i + 1]));
-      *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(p) = make_uint4(bf16x2_round(v[0]), bf16x2_round(v[1]), bf16x2_round(v[2]), bf16x2_round(v[3]));
     } else {
-      reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f32x2_unpack(v[i], &f[2 * i], &f[2 * i + 1]);
+      reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+      reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
     }
   } else {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f32x2_unpack(v[i], &f[2 * i], &f[2 * i + 1]);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < nv) p[i] = (T)v[i];
+      if (i < nv) p[i] = (T)f[i];
   }
 }
 
-// (count, mean, sum of squared deviations) of two disjoint parts, by the update of Chan, Golub and LeVeque
-// ("Updating formulae and a pairwise algorithm for computing sample variances", 1979): one pass over the
-// threads gives mean and variance without the cancellation of E[v^2] - E[v]^2.
-struct Moments {
-  float n, mean, m2;
-};
-VF4_DEV Moments join(const Moments& a, const Moments& b) {
-  const float n = a.n + b.n, f = n > 0.f ? __fdividef(b.n, n) : 0.f, d = b.mean - a.mean;
-  return {n, fmaf(d, f, a.mean), a.m2 + b.m2 + d * d * a.n * f};
-}
-
-// The row's moments, joined over its threads: a warp, or a CTA (red: its warps' moments; the caller
-// alternates between two such areas, so one barrier per call is enough).  kind RMS: mean 0, m2 the sum of
-// squares.  even: every thread holds as many columns, and the joins need no weights.
+// Sum over a row's threads: a warp, or a CTA (area: a float per warp; every call within a row has its own, so
+// one barrier per call is enough).
 template <int kThreads>
-VF4_DEV Moments row_moments(Moments v, int kind, bool even, Moments* red) {
-  if (kind == kNormRms) {
+VF4_DEV float row_sum(float v, float* area) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v.m2 += __shfl_xor_sync(0xFFFFFFFFu, v.m2, o);
-  } else if (even) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const float mean = __shfl_xor_sync(0xFFFFFFFFu, v.mean, o), m2 = __shfl_xor_sync(0xFFFFFFFFu, v.m2, o);
-      const float d = mean - v.mean;
-      v.mean = 0.5f * (v.mean + mean);
-      v.m2 = fmaf(d * d, 0.5f * v.n, v.m2 + m2);
-      v.n *= 2.f;
-    }
-  } else {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      Moments q{__shfl_xor_sync(0xFFFFFFFFu, v.n, o), __shfl_xor_sync(0xFFFFFFFFu, v.mean, o),
-                __shfl_xor_sync(0xFFFFFFFFu, v.m2, o)};
-      // both lanes of a pair join in the same order, so that all lanes end with the same values
-      v = (threadIdx.x & o) ? join(q, v) : join(v, q);
-    }
-  }
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
   if constexpr (kThreads > 32) {
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0) area[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = red[0];
+    v = 0.f;
 #pragma unroll
-    for (int i = 1; i < kThreads / 32; ++i) {
-      if (kind == kNormRms) v.m2 += red[i].m2;
-      else v = join(v, red[i]);
-    }
+    for (int i = 0; i < kThreads / 32; ++i) v += area[i];
   }
   return v;
 }
 
-// Centres v (LayerNorm) over the NV * 8 values of this thread's part of the row and returns 1 / sqrt(var + eps).
-template <int kThreads, int NV, bool kVec>
-VF4_DEV float centre(float (*v)[8], const int* nv, int kind, int K, float eps, Moments* red) {
-  Moments m{0.f, 0.f, 0.f};
-  if (kind == kNormLayer) {
-    float s = 0.f;
+// Mean and sum of squared deviations of a row whose threads hold n values each, from each thread's own: by pairs,
+// as Chan, Golub and LeVeque update them ("Updating formulae and a pairwise algorithm for computing sample
+// variances", 1979), so one pass over the threads gives both without the cancellation of E[v^2] - E[v]^2.
+template <int kThreads>
+VF4_DEV float2 row_moments(float n, float mean, float m2, float* area) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      m.n += (float)nv[j];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s += v[j][i];   // columns past K hold 0
-    }
-    m.mean = m.n > 0.f ? __fdividef(s, m.n) : 0.f;
+  for (int o = 1; o < 32; o <<= 1) {
+    const float b = __shfl_xor_sync(0xFFFFFFFFu, mean, o), d = b - mean;
+    m2 += __shfl_xor_sync(0xFFFFFFFFu, m2, o);
+    mean = 0.5f * (mean + b);
+    m2 = fmaf(d * d, 0.5f * n, m2);
+    n *= 2.f;
   }
+  if constexpr (kThreads > 32) {
+    constexpr int W = kThreads / 32;
+    if ((threadIdx.x & 31) == 0) {
+      area[threadIdx.x >> 5] = mean;
+      area[W + (threadIdx.x >> 5)] = m2;
+    }
+    __syncthreads();
+    mean = m2 = 0.f;
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+    for (int i = 0; i < W; ++i) mean += area[i];
+    mean *= 1.f / W;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (kVec ? nv[j] > 0 : i < nv[j]) {
-        const float d = v[j][i] - m.mean;
-        m.m2 = fmaf(d, d, m.m2);
-      }
-  m = row_moments<kThreads>(m, kind, K % (8 * kThreads) == 0, red);
-  if (kind == kNormLayer) {
+    for (int i = 0; i < W; ++i) {
+      const float d = area[i] - mean;
+      m2 += fmaf(d * d, n, area[W + i]);
+    }
+  }
+  return make_float2(mean, m2);
+}
+
+VF4_DEV float pair_sum(Pair a) {
+  float x, y;
+  f32x2_unpack(a, &x, &y);
+  return x + y;
+}
+
+// Pair i of a step without its elements past nv (non-vector rows; a vector row's steps are whole or empty).
+VF4_DEV Pair clip(Pair v, int i, int nv) {
+  float x, y;
+  f32x2_unpack(v, &x, &y);
+  return f32x2_pack(2 * i < nv ? x : 0.f, 2 * i + 1 < nv ? y : 0.f);
+}
+
+// Centres v (LayerNorm) over the NV * 8 values of this thread's part of the row and returns 1 / sqrt(var + eps).
+// Columns past K hold 0 before and after.  area: 3 * warps floats.
+template <int kThreads, int NV, bool kVec>
+VF4_DEV float centre(Pair (*v)[4], const int* nv, int kind, int K, float eps, float* area) {
+  constexpr int W = kThreads / 32;
+  auto squares = [&](Pair neg) {   // of v + neg, over this thread's columns
+    Pair q = 0ull;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (kVec ? nv[j] > 0 : i < nv[j]) v[j][i] -= m.mean;   // columns past K stay 0
+      for (int i = 0; i < 4; ++i) {
+        Pair d = add_f32x2(v[j][i], neg);
+        if (!kVec) d = clip(d, i, nv[j]);
+        if (!kVec || nv[j] > 0) q = fma_f32x2(d, d, q);
+      }
+    return pair_sum(q);
+  };
+  auto shift = [&](Pair neg) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (kVec && nv[j] <= 0) continue;
+        v[j][i] = add_f32x2(v[j][i], neg);
+        if (!kVec) v[j][i] = clip(v[j][i], i, nv[j]);
+      }
+  };
+  float m2;
+  if (kind == kNormLayer) {
+    Pair s = 0ull;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s = add_f32x2(s, v[j][i]);
+    const float sum = pair_sum(s);
+    if (K % (8 * kThreads) == 0) {   // every thread holds as many columns
+      const float n = (float)(K / kThreads), mean = __fdividef(sum, n);
+      const float2 mm = row_moments<kThreads>(n, mean, squares(both(-mean)), area);
+      m2 = mm.y;
+      shift(both(-mm.x));
+    } else {                         // in two passes over the threads
+      const Pair neg = both(-__fdividef(row_sum<kThreads>(sum, area), (float)K));
+      shift(neg);
+      m2 = row_sum<kThreads>(squares(0ull), area + 2 * W);
+    }
+  } else {
+    m2 = row_sum<kThreads>(squares(0ull), area);
   }
-  return rsqrtf(__fdividef(m.m2, (float)K) + eps);
+  return rsqrtf(__fdividef(m2, (float)K) + eps);
 }
 
 // z = v * r * w + b for eight columns.
-template <bool kVec>
-VF4_DEV void affine8(float* v, float r, const void* w, const void* b, int col, int f32, int nv) {
-  float p[8];
+template <typename P, bool kVec>
+VF4_DEV void affine8(Pair* v, float r, const void* w, const void* b, int col, int nv) {
+  Pair p[4];
   if (w) {
-    param8<kVec>(w, col, f32, nv, p);
+    param8<P, kVec>(w, col, nv, p);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] *= r;
+    for (int i = 0; i < 4; ++i) p[i] = mul_f32x2(p[i], both(r));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = r;
+    for (int i = 0; i < 4; ++i) p[i] = both(r);
   }
   if (b) {
-    float q[8];
-    param8<kVec>(b, col, f32, nv, q);
+    Pair q[4];
+    param8<P, kVec>(b, col, nv, q);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], p[i], q[i]);
+    for (int i = 0; i < 4; ++i) v[i] = fma_f32x2(v[i], p[i], q[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= p[i];
+    for (int i = 0; i < 4; ++i) v[i] = mul_f32x2(v[i], p[i]);
   }
 }
 
-// kThreads = 32: a warp per row, 8 rows per CTA in turn; else a CTA per row.  kOut: 0 no h, 1 h in T, 2 FP8.
-template <typename T, int kThreads, int NV, bool kVec, int kOut>
-__global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads, kThreads == 32 ? 2 : 1) gated_norm_kernel(const NormParams p) {
-  __shared__ Moments red[2][kThreads > 32 ? kThreads / 32 : 1];
+// kThreads = 32: a warp per row, 8 rows per CTA in turn; else a CTA per row.  P: the parameters' type.  kOut: 0 no
+// h, 1 h in T, 2 FP8.
+template <typename T, typename P, int kThreads, int NV, bool kVec, int kOut>
+__global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads, kThreads == 32 ? (NV > 4 ? 2 : 3) : 1) gated_norm_kernel(const NormParams p) {
+  __shared__ float red[2][3 * (kThreads / 32)];
   constexpr int kRows = kThreads == 32 ? 8 : 1;
   const int t = kThreads == 32 ? (threadIdx.x & 31) : threadIdx.x;
   const T *X = static_cast<const T*>(p.x), *Y = static_cast<const T*>(p.y);
@@ -173,35 +227,22 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads, kThreads == 3
   int nv[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) nv[j] = max(0, min(8, p.K - (j * kThreads + t) * 8));
-  // kAhead: the next row's x and y are loaded while this one is worked on (one warp per row leaves too few
-  // warps per SM to keep the memory busy otherwise)
-  constexpr bool kAhead = kThreads == 32 && sizeof(T) == 2 && kVec;
-  const int64_t row0 = blockIdx.x * (int64_t)kRows + (kThreads == 32 ? threadIdx.x >> 5 : 0), step = gridDim.x * (int64_t)kRows;
-  Raw8<T, kVec> xr[NV], yr[NV], xn[kAhead ? NV : 1], yn[kAhead ? NV : 1];
-  auto fetch = [&](int64_t row, Raw8<T, kVec>* a, Raw8<T, kVec>* b) {
+  // with several gates, a run of neighbouring rows per warp (CTA), which share a gate that then comes from L1
+  // (65792 x 1024 with 256 gates: 119 -> 102 us; without gates the runs cost 2%)
+  const int64_t runs = gridDim.x * (int64_t)kRows, run = blockIdx.x * (int64_t)kRows + (kThreads == 32 ? threadIdx.x >> 5 : 0);
+  const bool grouped = p.gate && p.rows_per_gate < p.M;
+  const int64_t end = grouped ? p.M * (run + 1) / runs : p.M, step = grouped ? 1 : runs;
+  for (int64_t row = grouped ? p.M * run / runs : run; row < end; row += step) {
+    Raw8<T, kVec> xr[NV];
+    Pair v[NV][4];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) a[j].load(X + row * p.ldx + (j * kThreads + t) * 8, row < p.M ? nv[j] : 0);
+    for (int j = 0; j < NV; ++j) xr[j].load(X + row * p.ldx + (j * kThreads + t) * 8, nv[j]);
     if (p.y) {
+      Raw8<T, kVec> yr[NV];
 #pragma unroll
-      for (int j = 0; j < NV; ++j) b[j].load(Y + row * p.ldy + (j * kThreads + t) * 8, row < p.M ? nv[j] : 0);
-    }
-  };
-  if (kAhead) fetch(row0, xn, yn);
-  for (int64_t row = row0; row < p.M; row += step) {
-    if constexpr (kAhead) {
+      for (int j = 0; j < NV; ++j) yr[j].load(Y + row * p.ldy + (j * kThreads + t) * 8, nv[j]);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        xr[j] = xn[j];
-        yr[j] = yn[j];
-      }
-      fetch(row + step, xn, yn);
-    } else {
-      fetch(row, xr, yr);
-    }
-    float v[NV][8];
-    if (p.y) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j) yr[j].get(v[j]);
+      for (int j = 0; j < NV; ++j) pairs8(yr[j], v[j]);
       float r2 = 1.f;
       if (p.post != kNormNone) r2 = centre<kThreads, NV, kVec>(v, nv, p.post, p.K, p.eps, red[0]);
       const int64_t gate_row = p.gate ? (int64_t)((uint32_t)row / p.rows_per_gate) * p.K : 0;
@@ -209,38 +250,44 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads, kThreads == 3
       for (int j = 0; j < NV; ++j) {
         if (nv[j] <= 0) continue;
         const int col = (j * kThreads + t) * 8;
-        float x[8], g[8];
-        if (p.post != kNormNone) affine8<kVec>(v[j], r2, p.w2, p.b2, col, p.p_f32, nv[j]);
+        Pair x[4], g[4];
+        if (p.post != kNormNone) affine8<P, kVec>(v[j], r2, p.w2, p.b2, col, nv[j]);
         if (p.gate) {
-          param8<kVec>(p.gate, gate_row + col, p.p_f32, nv[j], g);
+          param8<P, kVec>(p.gate, gate_row + col, nv[j], g);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] *= p.rs;
+          for (int i = 0; i < 4; ++i) g[i] = mul_f32x2(g[i], both(p.rs));
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] = p.rs;
+          for (int i = 0; i < 4; ++i) g[i] = both(p.rs);
         }
-        xr[j].get(x);
+        pairs8(xr[j], x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[j][i] = fmaf(v[j][i], g[i], x[i]);
+        for (int i = 0; i < 4; ++i) {
+          v[j][i] = fma_f32x2(v[j][i], g[i], x[i]);
+          if (!kVec) v[j][i] = clip(v[j][i], i, nv[j]);
+        }
         store_row8<T, kVec>(XO + row * p.K + col, nv[j], v[j]);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) xr[j].get(v[j]);
+      for (int j = 0; j < NV; ++j) pairs8(xr[j], v[j]);
     }
     if constexpr (kOut != 0) {
       const float r1 = centre<kThreads, NV, kVec>(v, nv, p.pre, p.K, p.eps, red[1]);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int col = (j * kThreads + t) * 8;
-        if (nv[j] > 0) affine8<kVec>(v[j], r1, p.w1, p.b1, col, p.p_f32, nv[j]);
+        if (nv[j] > 0) affine8<P, kVec>(v[j], r1, p.w1, p.b1, col, nv[j]);
         if constexpr (kOut == 1) {
           if (nv[j] > 0) store_row8<T, kVec>(H + row * p.K + col, nv[j], v[j]);
         } else {
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f32x2_unpack(v[j][i], &f[2 * i], &f[2 * i + 1]);
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (i >= nv[j]) v[j][i] = 0.f;
-          uint32_t m = amax8_bits(v[j]);
+            if (kVec ? nv[j] <= 0 : i >= nv[j]) f[i] = 0.f;
+          uint32_t m = amax8_bits(f);
 #pragma unroll
           for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
           if (nv[j] > 0) {
@@ -251,7 +298,7 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads, kThreads == 3
             const float q = __fdividef(448.f, a);
             uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = e4m3x2(v[j][2 * i] * q, v[j][2 * i + 1] * q);
+            for (int i = 0; i < 4; ++i) w[i] = e4m3x2(f[2 * i] * q, f[2 * i + 1] * q);
             *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.h) + row * p.ldc + col) =
                 make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
             if ((t & 15) == 0) p.scale[row * p.s_m + (col >> 7) * p.s_k] = __fdiv_rn(a, 448.f);
@@ -262,33 +309,36 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads, kThreads == 3
   }
 }
 
-template <typename T, int kThreads, int NV, bool kVec>
+template <typename T, typename P, int kThreads, int NV, bool kVec>
 static void launch_norm(const NormParams& p, int out, cudaStream_t s) {
   const int64_t rows = kThreads == 32 ? 8 : 1;
   const int64_t want = (p.M + rows - 1) / rows;
-  const int64_t most = (int64_t)num_sms() * (kThreads == 32 ? 4 : 16);
+  const int64_t most = (int64_t)num_sms() * (kThreads == 32 ? (NV > 4 ? 2 : 3) : 16);
   const unsigned grid = (unsigned)(want < most ? want : most);
   constexpr int block = kThreads == 32 ? 256 : kThreads;
-  if (out == 0) gated_norm_kernel<T, kThreads, NV, kVec, 0><<<grid, block, 0, s>>>(p);
-  else if (out == 1) gated_norm_kernel<T, kThreads, NV, kVec, 1><<<grid, block, 0, s>>>(p);
-  else gated_norm_kernel<T, kThreads, NV, kVec, 2><<<grid, block, 0, s>>>(p);
+  if (out == 0) gated_norm_kernel<T, P, kThreads, NV, kVec, 0><<<grid, block, 0, s>>>(p);
+  else if (out == 1) gated_norm_kernel<T, P, kThreads, NV, kVec, 1><<<grid, block, 0, s>>>(p);
+  else gated_norm_kernel<T, P, kThreads, NV, kVec, 2><<<grid, block, 0, s>>>(p);
 }
 
-// Threads per row and steps of 8 columns per thread by the rows' number and length.  Up to 1024 columns a warp
-// takes a row, unless there are so few rows that most SMs would get none or one: then, as for longer rows, a
-// CTA takes a row, of the threads that the row fills in one step where that is at most 256.
-template <typename T, bool kVec>
+// Threads per row and steps of 8 columns per thread by the rows' number and length.  Up to 1280 columns a warp
+// takes a row, unless there are so few rows that most SMs would get none or one (257 rows of 1024: 8.6 us with a
+// warp per row, 3.9 with a CTA); then, as for longer rows, a CTA takes a row, of as many threads as the row fills
+// in one or two steps.
+template <typename T, typename P, bool kVec>
 static void dispatch_norm(const NormParams& p, int out, cudaStream_t s) {
   const bool few = p.M <= 8 * (int64_t)num_sms();
-  if (p.K <= 256) launch_norm<T, 32, 1, kVec>(p, out, s);
-  else if (p.K <= 512 && !few) launch_norm<T, 32, 2, kVec>(p, out, s);
-  else if (p.K <= 1024 && !few) launch_norm<T, 32, 4, kVec>(p, out, s);
-  else if (p.K <= 1024) launch_norm<T, 128, 1, kVec>(p, out, s);
-  else if (p.K <= 1280) launch_norm<T, 160, 1, kVec>(p, out, s);
-  else if (p.K <= 2048) launch_norm<T, 256, 1, kVec>(p, out, s);
-  else if (p.K <= 4096) launch_norm<T, 256, 2, kVec>(p, out, s);
-  else if (p.K <= 8192) launch_norm<T, 256, 4, kVec>(p, out, s);
-  else launch_norm<T, 512, 4, kVec>(p, out, s);
+  if (p.K <= 256) launch_norm<T, P, 32, 1, kVec>(p, out, s);
+  else if (p.K <= 512 && !few) launch_norm<T, P, 32, 2, kVec>(p, out, s);
+  else if (p.K <= 1024 && !few) launch_norm<T, P, 32, 4, kVec>(p, out, s);
+  else if (p.K <= 1024) launch_norm<T, P, 128, 1, kVec>(p, out, s);
+  else if (p.K <= 1280 && !few) launch_norm<T, P, 32, 5, kVec>(p, out, s);
+  else if (p.K <= 1280) launch_norm<T, P, 160, 1, kVec>(p, out, s);
+  else if (p.K <= 2048) launch_norm<T, P, 256, 1, kVec>(p, out, s);
+  else if (p.K <= 4096) launch_norm<T, P, 256, 2, kVec>(p, out, s);
+  else if (p.K <= 5120) launch_norm<T, P, 320, 2, kVec>(p, out, s);
+  else if (p.K <= 8192) launch_norm<T, P, 256, 4, kVec>(p, out, s);
+  else launch_norm<T, P, 512, 4, kVec>(p, out, s);
 }
 
 }  // namespace vf4
@@ -308,6 +358,8 @@ extern "C" int vf4_gated_residual_norm(const void* x, int64_t ldx, const void* y
   if (K > 16384) return fail(VF4_ERR_UNSUPPORTED, "%s: rows of at most 16384 columns (K=%lld)", me, (long long)K);
   if ((dtype != VF4_BF16 && dtype != VF4_F32) || (param_dtype != VF4_BF16 && param_dtype != VF4_F32))
     return fail(VF4_ERR_ARG, "%s: bad dtype", me);
+  if (dtype == VF4_F32 && param_dtype != VF4_F32 && (gate || post_w || post_b || pre_w || pre_b))
+    return fail(VF4_ERR_UNSUPPORTED, "%s: fp32 rows take fp32 parameters", me);
   if (post < kNormNone || post > kNormRms || pre < kNormNone || pre > kNormRms) return fail(VF4_ERR_ARG, "%s: bad norm", me);
   if ((!y && (post != kNormNone || gate || pre == kNormNone)) || (post == kNormNone && (post_w || post_b)) ||
       (pre == kNormNone && (pre_w || pre_b)))
@@ -335,18 +387,20 @@ extern "C" int vf4_gated_residual_norm(const void* x, int64_t ldx, const void* y
   p.M = M; p.ldx = ldx; p.ldy = ldy;
   p.rows_per_gate = gate ? (uint32_t)(M / gate_groups) : 1u;
   p.K = (int)K; p.post = post; p.pre = pre;
-  p.p_f32 = param_dtype == VF4_F32;
   p.rs = residual_scale; p.eps = eps;
   p.x_out = x_out; p.h = h;
   p.ldc = ldc; p.scale = scale; p.s_m = stride_m; p.s_k = stride_k;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int out = pre == kNormNone ? 0 : h_fp8 ? 2 : 1;
-  if (dtype == VF4_BF16) {
-    if (vec) dispatch_norm<__nv_bfloat16, true>(p, out, s);
-    else dispatch_norm<__nv_bfloat16, false>(p, out, s);
+  if (dtype == VF4_F32) {
+    if (vec) dispatch_norm<float, float, true>(p, out, s);
+    else dispatch_norm<float, float, false>(p, out, s);
+  } else if (param_dtype == VF4_F32) {
+    if (vec) dispatch_norm<__nv_bfloat16, float, true>(p, out, s);
+    else dispatch_norm<__nv_bfloat16, float, false>(p, out, s);
   } else {
-    if (vec) dispatch_norm<float, true>(p, out, s);
-    else dispatch_norm<float, false>(p, out, s);
+    if (vec) dispatch_norm<__nv_bfloat16, __nv_bfloat16, true>(p, out, s);
+    else dispatch_norm<__nv_bfloat16, __nv_bfloat16, false>(p, out, s);
   }
   return launch_status(me);
 }

@@ -81,7 +81,7 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, norm="layer", po
     for name, t in zip(("post_weight", "post_bias", "pre_weight", "pre_bias"), params[1:]):
         _check_param(name, t, K)
     dtypes = {t.dtype for t in params if t is not None}
-    if dtypes and dtypes != {torch.bfloat16} and dtypes != {torch.float32}:
+    if dtypes and dtypes != {x.dtype} and dtypes != {torch.float32}:
         if not dtypes <= {torch.bfloat16, torch.float32, torch.float16}:
             raise _lib.VitFp4Error(f"gate, weights and biases are bf16 or fp32, got {sorted(map(str, dtypes))}")
         params = [None if t is None else t.float() for t in params]   # fp32 holds every bf16 and fp16 value
