@@ -11,7 +11,7 @@
 // R = G * Sq rows against the same keys, so a decoder's single token still reads each key once.
 //
 //   xattn_tc_kernel    tcgen05: 128-row tiles, 128 keys at a time, online softmax
-//   xattn_rows_kernel  up to 4 rows over short keys, plain FMAs: the keys stream through registers
+//   xattn_rows_kernel  up to 4 rows over short keys (plain_rows), plain FMAs: the keys stream through registers
 //
 // With fewer tiles than SMs the keys are cut into chunks: each CTA leaves its rows' maxima, sums and
 // unnormalised outputs in the workspace and xattn_join_kernel adds them up in order.
@@ -68,21 +68,26 @@ VF4_DEV int64_t o_offset(const XParams& p, int b, int hk, int r) {
 
 // ---------------------------------------------------------------------------------------
 // Up to 4 rows.  LPK lanes hold one key's D <= 8 LPK elements (16 bytes each), so a warp reads 32 / LPK keys
-// per load; every group of lanes keeps its own maximum, sum and output for the keys it sees, taking kU of
-// them at a time (loads of the next kU in flight), and the groups are joined at the end: lanes by shuffles,
-// warps through shared memory.  Bound by memory: each key and value is read once; 2 R FMAs per element.
+// per load; every group of lanes keeps its own maximum, sum and output for the keys it sees, kU of them at a
+// time (all their loads in flight together), and the groups are joined at the end: lanes by shuffles, warps
+// through shared memory.  Bound by memory latency first, which the SM's other CTAs hide (1024 problems of 257
+// keys: 4.2 TB/s); a few problems get eight warps each, which take an image's 257 tokens of 64 elements in one
+// batch (kU = 9: 36 keys per warp).
 // ---------------------------------------------------------------------------------------
-constexpr int kRowWarps = 4;
+constexpr int kRowWarps = 8;   // at most
 
 template <int LPK, int R>
 __global__ void __launch_bounds__(kRowWarps * 32) xattn_rows_kernel(const XParams p) {
-  constexpr int KPW = 32 / LPK, kU = 4;
+  constexpr int KPW = 32 / LPK, kU = R <= 2 ? 9 : 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int grp = lane / LPK, el = (lane % LPK) * 8;     // key group and first element of this lane
   const int chunk = blockIdx.x % p.chunks, item = blockIdx.x / p.chunks;
   const int b = item / p.Hkv, hk = item - b * p.Hkv;
   const bool on = el < p.D;
   const int k0 = chunk * p.chunk, k1 = min(keys_of(p, b), k0 + p.chunk);
+  // this warp's share of the keys
+  const int warps = blockDim.x >> 5, share = ((k1 - k0 + warps - 1) / warps + KPW - 1) / KPW * KPW;
+  const int w0 = k0 + warp * share, w1 = min(k1, w0 + share);
 
   float q[R][8], acc[R][8], m[R], l[R];
 #pragma unroll
@@ -102,33 +107,19 @@ __global__ void __launch_bounds__(kRowWarps * 32) xattn_rows_kernel(const XParam
   const __nv_bfloat16* kp = p.k + b * p.kb + hk * p.kh + el;
   const __nv_bfloat16* vp = p.v + b * p.vb + hk * p.vh + el;
   const uint8_t* mp = p.mask ? p.mask + b * p.mask_b : nullptr;
-  uint4 kw[kU], vw[kU];
-  bool keep[kU];
-  auto fetch = [&](int base) {
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int j = base + u * KPW + grp;
-      keep[u] = j < k1 && (!mp || mp[j] != 0);
-      kw[u] = vw[u] = make_uint4(0, 0, 0, 0);
-      if (keep[u] && on) {
-        kw[u] = __ldg(reinterpret_cast<const uint4*>(kp + (int64_t)j * p.ks));
-        vw[u] = __ldg(reinterpret_cast<const uint4*>(vp + (int64_t)j * p.vs));
-      }
-    }
-  };
-  constexpr int kStep = kRowWarps * KPW * kU;
-  const int first = k0 + warp * KPW * kU;
-  if (first < k1) fetch(first);
-  for (int base = first; base < k1; base += kStep) {
+  for (int base = w0; base < w1; base += KPW * kU) {
     uint4 kc[kU], vc[kU];
     bool kept[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      kc[u] = kw[u];
-      vc[u] = vw[u];
-      kept[u] = keep[u];
+      const int j = base + u * KPW + grp;
+      kept[u] = j < w1 && (!mp || mp[j] != 0);
+      kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
+      if (kept[u] && on) {
+        kc[u] = __ldg(reinterpret_cast<const uint4*>(kp + (int64_t)j * p.ks));
+        vc[u] = __ldg(reinterpret_cast<const uint4*>(vp + (int64_t)j * p.vs));
+      }
     }
-    if (base + kStep < k1) fetch(base + kStep);
     float s[kU][R];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
@@ -205,17 +196,19 @@ __global__ void __launch_bounds__(kRowWarps * 32) xattn_rows_kernel(const XParam
     }
   }
   __syncthreads();
-  for (int t = threadIdx.x; t < R * LPK; t += kRowWarps * 32) {
+  for (int t = threadIdx.x; t < R * LPK; t += blockDim.x) {
     const int r = t / LPK, e = (t - r * LPK) * 8;
     if (r >= p.R || e >= p.D) continue;
     float mx = -INFINITY, ls = 0.f, o[8];
 #pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) mx = fmaxf(mx, red_ml[w][r].x);
+    for (int w = 0; w < kRowWarps; ++w)
+      if (w < warps) mx = fmaxf(mx, red_ml[w][r].x);
     const float ms = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = 0.f;
 #pragma unroll
     for (int w = 0; w < kRowWarps; ++w) {
+      if (w >= warps) break;
       const float f = ex2_approx(red_ml[w][r].x - ms);
       ls = fmaf(red_ml[w][r].y, f, ls);
 #pragma unroll
@@ -758,18 +751,22 @@ static int make_kv_map(CUtensorMap* m, const void* ptr, const XParams& p, int64_
 }
 
 // The plain kernel takes up to 4 rows over short keys, where a CTA of the tensor-core kernel would spend most of
-// its time starting and ending; with long keys the tensor copies read faster than its lanes do.
-constexpr int kPlainRows = 4, kPlainKeys = 1024;
-static bool plain_rows(int64_t R, int64_t Skv) { return R <= kPlainRows && Skv <= kPlainKeys; }
+// its time starting and ending; its FMAs and shuffles grow with the rows, so the border falls.  Measured (64 x 16
+// problems of 64 elements; plain and tcgen05): 1 row over 257 keys 16.6 and 33.8 us, over 4097 163 and 192 (16391
+// keys of 128 elements, 32 problems: 80 and 51); 2 rows over 257 24.9 and 33.8, over 577 46.9 and 43.7; 4 rows
+// over 65 13.6 and 20.8, over 257 42.8 and 33.8.
+static bool plain_rows(int64_t R, int64_t Skv) {
+  return R == 1 ? Skv <= 4096 : R == 2 ? Skv <= 512 : R <= 4 && Skv <= 128;
+}
 
 // How many keys a CTA takes, and how many CTAs share a row tile (1: no workspace).
 static void plan_chunks(int64_t B, int64_t Hkv, int64_t R, int64_t Skv, int sms, int* chunk, int* chunks) {
   const bool plain = plain_rows(R, Skv);
   const int64_t items = B * Hkv * (plain ? 1 : (R + 127) / 128);
-  // plain kernel: 4 CTAs of 128 threads per SM, at least 256 keys each; tcgen05: as many CTAs as are resident at
+  // plain kernel: 4 CTAs per SM, at least 1024 keys each; tcgen05: as many CTAs as are resident at
   // once, at least 512 keys each (with key counts that differ, shorter chunks would even the CTAs out, but measured
   // slower: 4 images of up to 16391 keys, 32 heads over 8 of 128 elements: 45 us, 53 with twice as many)
-  const int64_t want = plain ? (int64_t)sms * 4 : (int64_t)sms * 2, least = plain ? 256 : 512;
+  const int64_t want = plain ? (int64_t)sms * 4 : (int64_t)sms * 2, least = plain ? 1024 : 512;
   int64_t n = want / items;
   if (n > (Skv + least - 1) / least) n = (Skv + least - 1) / least;
   if (n < 1) n = 1;
@@ -804,9 +801,13 @@ template <int LPK>
 static int launch_rows(const XParams& p, cudaStream_t s) {
   const int64_t grid = (int64_t)p.B * p.Hkv * p.chunks;
   if (grid > INT32_MAX) return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: sizes too large");
-  if (p.R == 1) xattn_rows_kernel<LPK, 1><<<(unsigned)grid, kRowWarps * 32, 0, s>>>(p);
-  else if (p.R == 2) xattn_rows_kernel<LPK, 2><<<(unsigned)grid, kRowWarps * 32, 0, s>>>(p);
-  else xattn_rows_kernel<LPK, 4><<<(unsigned)grid, kRowWarps * 32, 0, s>>>(p);
+  // as many warps per problem as keep 16 on every SM
+  int warps = kRowWarps;
+  while (warps > 1 && grid * warps > (int64_t)num_sms() * 24) warps /= 2;
+  const unsigned threads = 32u * (unsigned)warps;
+  if (p.R == 1) xattn_rows_kernel<LPK, 1><<<(unsigned)grid, threads, 0, s>>>(p);
+  else if (p.R == 2) xattn_rows_kernel<LPK, 2><<<(unsigned)grid, threads, 0, s>>>(p);
+  else xattn_rows_kernel<LPK, 4><<<(unsigned)grid, threads, 0, s>>>(p);
   return launch_status("vf4_cross_attn");
 }
 
