@@ -631,6 +631,12 @@ VF4_DEV bool elect_one() {
   return e != 0;
 }
 
+// Programmatic dependent launch: a kernel launched with the attribute may start before the one ahead of it in
+// the stream has ended.  wait: until that one has, and its writes are visible (no effect otherwise); launch: this
+// kernel's successor may start now.
+VF4_DEV void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+VF4_DEV void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 VF4_DEV void tma_prefetch(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
 }

@@ -44,6 +44,7 @@ __global__ void __launch_bounds__(256, 4) fp8_cast_rows_kernel(const T* __restri
   const int d_row = n_hw / kb, d_g = n_hw - d_row * kb;
   int row = hw / kb, g = hw - row * kb;
   const int64_t steps = (M * kb - (hw & ~1) + n_hw - 1) / n_hw;
+  griddep_launch();   // the product may set itself up meanwhile
   for (int64_t i = 0; i < steps; i += kU) {
     Raw8<T, kVec> v[kU];
     int at_row[kU], at_g[kU], nv[kU];
@@ -324,6 +325,7 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
     // time, and a block of four MMAs took 600 clocks to issue whatever its size (513 of 512 now).
     const bool elected = elect_one();
     if (warp == 0) {
+      griddep_wait();
       int s = 0, it = 0;
       uint32_t ph = 1;   // an unused stage counts as released
       bool ok = true;
@@ -410,6 +412,7 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
     }
   } else {
     if constexpr (C::kRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kEpiRegs));
+    griddep_wait();   // the launch may have come before the operands' cast had ended (the barriers above did not need it)
     const int quad = warp & 3, half = (warp - C::EPI0) >> 2;
     const int r = quad * 32 + lane;                       // row of the tile, lane of tensor memory
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(half * C::NC);
@@ -876,12 +879,13 @@ static int launch_fp8_gemm(F8Operand a, F8Operand b, int64_t K, F8Params p, cuda
   cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2] = {{}, early_launch()};
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)(C::kPair ? 2 : p.split);
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = C::kPair || p.split > 1 ? 1 : 0;
+  const bool cluster = C::kPair || p.split > 1;
+  cfg.attrs = cluster ? at : at + 1;
+  cfg.numAttrs = cluster ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, kern, ta, tb, to, p) != cudaSuccess) return launch_status("vf4_gemm_fp8_block");
   return launch_status("vf4_gemm_fp8_block");
 }

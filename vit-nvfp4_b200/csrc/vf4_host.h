@@ -40,6 +40,15 @@ int attn_device_error(int clear);
 int fp8_device_error(int clear);
 int xattn_device_error(int clear);
 
+// Launch attribute: the kernel may start while the one ahead of it in the stream is ending (it waits for that one's
+// end itself, griddep_wait, before it touches anything in global memory).
+inline cudaLaunchAttribute early_launch() {
+  cudaLaunchAttribute a;
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Opt kernel `kern` into `bytes` of dynamic shared memory on the current device.  The attribute

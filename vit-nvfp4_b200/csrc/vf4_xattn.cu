@@ -230,11 +230,15 @@ __global__ void __launch_bounds__(kRowWarps * 32) xattn_rows_kernel(const XParam
   }
 }
 
-// One warp per row: the chunks' partial results in order.  Maxima are in units of log2.
-__global__ void __launch_bounds__(128) xattn_join_kernel(const XParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = blockIdx.x * 4ll + (threadIdx.x >> 5);
-  if (row >= (int64_t)p.B * p.Hkv * p.R) return;
+// One CTA per row: warp w joins chunks w, w + 8, .., then the warps are joined, all in a fixed order.  Maxima are
+// in units of log2.  Started while the chunks' kernel ends.
+constexpr int kJoinWarps = 8;
+__global__ void __launch_bounds__(kJoinWarps * 32) xattn_join_kernel(const XParams p) {
+  __shared__ float4 red_o[kJoinWarps][32];
+  __shared__ float red_l[kJoinWarps];
+  griddep_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x;
   const int item = (int)(row / p.R), r = (int)(row - (int64_t)item * p.R);
   const int b = item / p.Hkv, hk = item - b * p.Hkv;
   const int n = min(p.chunks, (keys_of(p, b) + p.chunk - 1) / p.chunk);   // chunks that hold keys
@@ -244,25 +248,50 @@ __global__ void __launch_bounds__(128) xattn_join_kernel(const XParams p) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
   const float ms = mx == -INFINITY ? 0.f : mx;
-  float ls = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
   const int e = lane * 4;
-  for (int c = 0; c < n; ++c) {
-    const float2 ml = p.part_ml[at + (int64_t)c * p.R];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;   // a chunk without kept keys
-    const float f = ex2_approx(ml.x - ms);
-    ls = fmaf(ml.y, f, ls);
-    if (e < p.D) {
-      const float4 o = *reinterpret_cast<const float4*>(p.part_o + (at + (int64_t)c * p.R) * p.D + e);
-      acc[0] = fmaf(o.x, f, acc[0]);
-      acc[1] = fmaf(o.y, f, acc[1]);
-      acc[2] = fmaf(o.z, f, acc[2]);
-      acc[3] = fmaf(o.w, f, acc[3]);
+  float ls = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int kU = 4;   // chunks whose loads are in flight together
+  for (int c0 = warp; c0 < n; c0 += kJoinWarps * kU) {
+    float2 ml[kU];
+    float4 o[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int c = c0 + u * kJoinWarps;
+      ml[u] = make_float2(-INFINITY, 0.f);
+      o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c < n) {
+        ml[u] = p.part_ml[at + (int64_t)c * p.R];
+        if (e < p.D) o[u] = *reinterpret_cast<const float4*>(p.part_o + (at + (int64_t)c * p.R) * p.D + e);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (ml[u].x == -INFINITY && ml[u].y == 0.f) continue;   // a chunk without kept keys
+      const float f = ex2_approx(ml[u].x - ms);
+      ls = fmaf(ml[u].y, f, ls);
+      acc.x = fmaf(o[u].x, f, acc.x);
+      acc.y = fmaf(o[u].y, f, acc.y);
+      acc.z = fmaf(o[u].z, f, acc.z);
+      acc.w = fmaf(o[u].w, f, acc.w);
     }
   }
-  if (e < p.D) {
+  red_o[warp][lane] = acc;
+  if (lane == 0) red_l[warp] = ls;
+  __syncthreads();
+  if (warp == 0 && e < p.D) {
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) {
+      const float4 o = red_o[w][lane];
+      acc.x += o.x;
+      acc.y += o.y;
+      acc.z += o.z;
+      acc.w += o.w;
+      ls += red_l[w];
+    }
     const float f = ls > 0.f ? __fdividef(1.f, ls) : (ls == 0.f ? 0.f : ls);
     *reinterpret_cast<uint2*>(p.out + o_offset(p, b, hk, r) + e) =
-        make_uint2(bf16x2_round(f32x2_pack(acc[0] * f, acc[1] * f)), bf16x2_round(f32x2_pack(acc[2] * f, acc[3] * f)));
+        make_uint2(bf16x2_round(f32x2_pack(acc.x * f, acc.y * f)), bf16x2_round(f32x2_pack(acc.z * f, acc.w * f)));
   }
 }
 
@@ -842,6 +871,7 @@ int vf4_cross_attn(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const v
   if (B > (1 << 24) || H > (1 << 16) || Sq > (1 << 24) || Skv > (1 << 30) || H / Hkv * Sq > (1 << 28))
     return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: sizes too large");
   if (B == 0 || Sq == 0) return VF4_OK;
+  if (B * H * Sq > INT32_MAX) return fail(VF4_ERR_UNSUPPORTED, "vf4_cross_attn: sizes too large");
   if (!q || !out || (Skv > 0 && (!k || !v))) return fail(VF4_ERR_ARG, "vf4_cross_attn: null operand");
   const int64_t strides[] = {q_b, q_h, q_s, k_b, k_h, k_s, v_b, v_h, v_s, o_b, o_h, o_s};
   for (int64_t x : strides)
@@ -887,7 +917,14 @@ int vf4_cross_attn(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const v
     st = D <= 64 ? launch_tc<64>(p, s) : launch_tc<128>(p, s);
   if (st || p.chunks == 1) return st;
   const int64_t rows = B * H * Sq;
-  xattn_join_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(p);
+  cudaLaunchAttribute at[1] = {early_launch()};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)rows);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = s;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, xattn_join_kernel, p) != cudaSuccess) return launch_status("vf4_cross_attn (join)");
   return launch_status("vf4_cross_attn (join)");
 }
 
