@@ -142,27 +142,28 @@ struct F8Cfg {
   static constexpr bool kPair = BN == 256;
   static constexpr int A_BYTES = 128 * 128, B_BYTES = (kPair ? 128 : BN) * 128, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int ROWS = kPair ? 256 : 128;         // rows of a tile
-  static constexpr int STAGES = BN >= 128 ? 5 : 8;
+  static constexpr int STAGES = kPair ? 4 : BN == 128 ? 5 : 8;
   static constexpr int ACCS = BN == 256 ? 2 : 4;
   static constexpr int TMEM_COLS = ACCS * BN;            // 64 .. 512, a power of two
-  static constexpr int EW = BN >= 128 ? 2 : 1;           // epilogue warps per lane quadrant
+  static constexpr int EW = kPair ? 4 : BN == 128 ? 2 : 1;   // epilogue warps per lane quadrant
   static constexpr int NC = BN / EW;                     // columns per epilogue warp
   static constexpr int EPI_WARPS = 4 * EW;
-  // columns per TMEM load, two loads' registers per thread: the next load is in flight while one is
-  // multiplied in (tcgen05.ld takes about 100 clocks whatever its width, so wide ones)
-  static constexpr int CH = NC >= 64 ? 32 : 16;
-  // the 256-column tile needs 128 sums + 64 loaded values per thread: its epilogue warps take registers
-  // over from the four warps of the control group (2 of them idle)
+  // columns per TMEM load, and loads whose registers a thread holds: with two, the next load is in flight while one
+  // is multiplied in.  The 256-column tile has sixteen warps of 64 columns with one load each: eight warps of 128
+  // columns and two loads are as fast over long K (8192 x 5120 x 5120: 229 us) but 3 to 7% slower over K of 1280 to
+  // 4096, where their two staged halves of the output wait for each other
+  static constexpr int CH = NC >= 64 ? 32 : 16, BUF = kPair ? 1 : 2;
+  // those take registers over from the four warps of the control group (two of them idle)
   static constexpr bool kRegs = kPair;
   static constexpr int EPI0 = kRegs ? 4 : 2;             // first epilogue warp
   static constexpr int THREADS = 32 * (EPI0 + EPI_WARPS);
-  static constexpr int kLaunchRegs = 168, kControlRegs = 40, kEpiRegs = 232;   // 384 threads: 168 at launch
-  static_assert(!kRegs || 128 * kControlRegs + 256 * kEpiRegs <= THREADS * kLaunchRegs, "register split");
+  static constexpr int kLaunchRegs = 96, kControlRegs = 32, kEpiRegs = 112;   // 640 threads: 96 at launch
+  static_assert(!kRegs || 128 * kControlRegs + 512 * kEpiRegs <= THREADS * kLaunchRegs, "register split");
   static constexpr int STG_OFF = STAGES * STAGE_BYTES;   // bf16 output staging, 32 rows x 64 columns per warp
   static constexpr int STG_BYTES = kSwap ? 0 : EPI_WARPS * 4096;
   // scales on their way to the epilogue threads (kSwap loads them into registers instead): kRing K blocks
   // ahead, across tiles, {own row's, weight block's} per thread
-  static constexpr int kRing = kSwap ? 0 : 8;
+  static constexpr int kRing = kSwap ? 0 : 6;
   static constexpr int RING_OFF = STG_OFF + STG_BYTES, RING_SLOT = 32 * EPI_WARPS * 8;
   static constexpr int BIAS_OFF = RING_OFF + kRing * RING_SLOT;   // each epilogue warp's bias values
   static constexpr int BAR_OFF = BIAS_OFF + (kSwap ? 0 : EPI_WARPS * NC * 4);
@@ -502,19 +503,20 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
         if (!ok) return;
         tc_fence_after();
         constexpr int CH = C::CH;
-        uint32_t v[2][CH];
+        constexpr int BUF = C::BUF;
+        uint32_t v[BUF][CH];
         auto load = [&](int c) {
-          if constexpr (CH == 32) tmem_ld_32x32b_x32(lane_base + a * BN + CH * c, v[c & 1]);
-          else tmem_ld_32x32b_x16(lane_base + a * BN + CH * c, v[c & 1]);
+          if constexpr (CH == 32) tmem_ld_32x32b_x32(lane_base + a * BN + CH * c, v[c % BUF]);
+          else tmem_ld_32x32b_x16(lane_base + a * BN + CH * c, v[c % BUF]);
         };
         load(0);
 #pragma unroll
         for (int c = 0; c < C::NC / CH; ++c) {
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < CH; i += 16) reg_fence16(&v[c & 1][i]);
+          for (int i = 0; i < CH; i += 16) reg_fence16(&v[c % BUF][i]);
           if (c + 1 < C::NC / CH) {
-            load(c + 1);
+            if (BUF > 1) load(c + 1);
           } else {
             tc_fence_before();
             __syncwarp();
@@ -534,8 +536,9 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
                               __shfl_sync(0xFFFFFFFFu, u, (CH * c + 2 * i + 1) & 31));
             }
             unsigned long long& d = acc[CH / 2 * c + i];
-            d = fma_f32x2(f32x2_pack(__uint_as_float(v[c & 1][2 * i]), __uint_as_float(v[c & 1][2 * i + 1])), s2, d);
+            d = fma_f32x2(f32x2_pack(__uint_as_float(v[c % BUF][2 * i]), __uint_as_float(v[c % BUF][2 * i + 1])), s2, d);
           }
+          if (BUF == 1 && c + 1 < C::NC / CH) load(c + 1);
         }
         if (++a == C::ACCS) {
           a = 0;
