@@ -77,9 +77,11 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, norm="layer", po
             raise _lib.VitFp4Error(f"gate: a contiguous ({K},) or (G, {K}) tensor needed, got {tuple(gate.shape)}")
         if gate.dim() == 2 and (gate.shape[0] < 1 or M % gate.shape[0]):
             raise _lib.VitFp4Error(f"{M} rows do not divide into {gate.shape[0]} gates")
-    params = [gate, post_weight, post_bias, pre_weight, pre_bias]
-    for name, t in zip(("post_weight", "post_bias", "pre_weight", "pre_bias"), params[1:]):
-        _check_param(name, t, K)
+    _check_param("post_weight", post_weight, K)
+    _check_param("post_bias", post_bias, K)
+    _check_param("pre_weight", pre_weight, K)
+    _check_param("pre_bias", pre_bias, K)
+    params = (gate, post_weight, post_bias, pre_weight, pre_bias)
     dtypes = {t.dtype for t in params if t is not None}
     if dtypes and dtypes != {x.dtype} and dtypes != {torch.float32}:
         if not dtypes <= {torch.bfloat16, torch.float32, torch.float16}:

@@ -237,26 +237,41 @@ def _there(fn, first: torch.Tensor, *args):
         return fn(first, *args)
 
 
-def _timed(kind: str, sizes: tuple, work: float, name: str, *args) -> None:
-    """One launch under the probe's events (the label is only built when it is on)."""
+_entry: dict = {}
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_F8, _BF16, _F32, _U8 = torch.float8_e4m3fn, torch.bfloat16, torch.float32, torch.uint8
+_CODES = {torch.bfloat16: _lib.VF4_BF16, torch.float32: _lib.VF4_F32}
+
+
+def _call(name: str, kind: str, sizes: tuple, work: float, *args) -> None:
+    """One library call on the current stream (its last argument), under the probe's events when that is on."""
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(_lib.lib(), name)
+    stream = _raw_stream(_current_device())
     if probe.timing:
         with _Timed(f"{kind}_{'x'.join(map(str, sizes))}", work):
-            _lib.call(name, *args)
+            rc = fn(*args, stream)
     else:
-        _lib.call(name, *args)
+        rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc, name)
 
 
 def _rows_2d(x: torch.Tensor) -> torch.Tensor:
     """(M, K) view of (..., K) with unit column stride and non-overlapping rows (copies only if needed)."""
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if x2.stride(1) != 1 and x2.shape[1] > 1 or x2.stride(0) < x2.shape[1] and x2.shape[0] > 1:
+    (rows, cols), (s0, s1) = x2.shape, x2.stride()
+    if s1 != 1 and cols > 1 or s0 < cols and rows > 1:
         x2 = x2.contiguous()
     return x2
 
 
 def _ld(x2: torch.Tensor) -> int:
     """Row stride of a 2-D tensor, as the kernels take it (a single row may carry any stride)."""
-    return x2.stride(0) if x2.shape[0] > 1 else max(x2.stride(0), x2.shape[1])
+    rows, cols = x2.shape
+    s0 = x2.stride(0)
+    return s0 if rows > 1 or s0 > cols else cols
 
 
 def cast_fp8_block(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
@@ -265,27 +280,29 @@ def cast_fp8_block(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, 
     The activation scales are stored column block by column block, the order the product reads them in."""
     if _elsewhere(x):
         return _there(cast_fp8_block, x, block_rows)
-    code = _dtype_code(x)
+    code = _CODES.get(x.dtype)
+    if code is None:
+        code = _dtype_code(x)
     x2 = _rows_2d(x)
     M, K = x2.shape
     if K < 1:
         raise _lib.VitFp4Error("the FP8 block cast needs at least one column")
     ldc, kb, dev = (K + 15) // 16 * 16, (K + 127) // 128, x.device
-    codes = torch.empty_strided((M, ldc), (ldc, 1), dtype=torch.float8_e4m3fn, device=dev)
+    codes = torch.empty_strided((M, ldc), (ldc, 1), dtype=_F8, device=dev)
     rows = M if block_rows == 1 else (M + block_rows - 1) // block_rows
     s_m, s_k = (1, M) if block_rows == 1 else (kb, 1)
-    scale = torch.empty_strided((rows, kb), (s_m, s_k), dtype=torch.float32, device=dev)
-    _timed("cast_fp8_block", (M, K), M * K * (x2.element_size() + 1) + rows * kb * 4, "vf4_cast_fp8_block",
-           x2.data_ptr(), code, M, K, _ld(x2), block_rows, codes.data_ptr(), ldc, scale.data_ptr(), s_m, s_k, _stream())
+    scale = torch.empty_strided((rows, kb), (s_m, s_k), dtype=_F32, device=dev)
+    _call("vf4_cast_fp8_block", "cast_fp8_block", (M, K), M * K * (x2.element_size() + 1) + rows * kb * 4,
+          x2.data_ptr(), code, M, K, _ld(x2), block_rows, codes.data_ptr(), ldc, scale.data_ptr(), s_m, s_k)
     probe.launches += 1
     return (codes if ldc == K else codes[:, :K]), scale
 
 
 def _code_rows(t: torch.Tensor) -> torch.Tensor:
     """(rows, K) E4M3 codes whose rows start on 16-byte boundaries, as the tensor copies need them."""
-    if t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+    (rows, K), (s0, s1) = t.shape, t.stride()
+    if s1 == 1 and not s0 % 16 and s0 >= K and not t.data_ptr() % 16:
         return t
-    rows, K = t.shape
     buf = torch.empty((rows, (K + 15) // 16 * 16), dtype=torch.uint8, device=t.device)
     buf[:, :K] = t.view(torch.uint8)
     return buf[:, :K].view(torch.float8_e4m3fn)
@@ -301,9 +318,9 @@ def gemm_fp8_block(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_sc
     out = torch.empty_strided((M, N), (N, 1), dtype=out_dtype, device=a.device)
     as_m, as_k = a_scale.stride()
     bs_n, bs_k = b_scale.stride()
-    _timed("gemm_fp8_block", (M, N, K), 2.0 * M * N * K, "vf4_gemm_fp8_block", a.data_ptr(), _ld(a), a_scale.data_ptr(),
-           as_m, as_k, b.data_ptr(), _ld(b), b_scale.data_ptr(), bs_n, bs_k, M, N, K, _ptr(bias),
-           0 if bias is None else _dtype_code(bias), out.data_ptr(), N, 1 if out_dtype == torch.float32 else 0, _stream())
+    _call("vf4_gemm_fp8_block", "gemm_fp8_block", (M, N, K), 2.0 * M * N * K, a.data_ptr(), _ld(a), a_scale.data_ptr(),
+          as_m, as_k, b.data_ptr(), _ld(b), b_scale.data_ptr(), bs_n, bs_k, M, N, K, _ptr(bias),
+          0 if bias is None else _dtype_code(bias), out.data_ptr(), N, 1 if out_dtype == torch.float32 else 0)
     probe.launches += 1
     return out
 
@@ -314,16 +331,18 @@ def linear_fp8_block(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
     The rows' codes live in a workspace allocated per call."""
     if _elsewhere(x, w, w_scale, bias):
         return _there(linear_fp8_block, x, w, w_scale, bias)
-    code = _dtype_code(x)
+    code = _CODES.get(x.dtype)
+    if code is None:
+        code = _dtype_code(x)
     x, w = _rows_2d(x), _code_rows(w)
     (M, K), N, dev = x.shape, w.shape[0], x.device
     out = torch.empty_strided((M, N), (N, 1), dtype=x.dtype, device=dev)
     n = _lib.lib().vf4_linear_fp8_block_workspace_size(M, K)
-    ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=dev) if n else None
+    ws = torch.empty_strided((n,), (1,), dtype=_U8, device=dev) if n else None
     ws_n, ws_k = w_scale.stride()
-    _timed("linear_fp8_block", (M, N, K), 2.0 * M * N * K, "vf4_linear_fp8_block", x.data_ptr(), code, M, K, _ld(x),
-           w.data_ptr(), _ld(w), w_scale.data_ptr(), ws_n, ws_k, N, _ptr(bias), 0 if bias is None else _dtype_code(bias),
-           out.data_ptr(), N, _ptr(ws), n, _stream())
+    _call("vf4_linear_fp8_block", "linear_fp8_block", (M, N, K), 2.0 * M * N * K, x.data_ptr(), code, M, K, _ld(x),
+          w.data_ptr(), _ld(w), w_scale.data_ptr(), ws_n, ws_k, N, None if bias is None else bias.data_ptr(),
+          0 if bias is None else _dtype_code(bias), out.data_ptr(), N, None if ws is None else ws.data_ptr(), n)
     probe.launches += 2 if n else 1
     return out
 
@@ -348,21 +367,28 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor | None, gate: torch.Ten
     ldc = s_m = s_k = 0
     if pre is not None and fp8_out:
         ldc, kb = (K + 15) // 16 * 16, (K + 127) // 128
-        h = torch.empty_strided((M, ldc), (ldc, 1), dtype=torch.float8_e4m3fn, device=dev)
-        scale = torch.empty_strided((M, kb), (1, M), dtype=torch.float32, device=dev)
+        h = torch.empty_strided((M, ldc), (ldc, 1), dtype=_F8, device=dev)
+        scale = torch.empty_strided((M, kb), (1, M), dtype=_F32, device=dev)
         s_m, s_k = 1, M
     elif pre is not None:
         h = torch.empty_strided((M, K), (K, 1), dtype=x.dtype, device=dev)
-    param = gate if gate is not None else post_w if post_w is not None else post_b if post_b is not None else \
-        pre_w if pre_w is not None else pre_b if pre_b is not None else x
-    groups = 1 if gate is None or gate.dim() == 1 else gate.shape[0]
     if M == 0:   # empty tensors have no address, which would read as "not given"
         return x_out, h if h is None else h[:, :K], scale
+    param = x
+    for t in (gate, post_w, post_b, pre_w, pre_b):
+        if t is not None:
+            param = t
+            break
+    code, pcode = _CODES.get(x.dtype), _CODES.get(param.dtype)
+    if code is None or pcode is None:
+        code, pcode = _dtype_code(x), _dtype_code(param)
+    groups = 1 if gate is None or gate.dim() == 1 else gate.shape[0]
     esz = x.element_size()
-    _timed("gated_norm", (M, K), M * K * (esz * (1 if y is None else 3) + (0 if h is None else 1 if fp8_out else esz)),
-           "vf4_gated_residual_norm", x2.data_ptr(), _ld(x2), _ptr(y2), 0 if y2 is None else _ld(y2), _dtype_code(x), M, K,
-           _ptr(gate), groups, residual_scale, NORM_KINDS[post], _ptr(post_w), _ptr(post_b), NORM_KINDS[pre], _ptr(pre_w),
-           _ptr(pre_b), _dtype_code(param), eps, _ptr(x_out), _ptr(h), int(fp8_out), ldc, _ptr(scale), s_m, s_k, _stream())
+    _call("vf4_gated_residual_norm", "gated_norm", (M, K),
+          M * K * (esz * (1 if y is None else 3) + (0 if h is None else 1 if fp8_out else esz)), x2.data_ptr(), _ld(x2),
+          _ptr(y2), 0 if y2 is None else _ld(y2), code, M, K, _ptr(gate), groups, residual_scale, NORM_KINDS[post],
+          _ptr(post_w), _ptr(post_b), NORM_KINDS[pre], _ptr(pre_w), _ptr(pre_b), pcode, eps, _ptr(x_out), _ptr(h),
+          1 if fp8_out else 0, ldc, _ptr(scale), s_m, s_k)
     probe.launches += 1
     if h is not None and ldc and ldc != K:
         h = h[:, :K]
@@ -669,8 +695,8 @@ def attention_packed_qkv(qkv: torch.Tensor, num_heads: int, scale: float, head_g
 
 def _attn_view(t: torch.Tensor) -> torch.Tensor:
     """(B, H, S, D) with the strides the cross attention kernels read in place (copied otherwise)."""
-    st = t.stride()
-    if st[3] == 1 and not (st[0] | st[1] | st[2]) % 8 and not t.data_ptr() % 16 and (st[2] >= t.shape[3] or t.shape[2] <= 1):
+    sb, sh, ss, sd = t.stride()
+    if sd == 1 and not (sb | sh | ss) & 7 and not t.data_ptr() & 15 and (ss >= t.shape[3] or t.shape[2] <= 1):
         return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
 
@@ -694,10 +720,11 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
     qb, qh, qs, _ = q.stride()
     kb, kh, ks, _ = k.stride()
     vb, vh, vs, _ = v.stride()
-    _timed("cross_attn", (B * H, Sq, Skv, D), 4.0 * B * H * Sq * Skv * D, "vf4_cross_attn", q.data_ptr(), qb, qh, qs,
-           k.data_ptr() or None, kb, kh, ks, v.data_ptr() or None, vb, vh, vs, B, H, Hkv, Sq, Skv, D, scale, _ptr(kv_lens),
-           _ptr(key_mask), 0 if key_mask is None else key_mask.stride(0), out.data_ptr(), Sq * H * D, D, H * D, _ptr(ws), n,
-           _stream())
+    _call("vf4_cross_attn", "cross_attn", (B * H, Sq, Skv, D), 4.0 * B * H * Sq * Skv * D, q.data_ptr(), qb, qh, qs,
+          k.data_ptr() or None, kb, kh, ks, v.data_ptr() or None, vb, vh, vs, B, H, Hkv, Sq, Skv, D, scale,
+          None if kv_lens is None else kv_lens.data_ptr(), None if key_mask is None else key_mask.data_ptr(),
+          0 if key_mask is None else key_mask.stride(0), out.data_ptr(), Sq * H * D, D, H * D,
+          None if ws is None else ws.data_ptr(), n)
     probe.launches += 2 if n else 1
     return out
 
