@@ -3,7 +3,9 @@
     python -m vitfp4._build            # or vitfp4._build.build()
 
 The library lands next to this file (``vitfp4/libvitfp4.so``) so it travels with the
-source tree; it is rebuilt only when a source or header is newer than the library.
+source tree; it is rebuilt only when a source or header is newer than the library.  Beside it
+``vitfp4/_fast.so``, a host-side module (g++, torch's headers) that makes the plain calls of the small
+ops without the Python argument path; without it those calls take that path to the same kernels.
 """
 from __future__ import annotations
 
@@ -42,6 +44,35 @@ def _deps() -> list[str]:
         glob.glob(os.path.join(INCLUDE, "*.h"))
 
 
+FAST_SRC = os.path.join(CSRC, "host", "vf4_fast.cpp")
+FAST = os.path.join(PKG, "_fast.so")
+
+
+def build_fast(force: bool = False) -> str:
+    """Compile csrc/host/vf4_fast.cpp against torch and libvitfp4.so; returns the module's path."""
+    deps = [FAST_SRC, os.path.join(INCLUDE, "vitfp4.h")]
+    if not force and os.path.exists(FAST) and all(os.path.getmtime(d) <= os.path.getmtime(FAST) for d in deps):
+        return FAST
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
+    tmp = FAST + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f for p in inc for f in ("-isystem", p)], "-I", INCLUDE, FAST_SRC, "-o", tmp,
+           "-L", PKG, "-l:libvitfp4.so", "-Wl,-rpath,$ORIGIN", "-L", os.path.join(root, "lib"),
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if r.returncode:
+        sys.stderr.write(r.stdout)
+        raise RuntimeError("g++ failed for vf4_fast.cpp")
+    os.replace(tmp, FAST)
+    return FAST
+
+
 def up_to_date() -> bool:
     if not os.path.exists(LIB):
         return False
@@ -52,6 +83,7 @@ def up_to_date() -> bool:
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -> str:
     """Compile every csrc/*.cu for sm_100a and link libvitfp4.so; returns its path."""
     if not force and up_to_date():
+        build_fast()
         return LIB
     nvcc = _nvcc()
     objdir = os.path.join(os.path.dirname(PKG), "_build")
@@ -80,6 +112,7 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -
         sys.stderr.write(r.stdout)
         raise RuntimeError("link of libvitfp4.so failed")
     os.replace(tmp, LIB)
+    build_fast(force)
     return LIB
 
 

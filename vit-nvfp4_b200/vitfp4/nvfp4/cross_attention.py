@@ -37,6 +37,10 @@ def cross_sdpa(query, key, value, *, kv_lens=None, key_mask=None, scale=None):
     (B, Skv) bool: False keys are not used.  Unused keys and values may hold anything; a query without any used key
     gives 0.  ``scale`` defaults to 1 / sqrt(D).  The result is laid out as (B, Sq, H, D), ready for the output
     projection."""
+    if not torch.compiler.is_compiling():
+        out = ops.fast_cross(query, key, value, kv_lens, key_mask, scale)
+        if out is not None:
+            return out
     for name, t in (("query", query), ("key", key), ("value", value)):
         if t.dtype != torch.bfloat16 or t.dim() != 4:
             raise _lib.VitFp4Error(f"{name}: a 4-D bf16 tensor needed, got {tuple(t.shape)} {t.dtype}")

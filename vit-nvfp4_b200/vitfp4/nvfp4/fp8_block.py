@@ -95,6 +95,10 @@ def quantize_to_fp8_block(x: torch.Tensor, block_rows: int = 1):
 
     ``block_rows`` 1: a scale per row and 128 columns (activations).  128: a scale per 128 x 128 block of a 2-D
     weight -> scale (ceil(N / 128), ceil(K / 128))."""
+    if block_rows == 1 and not torch.compiler.is_compiling():
+        out = ops.fast_cast(x)
+        if out is not None:
+            return out
     if block_rows not in (1, _BLOCK):
         raise _lib.VitFp4Error(f"block_rows is 1 or {_BLOCK}, got {block_rows}")
     if x.dim() < 1 or x.dim() != 2 and block_rows != 1:
@@ -133,6 +137,10 @@ def fp8_block_gemm(a, a_scale, b, b_scale, *, bias=None, out_dtype=torch.bfloat1
 
 def fp8_block_linear(x, w, w_scale, *, bias=None):
     """Linear layer with an FP8 block weight: online cast of x (..., K), product, + bias; output in x.dtype."""
+    if not torch.compiler.is_compiling():
+        out = ops.fast_linear(x, w, w_scale, bias)
+        if out is not None:
+            return out
     _check_weight(w, w_scale, bias)
     if x.shape[-1] != w.shape[1]:
         raise _lib.VitFp4Error(f"x has {x.shape[-1]} columns, the weight {w.shape[1]}")

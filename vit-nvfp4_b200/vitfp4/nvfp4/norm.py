@@ -54,6 +54,12 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, norm="layer", po
     ``out_dtype`` None or x's: h in x's type; ``torch.float8_e4m3fn``: h = (codes, scales) in the FP8 block format
     that ``fp8_block_gemm`` reads.  ``y`` None: (x, N_pre(x)).  Arithmetic in fp32; x' is rounded once for storage
     and enters N_pre unrounded."""
+    if post_norm and pre_norm and norm in ops.NORM_KINDS and not torch.compiler.is_compiling() and \
+            (out_dtype is None or out_dtype == torch.float8_e4m3fn):
+        out = ops.fast_norm(x, y, gate, residual_scale, ops.NORM_KINDS[norm], post_weight, post_bias, pre_weight,
+                            pre_bias, eps, out_dtype is not None)
+        if out is not None:
+            return out
     if norm not in ("layer", "rms"):
         raise _lib.VitFp4Error(f"norm is 'layer' or 'rms', got {norm!r}")
     if x.dtype not in (torch.bfloat16, torch.float32) or x.dim() < 1 or x.shape[-1] < 1:

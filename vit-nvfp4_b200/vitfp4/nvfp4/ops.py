@@ -395,6 +395,32 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor | None, gate: torch.Ten
     return x_out, h, scale
 
 
+try:   # the plain calls in one C++ step; where it is not built they take the functions of this file
+    from .. import _fast as _fast_module
+except ImportError:
+    _fast_module = None
+
+
+def _fast(name: str):
+    """The C++ form of an op's plain call -> its outputs, or None for any other call, which then goes the Python way
+    (also while the probe times calls)."""
+    fn = getattr(_fast_module, name, None)
+    if fn is None:
+        return lambda *a: None
+
+    def call(*a):
+        if probe.timing:
+            return None
+        r = fn(*a)
+        if r is not None:
+            probe.launches += _fast_module.launched()
+        return r
+    return call
+
+
+fast_cast, fast_linear, fast_norm, fast_cross = (_fast(n) for n in ("cast", "linear", "norm", "cross"))
+
+
 def to_blocked(sf: torch.Tensor) -> torch.Tensor:
     """(R, C) E4M3 scales (uint8 or float8_e4m3fn) -> flat 128x4-tiled uint8."""
     _need_cuda(sf)
