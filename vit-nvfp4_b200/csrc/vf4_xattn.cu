@@ -230,15 +230,17 @@ __global__ void __launch_bounds__(kRowWarps * 32) xattn_rows_kernel(const XParam
   }
 }
 
-// One CTA per row: warp w joins chunks w, w + 8, .., then the warps are joined, all in a fixed order.  Maxima are
-// in units of log2.  Started while the chunks' kernel ends.
+// per_row warps per row (1, 2, 4 or 8 of the CTA's 8; by the number of chunks): warp w of them joins chunks w,
+// w + per_row, .., then the warps are joined, all in a fixed order.  Maxima are in units of log2.  Started while the
+// chunks' kernel ends.
 constexpr int kJoinWarps = 8;
-__global__ void __launch_bounds__(kJoinWarps * 32) xattn_join_kernel(const XParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) xattn_join_kernel(const XParams p, const int per_row) {
   __shared__ float4 red_o[kJoinWarps][32];
   __shared__ float red_l[kJoinWarps];
   griddep_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp & (per_row - 1);
+  const int64_t rows = (int64_t)p.B * p.Hkv * p.R, own = blockIdx.x * (int64_t)(kJoinWarps / per_row) + warp / per_row;
+  const int64_t row = own < rows ? own : rows - 1;   // past the last row: the last one, without storing it
   const int item = (int)(row / p.R), r = (int)(row - (int64_t)item * p.R);
   const int b = item / p.Hkv, hk = item - b * p.Hkv;
   const int n = min(p.chunks, (keys_of(p, b) + p.chunk - 1) / p.chunk);   // chunks that hold keys
@@ -252,12 +254,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) xattn_join_kernel(const XPara
   float ls = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int kU = 4;   // chunks whose loads are in flight together
-  for (int c0 = warp; c0 < n; c0 += kJoinWarps * kU) {
+  for (int c0 = sub; c0 < n; c0 += per_row * kU) {
     float2 ml[kU];
     float4 o[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int c = c0 + u * kJoinWarps;
+      const int c = c0 + u * per_row;
       ml[u] = make_float2(-INFINITY, 0.f);
       o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (c < n) {
@@ -279,9 +281,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) xattn_join_kernel(const XPara
   red_o[warp][lane] = acc;
   if (lane == 0) red_l[warp] = ls;
   __syncthreads();
-  if (warp == 0 && e < p.D) {
-#pragma unroll
-    for (int w = 1; w < kJoinWarps; ++w) {
+  if (sub == 0 && own < rows && e < p.D) {
+    for (int w = warp + 1; w < warp + per_row; ++w) {
       const float4 o = red_o[w][lane];
       acc.x += o.x;
       acc.y += o.y;
@@ -919,12 +920,16 @@ int vf4_cross_attn(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const v
   const int64_t rows = B * H * Sq;
   cudaLaunchAttribute at[1] = {early_launch()};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)rows);
+  // four chunks per warp have their loads in flight together: 4848 rows of 7 chunks take 31 us in all with two warps
+  // per row and 43 with eight, one row of 64 chunks 13 us with eight and 31 with one
+  int per_row = 1;
+  while (per_row < kJoinWarps && per_row * 4 < p.chunks) per_row *= 2;
+  cfg.gridDim = dim3((unsigned)((rows * per_row + kJoinWarps - 1) / kJoinWarps));
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = s;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, xattn_join_kernel, p) != cudaSuccess) return launch_status("vf4_cross_attn (join)");
+  if (cudaLaunchKernelEx(&cfg, xattn_join_kernel, p, per_row) != cudaSuccess) return launch_status("vf4_cross_attn (join)");
   return launch_status("vf4_cross_attn (join)");
 }
 
