@@ -356,11 +356,10 @@ VF4_API int vf4_gemm_fp8_block(const uint8_t* a, int64_t lda, const float* a_sca
                                int64_t ldo, int out_dtype, vf4_stream_t stream);
 
 /* Linear layer with an FP8 block weight: vf4_cast_fp8_block of the rows x (M, K), then vf4_gemm_fp8_block, in one
- * call: out = x W^T + bias in x's dtype.  Up to 4 rows (K up to 24576
- * for one row, 12288 for two, 6144 beyond) take one launch that
- * casts the rows itself.  workspace: vf4_linear_fp8_block_workspace_size(M, K) bytes (0: none needed), 16-byte
- * aligned, used until the call's work is done. */
-VF4_API int64_t vf4_linear_fp8_block_workspace_size(int64_t M, int64_t K);
+ * call: out = x W^T + bias in x's dtype.  One or two rows times a small
+ * weight take one launch that casts the rows itself.  workspace: vf4_linear_fp8_block_workspace_size(M, N, K) bytes (0:
+ * none needed), 16-byte aligned, used until the call's work is done. */
+VF4_API int64_t vf4_linear_fp8_block_workspace_size(int64_t M, int64_t N, int64_t K);
 VF4_API int vf4_linear_fp8_block(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w, int64_t ldw,
                                  const float* w_scale, int64_t ws_n, int64_t ws_k, int64_t N, const void* bias,
                                  int bias_dtype, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes,

@@ -39,7 +39,8 @@ def _calls():
     return [
         ("cast", 1, lambda: api.quantize_to_fp8_block(x)),
         ("cast f32", 1, lambda: api.quantize_to_fp8_block(x.float())),
-        ("linear few", 1, lambda: api.fp8_block_linear(x[:3], w, ws, bias=bias)),
+        ("linear one", 1, lambda: api.fp8_block_linear(x[:1], w, ws, bias=bias)),
+        ("linear few", 2, lambda: api.fp8_block_linear(x[:3], w, ws, bias=bias)),
         ("linear", 2, lambda: api.fp8_block_linear(many, w, ws)),
         ("linear f32", 2, lambda: api.fp8_block_linear(many.float(), w, ws, bias=bias.float())),
         ("norm", 1, lambda: api.gated_residual_norm(x, y, gate=gate, residual_scale=0.5, post_weight=nw, pre_weight=nw, pre_bias=nw)),
@@ -74,7 +75,7 @@ def test_both_paths_give_the_same(monkeypatch):
             assert a.shape == b.shape and a.dtype == b.dtype and a.stride() == b.stride(), name
             assert torch.equal(a.float(), b.float()), name
         taken.append(name)
-    assert len(ops.probe.records) and len(taken) == 11
+    assert len(ops.probe.records) and len(taken) == 12
     ops.probe.reset()
 
 

@@ -193,6 +193,24 @@ def test_linear_is_cast_then_product(shape, N, K, dtype):
         _check(y.reshape(-1, N), want, mag, K, bias)
 
 
+# one and two rows in one launch: several passes over the weight rows, up to four chunks of columns; narrow tiles with
+# more tiles than CTAs and an odd number of K blocks, and shared by clusters of each size; two waves of 128 x 128 tiles
+@pytest.mark.parametrize("M,N,K", [(1, 9001, 500), (2, 8192, 512), (1, 700, 2047), (1, 701, 2049), (2, 5000, 1024), (16, 38100, 384),
+                                   (17, 38100, 300), (40, 19300, 384), (16, 1000, 1300), (31, 4900, 2600), (64, 1000, 1300),
+                                   (50, 5000, 2700), (100, 2200, 1700), (2050, 1280, 260)])
+def test_linear_at_the_edges_of_its_variants(M, N, K):
+    from vitfp4.nvfp4 import fp8_block_linear, quantize_to_fp8_block
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    x = torch.randn(M, K, device="cuda", generator=g).bfloat16()
+    w, ws = quantize_to_fp8_block(torch.randn(N, K, device="cuda", generator=g) * 0.05, 128)
+    bias = torch.randn(N, device="cuda", generator=g).bfloat16()
+    codes, scale = quantize_to_fp8_block(x)
+    want, mag = _product64(codes, scale, w, ws)
+    y = fp8_block_linear(x, w, ws, bias=bias)
+    _check(y, want, mag, K, bias)
+    assert torch.equal(y, fp8_block_linear(x, w, ws, bias=bias))   # no order of additions depends on timing
+
+
 def test_linear_captured_replayed_and_on_another_stream():
     from vitfp4.nvfp4 import fp8_block_linear, quantize_to_fp8_block
     g = torch.Generator(device="cuda").manual_seed(4)

@@ -130,7 +130,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
         ws.size(1) != (K + 127) / 128 || !vector_ok(bias, N) || (bias.defined() && code_of(bias) < 0))
       return nullptr;
     at::Tensor y = make({M, N}, {N, 1}, x.scalar_type(), x), work;
-    const int64_t need = vf4_linear_fp8_block_workspace_size(M, K);
+    const int64_t need = vf4_linear_fp8_block_workspace_size(M, N, K);
     if (need) work = make({need}, {1}, at::kByte, x);
     if (vf4_linear_fp8_block(x.const_data_ptr(), code_of(x), M, K, ld, static_cast<const uint8_t*>(w.const_data_ptr()), ldw,
                              static_cast<const float*>(ws.const_data_ptr()), ws.stride(0), ws.stride(1), N, ptr(bias),

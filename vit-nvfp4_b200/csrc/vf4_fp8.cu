@@ -30,7 +30,7 @@ int fp8_device_error(int clear) {
 // The blocks of all rows are numbered in one sequence, row by row, and dealt to the half-warps, so
 // short and long rows fill the machine alike.  Bound by memory: 1 byte out per 2 (bf16) or 4 (fp32)
 // bytes in; kU blocks per half-warp are loaded before the first is reduced, to keep enough bytes in
-// flight.
+// flight (16400 x 5120 bf16: 59 us with 4, 61 with 2, 73 with 1).
 // ---------------------------------------------------------------------------------------
 template <typename T, bool kVec, int kU>
 __global__ void __launch_bounds__(256, 4) fp8_cast_rows_kernel(const T* __restrict__ x, int64_t M, int K, int64_t ld,
@@ -142,10 +142,13 @@ struct F8Cfg {
   static constexpr bool kPair = BN == 256;
   static constexpr int A_BYTES = 128 * 128, B_BYTES = (kPair ? 128 : BN) * 128, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int ROWS = kPair ? 256 : 128;         // rows of a tile
-  static constexpr int STAGES = kPair ? 4 : BN == 128 ? 5 : 8;
+  // 16 and 32 columns: two CTAs on an SM, one's epilogue beside the other's loads (32 x 5120 x 5120: 10.3 us, 13.0 with
+  // one CTA of 8 stages).  64 columns: one (64 x 5120 x 1280: 7.1 us, 8.6 with two of 4 stages)
+  static constexpr int PER_SM = kSwap && BN < 64 ? 2 : 1;
+  static constexpr int STAGES = kPair ? 4 : kSwap && BN == 64 ? 8 : 5;
   static constexpr int ACCS = BN == 256 ? 2 : 4;
   static constexpr int TMEM_COLS = ACCS * BN;            // 64 .. 512, a power of two
-  static constexpr int EW = kPair ? 4 : BN == 128 ? 2 : 1;   // epilogue warps per lane quadrant
+  static constexpr int EW = kPair ? 4 : BN >= 64 ? 2 : 1;   // epilogue warps per lane quadrant
   static constexpr int NC = BN / EW;                     // columns per epilogue warp
   static constexpr int EPI_WARPS = 4 * EW;
   // columns per TMEM load, and loads whose registers a thread holds: with two, the next load is in flight while one
@@ -161,15 +164,17 @@ struct F8Cfg {
   static_assert(!kRegs || 128 * kControlRegs + 512 * kEpiRegs <= THREADS * kLaunchRegs, "register split");
   static constexpr int STG_OFF = STAGES * STAGE_BYTES;   // bf16 output staging, 32 rows x 64 columns per warp
   static constexpr int STG_BYTES = kSwap ? 0 : EPI_WARPS * 4096;
-  // scales on their way to the epilogue threads (kSwap loads them into registers instead): kRing K blocks
-  // ahead, across tiles, {own row's, weight block's} per thread
+  // scales on their way to the epilogue threads: kRing K blocks ahead, across tiles, {own row's, weight block's}
+  // per thread.  kSwap loads them into registers instead and hands each block's to the warp's other lanes through
+  // SW_OFF: two blocks of NC values per warp (read as broadcasts; a shuffle per column held the block up)
   static constexpr int kRing = kSwap ? 0 : 6;
   static constexpr int RING_OFF = STG_OFF + STG_BYTES, RING_SLOT = 32 * EPI_WARPS * 8;
   static constexpr int BIAS_OFF = RING_OFF + kRing * RING_SLOT;   // each epilogue warp's bias values
-  static constexpr int BAR_OFF = BIAS_OFF + (kSwap ? 0 : EPI_WARPS * NC * 4);
+  static constexpr int SW_OFF = BIAS_OFF;
+  static constexpr int BAR_OFF = BIAS_OFF + (kSwap ? 2 : 1) * EPI_WARPS * NC * 4;
   static constexpr int NBAR = 2 * STAGES + 2 * ACCS;
   static constexpr int SMEM = 1024 + BAR_OFF + 8 * NBAR + 16;
-  static_assert(SMEM <= 227 * 1024, "shared memory");
+  static_assert(PER_SM * (SMEM + 1024) <= 228 * 1024 && PER_SM * TMEM_COLS <= 512, "shared and tensor memory of an SM");
   static_assert(kPair || BN * 128 * 4 <= STAGES * STAGE_BYTES, "the split sums reuse the stages");
 };
 
@@ -236,7 +241,6 @@ VF4_DEV void store8(const F8Params& p, int64_t m, int n0, const float* z) {
 template <bool kF32>
 VF4_DEV void store1(const F8Params& p, int m, int n, float y) {
   if (m >= p.M || n >= p.N) return;
-  y += bias_at(p, n);
   if constexpr (kF32) static_cast<float*>(p.out)[(int64_t)m * p.ldo + n] = y;
   else static_cast<__nv_bfloat16*>(p.out)[(int64_t)m * p.ldo + n] = __float2bfloat16_rn(y);
 }
@@ -263,7 +267,7 @@ VF4_DEV float ld_shared_cluster(uint32_t addr) {
 }
 
 template <int BN, bool kSwap, bool kF32>
-__global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
+__global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, F8Cfg<BN, kSwap>::PER_SM)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmO, const F8Params p) {
   using C = F8Cfg<BN, kSwap>;
@@ -457,20 +461,19 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
       const int tr = tile / p.tiles_c, tc = tile - tr * p.tiles_c;
       const int row0 = tr * C::ROWS + (C::kPair ? rank * 128 : 0) + quad * 32;   // first row of this warp
       const int row = row0 + lane, col0 = tc * BN + half * C::NC;
-      // kSwap: one activation row's scale per lane (two with 64 columns), the weight's alike for all.  The
-      // values of blocks kb + 1 and kb + 2 are on their way while kb is worked on, multiplied only when used.
-      constexpr int kAhead = 3;
-      [[maybe_unused]] float sw[kAhead], sx[kAhead], sy[kAhead];
+      // kSwap: one activation row's scale per lane, the weight's alike for all.  The values of the next kAhead - 1
+      // blocks are on their way while kb is worked on, multiplied only when used.
+      constexpr int kAhead = kSwap ? 6 : 3;
+      [[maybe_unused]] float sw[kAhead], sx[kAhead];
       const bool have = kSwap && lane < C::NC && col0 + lane < p.M;
-      const bool have2 = kSwap && C::NC > 32 && col0 + 32 + lane < p.M;
       const float* s_own = p.sa + (int64_t)(have ? col0 + lane : 0) * p.sa_m;
       const float* s_blk = p.sb + (int64_t)tr * p.sb_n;
       auto fetch = [&](int kb, int slot) {
         if (kb >= k1) return;
         sw[slot] = __ldg(s_blk + kb * p.sb_k);
         sx[slot] = have ? __ldg(s_own + kb * p.sa_k) : 0.f;
-        if constexpr (C::NC > 32) sy[slot] = have2 ? __ldg(s_own + 32 * p.sa_m + kb * p.sa_k) : 0.f;
       };
+      if constexpr (kSwap) __syncwarp();   // the last tile's scales have been read
       unsigned long long acc[C::NC / 2];
 #pragma unroll
       for (int i = 0; i < C::NC / 2; ++i) acc[i] = 0ull;
@@ -486,11 +489,13 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
         for (int u = 0; u + 1 < kAhead; ++u) fetch(k0 + u, u);
       }
       auto block = [&](int kb, int slot) {
-        float s0, s1 = 0.f;
+        [[maybe_unused]] float s0 = 0.f;
+        // kAhead is even, so neighbouring blocks use different halves; a half is written again after two __syncwarp
+        [[maybe_unused]] float* sc = reinterpret_cast<float*>(gb + C::SW_OFF) + ((warp - C::EPI0) * 2 + (slot & 1)) * C::NC;
         if constexpr (kSwap) {
           fetch(kb + kAhead - 1, (slot + kAhead - 1) % kAhead);
-          s0 = sx[slot] * sw[slot];
-          if constexpr (C::NC > 32) s1 = sy[slot] * sw[slot];
+          if (lane < C::NC) sc[lane] = sx[slot] * sw[slot];
+          __syncwarp();
         } else {
           cp_async_wait<C::kRing - 2>();   // this block's pair, the oldest of the groups in flight
           const float2 q = ld_shared_f2(ring + use);
@@ -526,17 +531,21 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
             }
           }
 #pragma unroll
-          for (int i = 0; i < CH / 2; ++i) {
-            unsigned long long s2;
+          for (int i = 0; i < CH / 2; i += 2) {
+            unsigned long long s2[2];
             if constexpr (!kSwap) {
-              s2 = f32x2_pack(s0, s0);
+              s2[0] = s2[1] = f32x2_pack(s0, s0);
             } else {
-              const float u = CH * c + 2 * i < 32 ? s0 : s1;
-              s2 = f32x2_pack(__shfl_sync(0xFFFFFFFFu, u, (CH * c + 2 * i) & 31),
-                              __shfl_sync(0xFFFFFFFFu, u, (CH * c + 2 * i + 1) & 31));
+              const float4 q = *reinterpret_cast<const float4*>(sc + CH * c + 2 * i);
+              s2[0] = f32x2_pack(q.x, q.y);
+              s2[1] = f32x2_pack(q.z, q.w);
             }
-            unsigned long long& d = acc[CH / 2 * c + i];
-            d = fma_f32x2(f32x2_pack(__uint_as_float(v[c % BUF][2 * i]), __uint_as_float(v[c % BUF][2 * i + 1])), s2, d);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              unsigned long long& d = acc[CH / 2 * c + i + e];
+              d = fma_f32x2(f32x2_pack(__uint_as_float(v[c % BUF][2 * (i + e)]), __uint_as_float(v[c % BUF][2 * (i + e) + 1])),
+                            s2[e], d);
+            }
           }
           if (BUF == 1 && c + 1 < C::NC / CH) load(c + 1);
         }
@@ -586,6 +595,7 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
         }
       } else if (p.split == 1) {
         float y[8];
+        const float own = kSwap ? bias_at(p, row) : 0.f;
 #pragma unroll
         for (int c = 0; c < C::NC / 8; ++c) {
 #pragma unroll
@@ -594,7 +604,7 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
             store8<kF32>(p, row, col0 + 8 * c, y);
           } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) store1<kF32>(p, col0 + 8 * c + i, row, y[i]);
+            for (int i = 0; i < 8; ++i) store1<kF32>(p, col0 + 8 * c + i, row, y[i] + own);
           }
         }
       } else {
@@ -619,7 +629,20 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
   if (!C::kPair && p.split > 1) {
     __syncwarp();
     cluster_sync_all();
-    // rank's share of the columns, summed over the ranks in their order
+    // rank's share of the columns, summed over the ranks in their order.  The loads of two ranks (split is even)
+    // are in flight together: one at a time, each waited for by its addition, they took longer than the MMAs
+    auto add2 = [&](auto& y, int q, int c, int r) {
+      constexpr int U = sizeof(y) / sizeof(float);
+      const uint32_t at = (uint32_t)(c * 128 + r) * 4u;
+      const uint32_t s0 = mapa_shared(base, (uint32_t)q) + at, s1 = mapa_shared(base, (uint32_t)q + 1) + at;
+      float v0[U], v1[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) v0[i] = ld_shared_cluster(s0 + (uint32_t)i * 512u);
+#pragma unroll
+      for (int i = 0; i < U; ++i) v1[i] = ld_shared_cluster(s1 + (uint32_t)i * 512u);
+#pragma unroll
+      for (int i = 0; i < U; ++i) y[i] = (y[i] + v0[i]) + v1[i];
+    };
     if (warp >= C::EPI0 && first < tiles) {
       const int tr = first / p.tiles_c, tc = first - tr * p.tiles_c;
       const int quad = warp & 3, half = (warp - C::EPI0) >> 2, r = quad * 32 + lane;
@@ -628,20 +651,20 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
         for (int c = rank * per + half; c < (rank + 1) * per; c += C::EW) {
           float y[8];
           bias8(p, tc * BN + 8 * c, y);
-          for (int q = 0; q < p.split; ++q) {
-            const uint32_t src = mapa_shared(base, (uint32_t)q) + (uint32_t)((8 * c) * 128 + r) * 4u;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] += ld_shared_cluster(src + (uint32_t)i * 512u);
-          }
+          for (int q = 0; q < p.split; q += 2) add2(y, q, 8 * c, r);
           store8<kF32>(p, tr * 128 + r, tc * BN + 8 * c, y);
         }
       } else {
+        constexpr int U = BN / 8;   // columns at a time: the share of one of 8 ranks
         const int cols = BN / p.split;
-        for (int c = rank * cols + half; c < (rank + 1) * cols; c += C::EW) {
-          float y = 0.f;
-          for (int q = 0; q < p.split; ++q)
-            y += ld_shared_cluster(mapa_shared(base, (uint32_t)q) + (uint32_t)(c * 128 + r) * 4u);
-          store1<kF32>(p, tc * BN + c, tr * 128 + r, y);
+        const float bias = bias_at(p, tr * 128 + r);
+        for (int c = rank * cols + half * U; c < (rank + 1) * cols; c += C::EW * U) {
+          float y[U];
+#pragma unroll
+          for (int i = 0; i < U; ++i) y[i] = 0.f;
+          for (int q = 0; q < p.split; q += 2) add2(y, q, c, r);
+#pragma unroll
+          for (int i = 0; i < U; ++i) store1<kF32>(p, tc * BN + c + i, tr * 128 + r, y[i] + bias);
         }
       }
     }
@@ -663,13 +686,13 @@ __global__ void __launch_bounds__(F8Cfg<BN, kSwap>::THREADS, 1)
 }
 
 // ---------------------------------------------------------------------------------------
-// Linear layer of up to 4 rows (a decoder's token, a class token): cast and product in one launch.  Bound by
+// Linear layer of one or two rows (a decoder's token, a class token): cast and product in one launch.  Bound by
 // reading the weight once.  Every CTA casts the rows for itself into shared memory (decoded: code * scale, in
 // the order in which the lanes read them), while its warps' first weights are on their way; then a warp takes
 // two weight rows at a time, 512 columns (16 per lane) by 512.  The tensor core would pad the rows to 16 and
 // needs a cast kernel before it and a reduction after it.
 // ---------------------------------------------------------------------------------------
-constexpr int kVecRows = 4, kVecWarps = 8;
+constexpr int kVecRows = 2, kVecChunks = 4, kVecWarps = 8;
 
 struct F8Vec {
   const void* x;
@@ -699,16 +722,24 @@ __global__ void __launch_bounds__(kVecWarps * 32, 2) fp8_linear_rows_kernel(cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wid = blockIdx.x * kVecWarps + warp, total = gridDim.x * kVecWarps;
   const int row_floats = a.chunks * 512;
-  // two weight rows n and n + total, chunk by chunk
-  uint4 w[2];
-  auto fetch = [&](int n, int c, uint4* d) {
+  // two weight rows n and n + total, chunk by chunk, kDeep chunks on their way
+  constexpr int kDeep = 2;
+  uint4 w[kDeep][2];
+  int fn = wid, fc = 0;
+  auto fetch = [&](uint4* d) {
+    if (fn >= p.N) return;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = n + i * total;
-      d[i] = r < p.N ? load_codes(a.b + (int64_t)r * a.ldb, c * 512 + lane * 16, a.K) : make_uint4(0, 0, 0, 0);
+      const int r = fn + i * total;
+      d[i] = r < p.N ? load_codes(a.b + (int64_t)r * a.ldb, fc * 512 + lane * 16, a.K) : make_uint4(0, 0, 0, 0);
+    }
+    if (++fc == a.chunks) {
+      fc = 0;
+      fn += 2 * total;
     }
   };
-  fetch(wid, 0, w);
+#pragma unroll
+  for (int u = 0; u < kDeep; ++u) fetch(w[u]);
   // the cast: a warp per block of 128 columns, 4 per lane
   for (int i = warp; i < R * a.chunks * 4; i += kVecWarps) {
     const int m = i / (a.chunks * 4), g = i - m * (a.chunks * 4), k = g * 128 + lane * 4;
@@ -741,16 +772,18 @@ __global__ void __launch_bounds__(kVecWarps * 32, 2) fp8_linear_rows_kernel(cons
         make_float4(lo.x * q.scale, lo.y * q.scale, hi.x * q.scale, hi.y * q.scale);
   }
   __syncthreads();
-  for (int n = wid; n < p.N; n += 2 * total) {
-    float acc[2][R];
+  float acc[2][R];
+  int n = wid, c = 0;
+  while (n < p.N) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int u = 0; u < kDeep; ++u) {
+      if (n >= p.N) break;
+      if (c == 0) {
 #pragma unroll
-      for (int m = 0; m < R; ++m) acc[i][m] = 0.f;
-    for (int c = 0; c < a.chunks; ++c) {
-      const uint4 now[2] = {w[0], w[1]};
-      const bool last = c + 1 == a.chunks;
-      if (!last || n + 2 * total < p.N) fetch(last ? n + 2 * total : n, last ? 0 : c + 1, w);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int m = 0; m < R; ++m) acc[i][m] = 0.f;
+      }
       const int g = min(c * 4 + (lane >> 3), p.kb - 1);   // this lane's block (past K its codes are 0)
       float4 x[R][4];
 #pragma unroll
@@ -760,13 +793,13 @@ __global__ void __launch_bounds__(kVecWarps * 32, 2) fp8_linear_rows_kernel(cons
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float s = __ldg(p.sb + (int64_t)(min(n + i * total, p.N - 1) >> 7) * p.sb_n + g * p.sb_k);
-        const uint32_t u[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
+        const uint32_t v[4] = {w[u][i].x, w[u][i].y, w[u][i].z, w[u][i].w};
         float d[R];
 #pragma unroll
         for (int m = 0; m < R; ++m) d[m] = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 lo = e4m3x2_to_f32x2(u[j]), hi = e4m3x2_to_f32x2(u[j] >> 16);
+          const float2 lo = e4m3x2_to_f32x2(v[j]), hi = e4m3x2_to_f32x2(v[j] >> 16);
 #pragma unroll
           for (int m = 0; m < R; ++m) {
             d[m] = fmaf(lo.x, x[m][j].x, d[m]);
@@ -778,42 +811,42 @@ __global__ void __launch_bounds__(kVecWarps * 32, 2) fp8_linear_rows_kernel(cons
 #pragma unroll
         for (int m = 0; m < R; ++m) acc[i][m] = fmaf(d[m], s, acc[i][m]);
       }
-    }
+      fetch(w[u]);
+      if (++c == a.chunks) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int m = 0; m < R; ++m) {
+          for (int m = 0; m < R; ++m) {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) acc[i][m] += __shfl_xor_sync(0xFFFFFFFFu, acc[i][m], o);
-        if (lane == 0) store1<sizeof(T) == 4>(p, m, n + i * total, acc[i][m]);
+            for (int o = 16; o; o >>= 1) acc[i][m] += __shfl_xor_sync(0xFFFFFFFFu, acc[i][m], o);
+            if (lane == 0) store1<sizeof(T) == 4>(p, m, n + i * total, acc[i][m] + bias_at(p, n + i * total));
+          }
+        c = 0;
+        n += 2 * total;
       }
+    }
   }
 }
 
-// What the kernel above takes: its rows' decoded values fit shared memory twice per SM.
-static int rows_held(int64_t M) { return M == 3 ? 4 : (int)M; }
-static bool few_rows(int64_t M, int64_t K) {
-  return M <= kVecRows && rows_held(M) * ((K + 511) / 512) * 2048 <= 96 * 1024;
+// What the kernel above takes.  Measured, whole layer (cast and tensor-core product in brackets): 1 x 4096 x 1024
+// 3.7 us (6.7), 1 x 5120 x 1280 5.9 (6.5), 1 x 4096 x 2048 5.4 (6.7), 2 x 4096 x 1024 4.9 (6.7); beyond that its decoding of
+// the codes costs more than two launches: 1 x 16384 x 1024 7.6 (6.8), 1 x 1280 x 5120 9.7 (6.5), 2 x 16384 x 512 7.4 (5.8),
+// 2 x 1280 x 2560 8.4 (6.1), and with four rows 4 x 4096 x 1024 7.3 (6.7).
+static bool few_rows(int64_t M, int64_t N, int64_t K) {
+  const int64_t chunks = M * ((K + 511) / 512);
+  return M <= kVecRows && chunks <= kVecChunks && chunks * N <= 16384;
 }
 
 template <typename T>
 static int launch_rows(const F8Vec& a, const F8Params& p, cudaStream_t s) {
-  const int R = rows_held(p.M);
-  const size_t smem = (size_t)R * a.chunks * 2048;
+  const size_t smem = (size_t)p.M * a.chunks * 2048;
   const int sms = num_sms();
   int64_t grid = ((int64_t)p.N + 2 * kVecWarps - 1) / (2 * kVecWarps);   // two rows per warp, if that fills the machine
   if (grid < sms) grid = ((int64_t)p.N + kVecWarps - 1) / kVecWarps;
   if (grid > 2 * sms) grid = 2 * sms;
-  auto run = [&](auto kern) {
-    if (smem > 48 * 1024) {
-      if (int st = smem_optin(kern, 96 * 1024)) return st;
-    }
-    kern<<<(unsigned)grid, kVecWarps * 32, smem, s>>>(a, p);
-    return launch_status("vf4_linear_fp8_block");
-  };
-  if (R == 1) return run(fp8_linear_rows_kernel<T, 1>);
-  if (R == 2) return run(fp8_linear_rows_kernel<T, 2>);
-  return run(fp8_linear_rows_kernel<T, 4>);
+  if (p.M == 1) fp8_linear_rows_kernel<T, 1><<<(unsigned)grid, kVecWarps * 32, smem, s>>>(a, p);
+  else fp8_linear_rows_kernel<T, 2><<<(unsigned)grid, kVecWarps * 32, smem, s>>>(a, p);
+  return launch_status("vf4_linear_fp8_block");
 }
 
 static int make_code_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t K, int64_t ld, int box_rows) {
@@ -868,9 +901,15 @@ static int launch_fp8_gemm(F8Operand a, F8Operand b, int64_t K, F8Params p, cuda
   p.tiles_r = (int)((a.rows + C::ROWS - 1) / C::ROWS);
   p.tiles_c = (int)((b.rows + BN - 1) / BN);
   const int tiles = p.tiles_r * p.tiles_c, sms = num_sms();
-  // share a tile among up to 8 CTAs (the portable cluster size) while that leaves no SM two of them
+  // Share a tile among up to 8 CTAs (the portable cluster size) while all are resident at once, if that takes enough
+  // K blocks off each: joining the sums costs 1 us and more, a block 0.2 to 0.4.  16 x 1280 x 5120 takes 5.6 us shared
+  // by 8 and 13.4 alone, 257 x 1280 x 5120 11.8 (4) and 19.4, 257 x 1280 x 2560 9.7 (4) and 11.5; but 257 x 1280 x
+  // 1280 8.8 (4) and 7.8, 16 x 5120 x 1280 6.3 (2) and 5.9.  16 columns with two CTAs on most SMs already read
+  // the weight at the memory's rate: 16 x 16384 x 4096 takes 15.1 us alone, 16.5 shared by 2.
+  const int most = BN == 16 ? sms + sms / 4 : sms * C::PER_SM;
   p.split = 1;
-  while (!C::kPair && p.split < 8 && tiles * p.split * 2 <= sms && p.split * 2 <= p.kb) p.split *= 2;
+  while (!C::kPair && p.split < 8 && tiles * p.split * 2 <= most && p.split * 2 <= p.kb) p.split *= 2;
+  if (p.kb - p.kb / p.split < (kSwap ? 8 : 10)) p.split = 1;
   p.out_tma = !kSwap && !kF32 && p.split == 1 && p.out_vec;
   if (p.out_tma) {
     if (int st = make_bf16_out_map(&to, p.out, p.M, p.N, p.ldo)) return st;
@@ -878,7 +917,7 @@ static int launch_fp8_gemm(F8Operand a, F8Operand b, int64_t K, F8Params p, cuda
   cudaLaunchConfig_t cfg = {};
   const int pairs = sms / 2;
   cfg.gridDim = dim3((unsigned)(C::kPair ? 2 * (tiles < pairs ? tiles : pairs)
-                                         : p.split > 1 ? tiles * p.split : (tiles < sms ? tiles : sms)));
+                                         : p.split > 1 ? tiles * p.split : (tiles < sms * C::PER_SM ? tiles : sms * C::PER_SM)));
   cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;
@@ -895,11 +934,19 @@ static int launch_fp8_gemm(F8Operand a, F8Operand b, int64_t K, F8Params p, cuda
 
 template <bool kF32>
 static int dispatch_fp8_gemm(F8Operand x, F8Operand w, int64_t K, const F8Params& p, cudaStream_t s) {
+  // Up to 64 rows: operands swapped, in the narrowest tile that holds them.  16 x 5120 x 1280 takes 6.0 us with 16
+  // columns, 6.5 with 32, 9.8 unswapped; 32 x 5120 x 5120 10.3 with 32, 12.8 with 64, 15.5 unswapped; 64 x 5120 x 1280 7.1 with
+  // 64 and 9.9 unswapped; 65 x 5120 x 5120 15.7 unswapped and 18.4 in two tiles of 64.
   if (x.rows <= 16) return launch_fp8_gemm<16, true, kF32>(w, x, K, p, s);
   if (x.rows <= 32) return launch_fp8_gemm<32, true, kF32>(w, x, K, p, s);
   if (x.rows <= 64) return launch_fp8_gemm<64, true, kF32>(w, x, K, p, s);
-  const int64_t big = (x.rows + 255) / 256 * ((w.rows + 255) / 256);
-  if (big >= num_sms() / 2) return launch_fp8_gemm<256, false, kF32>(x, w, K, p, s);
+  // A round of 256 x 256 tiles (a pair of SMs each) takes 1.5 times a round of 128 x 128 tiles (one SM each): 2056 x
+  // 1280 x 5120 is one round in 29 us against two in 37, 4112 x 5120 x 1280 five in 41 against nine in 48; but 1024 x 2048 x 2048
+  // one in 15.8 against one in 10.8.
+  const int64_t sms = num_sms(), pairs = sms / 2;
+  const int64_t big = ((x.rows + 255) / 256 * ((w.rows + 255) / 256) + pairs - 1) / pairs;
+  const int64_t small = ((x.rows + 127) / 128 * ((w.rows + 127) / 128) + sms - 1) / sms;
+  if (3 * big <= 2 * small) return launch_fp8_gemm<256, false, kF32>(x, w, K, p, s);
   return launch_fp8_gemm<128, false, kF32>(x, w, K, p, s);
 }
 
@@ -1006,8 +1053,8 @@ int vf4_gemm_fp8_block(const uint8_t* a, int64_t lda, const float* a_scale, int6
 }
 
 // workspace of vf4_linear_fp8_block: the rows' codes, then their scales, column block by column block
-int64_t vf4_linear_fp8_block_workspace_size(int64_t M, int64_t K) {
-  if (M <= 0 || K <= 0 || M > (1 << 30) || K > (1 << 20) || few_rows(M, K)) return 0;
+int64_t vf4_linear_fp8_block_workspace_size(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0 || M > (1 << 30) || N > (1 << 24) || K > (1 << 20) || few_rows(M, N, K)) return 0;
   return M * ((K + 15) / 16 * 16) + M * ((K + 127) / 128) * 4;
 }
 
@@ -1015,12 +1062,12 @@ int vf4_linear_fp8_block(const void* x, int dtype, int64_t M, int64_t K, int64_t
                          const float* w_scale, int64_t ws_n, int64_t ws_k, int64_t N, const void* bias, int bias_dtype,
                          void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, vf4_stream_t stream) {
   if (int st = check_device()) return st;
-  const int64_t need = vf4_linear_fp8_block_workspace_size(M, K);
+  const int64_t need = vf4_linear_fp8_block_workspace_size(M, N, K);
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(VF4_ERR_ARG, "vf4_linear_fp8_block: %lld bytes of 16-byte aligned workspace needed, got %lld", (long long)need,
                 (long long)workspace_bytes);
-  if (M > 0 && few_rows(M, K)) {
-    if (K <= 0 || N <= 0 || ldx < K || ldo < N || N > (1 << 24))
+  if (M > 0 && N > 0 && K > 0 && few_rows(M, N, K)) {
+    if (ldx < K || ldo < N)
       return fail(VF4_ERR_ARG, "vf4_linear_fp8_block: bad sizes M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
     if ((dtype != VF4_BF16 && dtype != VF4_F32) || (bias && bias_dtype != VF4_BF16 && bias_dtype != VF4_F32))
       return fail(VF4_ERR_ARG, "vf4_linear_fp8_block: bad dtype");

@@ -60,7 +60,7 @@ SIGNATURES: dict[str, list] = {
     "vf4_attn_workspace_size_modes": [_L, _L, _L, _L, _I, _I, _I],
     "vf4_cast_fp8_block": [_P, _I, _L, _L, _L, _I, _P, _L, _P, _L, _L, _P],
     "vf4_gemm_fp8_block": [_P, _L, _P, _L, _L, _P, _L, _P, _L, _L, _L, _L, _L, _P, _I, _P, _L, _I, _P],
-    "vf4_linear_fp8_block_workspace_size": [_L, _L],
+    "vf4_linear_fp8_block_workspace_size": [_L, _L, _L],
     "vf4_linear_fp8_block": [_P, _I, _L, _L, _L, _P, _L, _P, _L, _L, _L, _P, _I, _P, _L, _P, _L, _P],
     "vf4_gated_residual_norm": [_P, _L, _P, _L, _I, _L, _L, _P, _L, ctypes.c_float, _I, _P, _P, _I, _P, _P, _I,
                                 ctypes.c_float, _P, _P, _I, _L, _P, _L, _L, _P],

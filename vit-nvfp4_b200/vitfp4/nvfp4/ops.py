@@ -337,7 +337,7 @@ def linear_fp8_block(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
     x, w = _rows_2d(x), _code_rows(w)
     (M, K), N, dev = x.shape, w.shape[0], x.device
     out = torch.empty_strided((M, N), (N, 1), dtype=x.dtype, device=dev)
-    n = _lib.lib().vf4_linear_fp8_block_workspace_size(M, K)
+    n = _lib.lib().vf4_linear_fp8_block_workspace_size(M, N, K)
     ws = torch.empty_strided((n,), (1,), dtype=_U8, device=dev) if n else None
     ws_n, ws_k = w_scale.stride()
     _call("vf4_linear_fp8_block", "linear_fp8_block", (M, N, K), 2.0 * M * N * K, x.data_ptr(), code, M, K, _ld(x),
