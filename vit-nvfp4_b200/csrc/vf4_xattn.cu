@@ -334,6 +334,9 @@ struct XCfg {
   static constexpr int BAR_OFF = KX_OFF + NK * EXT;
   static constexpr int NBAR = 3 * (NK + NV) + 6;
   static constexpr int SMEM = 1024 + BAR_OFF + 8 * NBAR + 16;
+  // 4 x 16 heads of 1024 x 4096 x 128: 146 us with 3, 152 with 4, 157 with 2; 32 x 16 of 64 x 1025 x 80: 36.4, 38.2 and
+  // 36.9; 8 x 16 of 1024 x 4096 x 64: 197 with 4, 200 with 3, 205 without the polynomial
+  static constexpr int kPolyEvery = DP == 64 ? 4 : 3;
   static constexpr int THREADS = 256;
   static constexpr int kLaunchRegs = 128, kControlRegs = 40, kSoftRegs = 216;
   static_assert(128 * kControlRegs + 128 * kSoftRegs <= THREADS * kLaunchRegs, "register split");
@@ -377,7 +380,6 @@ VF4_DEV unsigned long long ex2_poly_x2(unsigned long long x) {
                     __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23)));
 }
 
-constexpr int kPolyEvery = 4;
 
 template <int DP>
 __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
@@ -677,7 +679,7 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
           for (int e = 32 * h; e < 32 * h + 32; ++e) {
             const unsigned long long x = fma_f32x2(f32x2_pack(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), c2, nm2);
             unsigned long long pr;
-            if (e % kPolyEvery == kPolyEvery - 1) {
+            if (e % C::kPolyEvery == C::kPolyEvery - 1) {
               pr = ex2_poly_x2(x);
             } else {
               float x0, x1;
