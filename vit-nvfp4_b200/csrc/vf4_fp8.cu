@@ -30,10 +30,11 @@ int fp8_device_error(int clear) {
 // The blocks of all rows are numbered in one sequence, row by row, and dealt to the half-warps, so
 // short and long rows fill the machine alike.  Bound by memory: 1 byte out per 2 (bf16) or 4 (fp32)
 // bytes in; kU blocks per half-warp are loaded before the first is reduced, to keep enough bytes in
-// flight (16400 x 5120 bf16: 59 us with 4, 61 with 2, 73 with 1).
+// flight, as few as leave registers for five CTAs per SM (16400 x 1280 and 16400 x 5120 bf16: 16.6 and 58.2 us with two
+// blocks; 17.4 and 58.9 with four and four CTAs, 17.5 and 61.3 with three, 20.6 and 72.5 with one).
 // ---------------------------------------------------------------------------------------
 template <typename T, bool kVec, int kU>
-__global__ void __launch_bounds__(256, 4) fp8_cast_rows_kernel(const T* __restrict__ x, int64_t M, int K, int64_t ld,
+__global__ void __launch_bounds__(256, 5) fp8_cast_rows_kernel(const T* __restrict__ x, int64_t M, int K, int64_t ld,
                                                                uint8_t* __restrict__ codes, int64_t ldc,
                                                                float* __restrict__ scale, int64_t s_m, int64_t s_k) {
   const int kb = (K + 127) >> 7;
@@ -978,11 +979,11 @@ int vf4_cast_fp8_block(const void* x, int dtype, int64_t M, int64_t K, int64_t l
   const auto* xf = static_cast<const float*>(x);
   if (block_rows == 1) {
     const int64_t want = (M * kb + 15) / 16;   // 16 blocks per CTA and step
-    const int64_t most = (int64_t)num_sms() * 4;   // the CTAs that are resident at once
+    const int64_t most = (int64_t)num_sms() * 5;   // the CTAs that are resident at once
     const unsigned grid = (unsigned)(want < most ? want : most);
     const int K32 = (int)K;
 #define VF4_CAST_ROWS(T, X, V) \
-  fp8_cast_rows_kernel<T, V, 4><<<grid, 256, 0, s>>>(X, M, K32, ld, codes, ldc, scale, stride_m, stride_k)
+  fp8_cast_rows_kernel<T, V, 2><<<grid, 256, 0, s>>>(X, M, K32, ld, codes, ldc, scale, stride_m, stride_k)
     if (dtype == VF4_BF16) {
       if (vec) VF4_CAST_ROWS(__nv_bfloat16, xb, true);
       else VF4_CAST_ROWS(__nv_bfloat16, xb, false);
