@@ -46,6 +46,10 @@ def _calls():
         ("norm", 1, lambda: api.gated_residual_norm(x, y, gate=gate, residual_scale=0.5, post_weight=nw, pre_weight=nw, pre_bias=nw)),
         ("norm rms f32", 1, lambda: api.gated_residual_norm(x.float(), y.float(), norm="rms")),
         ("norm fp8", 1, lambda: api.gated_residual_norm(x, y, gate=gate[0], pre_weight=nw, out_dtype=F8)),
+        ("cast 3d", 1, lambda: api.quantize_to_fp8_block(x.view(2, 3, 256))),
+        ("linear 4d", 2, lambda: api.fp8_block_linear(many.view(3, 5, 6, 256), w, ws, bias=bias)),
+        ("norm 3d", 1, lambda: api.gated_residual_norm(x.view(3, 2, 256), y.view(3, 2, 256), gate=gate, norm="rms")),
+        ("norm fp8 3d", 1, lambda: api.gated_residual_norm(x.view(3, 2, 256), y.view(3, 2, 256), out_dtype=F8)),
         ("cross", 1, lambda: api.cross_sdpa(q, k, v, kv_lens=lens, scale=0.2)),
         ("cross mask", 1, lambda: api.cross_sdpa(q, k, v, key_mask=mask)),
         ("cross chunks", 2, lambda: api.cross_sdpa(q, k.repeat(1, 1, 3, 1), v.repeat(1, 1, 3, 1))),
@@ -75,7 +79,7 @@ def test_both_paths_give_the_same(monkeypatch):
             assert a.shape == b.shape and a.dtype == b.dtype and a.stride() == b.stride(), name
             assert torch.equal(a.float(), b.float()), name
         taken.append(name)
-    assert len(ops.probe.records) and len(taken) == 12
+    assert len(ops.probe.records) and len(taken) == 16
     ops.probe.reset()
 
 
@@ -99,3 +103,21 @@ def test_calls_that_are_not_plain_go_the_python_way():
         assert m.norm(y, y, None, 1.0, kind, None, None, None, None, 1e-6, False) is None
     with pytest.raises(Exception):
         api.gated_residual_norm(y, y, norm=None)
+
+
+@pytest.mark.gpu
+def test_calls_that_only_look_alike():
+    from vitfp4 import _lib
+    from vitfp4 import nvfp4 as api
+    x = torch.randn(2, 3, 256, device="cuda").bfloat16()
+    w, ws = api.quantize_to_fp8_block(torch.randn(64, 256, device="cuda"), 128)
+    with pytest.raises(_lib.VitFp4Error):      # as many rows, another shape
+        api.gated_residual_norm(x, x.view(3, 2, 256))
+    turned = x.transpose(0, 1)                 # not contiguous: rows in another order
+    assert torch.equal(api.fp8_block_linear(turned, w, ws), api.fp8_block_linear(turned.contiguous(), w, ws))
+    assert torch.equal(api.gated_residual_norm(turned, turned)[1], api.gated_residual_norm(turned.contiguous(), turned.contiguous())[1])
+    empty = x[:, :0]
+    assert api.fp8_block_linear(empty, w, ws).shape == (2, 0, 64) and api.quantize_to_fp8_block(empty)[1].shape == (2, 0, 2)
+    assert api.gated_residual_norm(empty, empty, out_dtype=F8)[1][1].shape == (2, 0, 2)
+    one = x[0, 0]
+    assert torch.equal(api.fp8_block_linear(one, w, ws), api.fp8_block_linear(one[None], w, ws)[0])

@@ -5,7 +5,8 @@
 // calls the C ABI of libvitfp4.so on torch's current stream and returns the outputs -- or returns None, without having
 // done anything, for whatever is not the plain case: then the caller goes the Python path, which copes with it
 // (copies, other devices, the probe, torch.library where gradients are recorded) or says what is wrong.  Plain means:
-// exact tensors on the current CUDA device, no gradients recorded, layouts that the kernels read as they are.
+// exact tensors on the current CUDA device, no gradients recorded, layouts that the kernels read as they are (more than
+// two dimensions: contiguous).
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
@@ -67,6 +68,19 @@ bool rows_ok(const at::Tensor& t, int64_t* ld) {
   return true;
 }
 
+// (..., K) as rows: a contiguous tensor of more dimensions as (rows, K); others as they are.
+at::Tensor rows_of(const at::Tensor& t) {
+  return t.defined() && t.dim() > 2 && t.numel() > 0 && t.is_contiguous() ? t.view({-1, t.size(-1)}) : t;
+}
+
+// Rows (rows, n) of an output with x's leading dimensions.
+at::Tensor like_x(const at::Tensor& rows, const at::Tensor& x) {
+  if (x.dim() == 2) return rows;
+  c10::SmallVector<int64_t, 6> size(x.sizes().begin(), x.sizes().end());
+  size.back() = rows.size(1);
+  return rows.view(size);
+}
+
 bool vector_ok(const at::Tensor& t, int64_t n) { return !t.defined() || (t.dim() == 1 && t.size(0) == n && (n == 1 || t.stride(0) == 1)); }
 
 const void* ptr(const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
@@ -102,7 +116,7 @@ PyObject* cast(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 1) return nullptr;
     Args in;
-    const at::Tensor x = in.get(a[0]);
+    const at::Tensor x0 = in.get(a[0]), x = rows_of(x0);
     int64_t ld;
     if (!in.ok || code_of(x) < 0 || !rows_ok(x, &ld) || x.size(1) % 16) return nullptr;
     const int64_t M = x.size(0), K = x.size(1), kb = (K + 127) / 128;
@@ -111,7 +125,7 @@ PyObject* cast(PyObject*, PyObject* const* a, Py_ssize_t n) {
                            static_cast<float*>(scale.mutable_data_ptr()), 1, M, stream(in.device)))
       return nullptr;
     g_launched = 1;
-    return pair(codes, scale);
+    return pair(like_x(codes, x0), like_x(scale, x0));
   });
 }
 
@@ -120,7 +134,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 4) return nullptr;
     Args in;
-    const at::Tensor x = in.get(a[0]), w = in.get(a[1]), ws = in.get(a[2]), bias = in.get(a[3], true);
+    const at::Tensor x0 = in.get(a[0]), x = rows_of(x0), w = in.get(a[1]), ws = in.get(a[2]), bias = in.get(a[3], true);
     int64_t ld, ldw;
     if (!in.ok || code_of(x) < 0 || !rows_ok(x, &ld) || w.scalar_type() != at::kFloat8_e4m3fn || !rows_ok(w, &ldw) ||
         ldw % 16 || reinterpret_cast<uintptr_t>(w.const_data_ptr()) % 16)
@@ -138,7 +152,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
                              need ? work.mutable_data_ptr() : nullptr, need, stream(in.device)))
       return nullptr;
     g_launched = need ? 2 : 1;
-    return THPVariable_Wrap(y);
+    return THPVariable_Wrap(like_x(y, x0));
   });
 }
 
@@ -148,7 +162,7 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 11) return nullptr;
     Args in;
-    const at::Tensor x = in.get(a[0]), y = in.get(a[1]), gate = in.get(a[2], true);
+    const at::Tensor x0 = in.get(a[0]), y0 = in.get(a[1]), x = rows_of(x0), y = rows_of(y0), gate = in.get(a[2], true);
     at::Tensor p[4];
     for (int i = 0; i < 4; ++i) p[i] = in.get(a[5 + i], true);
     const double rs = PyFloat_AsDouble(a[3]), eps = PyFloat_AsDouble(a[9]);
@@ -160,7 +174,7 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (kind != 1 && kind != 2) return nullptr;
     const bool fp8 = a[10] == Py_True;
     int64_t ldx, ldy;
-    if (!in.ok || code_of(x) < 0 || !rows_ok(x, &ldx) || !rows_ok(y, &ldy) || y.sizes() != x.sizes() ||
+    if (!in.ok || code_of(x) < 0 || !rows_ok(x, &ldx) || !rows_ok(y, &ldy) || y0.sizes() != x0.sizes() ||
         y.scalar_type() != x.scalar_type())
       return nullptr;
     const int64_t M = x.size(0), K = x.size(1), kb = (K + 127) / 128;
@@ -190,14 +204,14 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                 fp8 ? static_cast<float*>(scale.mutable_data_ptr()) : nullptr, 1, M, stream(in.device)))
       return nullptr;
     g_launched = 1;
-    if (!fp8) return pair(out, h);
-    PyObject* codes = pair(h, scale);
+    if (!fp8) return pair(like_x(out, x0), like_x(h, x0));
+    PyObject* codes = pair(like_x(h, x0), like_x(scale, x0));
     PyObject* r = codes ? PyTuple_New(2) : nullptr;
     if (!r) {
       Py_XDECREF(codes);
       return nullptr;
     }
-    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(out));
+    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(like_x(out, x0)));
     PyTuple_SET_ITEM(r, 1, codes);
     return r;
   });

@@ -107,7 +107,7 @@ def quantize_to_fp8_block(x: torch.Tensor, block_rows: int = 1):
     codes, scale = (cast_fp8_block_op if _traced(x) else ops.cast_fp8_block)(x2, block_rows)
     if x.dim() == 2:
         return codes, scale
-    return codes.unflatten(0, x.shape[:-1]) if x.dim() > 1 else codes[0], scale.reshape(*x.shape[:-1], -1)
+    return codes.unflatten(0, x.shape[:-1]) if x.dim() > 1 else codes[0], scale.reshape(*x.shape[:-1], scale.shape[-1])
 
 
 def dequantize_fp8_block(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:

@@ -109,5 +109,5 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, norm="layer", po
     new = x if y is None else new if x.dim() == 2 else new.view(x.shape)
     if h is not None and x.dim() != 2:
         h = h.unflatten(0, x.shape[:-1]) if x.dim() > 1 else h[0]
-        scale = None if scale is None else scale.reshape(*x.shape[:-1], -1)
+        scale = None if scale is None else scale.reshape(*x.shape[:-1], scale.shape[-1])
     return new, ((h, scale) if fp8 else h)
