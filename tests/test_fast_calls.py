@@ -50,6 +50,10 @@ def _calls():
         ("linear 4d", 2, lambda: api.fp8_block_linear(many.view(3, 5, 6, 256), w, ws, bias=bias)),
         ("norm 3d", 1, lambda: api.gated_residual_norm(x.view(3, 2, 256), y.view(3, 2, 256), gate=gate, norm="rms")),
         ("norm fp8 3d", 1, lambda: api.gated_residual_norm(x.view(3, 2, 256), y.view(3, 2, 256), out_dtype=F8)),
+        ("cast odd", 1, lambda: api.quantize_to_fp8_block(x.float()[:, :201])),
+        ("cast odd 3d", 1, lambda: api.quantize_to_fp8_block(x[:, :130].reshape(2, 3, 130).contiguous())),
+        ("linear odd", 2, lambda: api.fp8_block_linear(many[:, :201], *api.quantize_to_fp8_block(many[:64, :201], 128))),
+        ("norm fp8 odd 3d", 1, lambda: api.gated_residual_norm(*[t[:, :201].reshape(2, 3, 201).contiguous() for t in (x, y)], out_dtype=F8)),
         ("cross", 1, lambda: api.cross_sdpa(q, k, v, kv_lens=lens, scale=0.2)),
         ("cross mask", 1, lambda: api.cross_sdpa(q, k, v, key_mask=mask)),
         ("cross chunks", 2, lambda: api.cross_sdpa(q, k.repeat(1, 1, 3, 1), v.repeat(1, 1, 3, 1))),
@@ -79,7 +83,7 @@ def test_both_paths_give_the_same(monkeypatch):
             assert a.shape == b.shape and a.dtype == b.dtype and a.stride() == b.stride(), name
             assert torch.equal(a.float(), b.float()), name
         taken.append(name)
-    assert len(ops.probe.records) and len(taken) == 16
+    assert len(ops.probe.records) and len(taken) == 20
     ops.probe.reset()
 
 
@@ -88,7 +92,7 @@ def test_calls_that_are_not_plain_go_the_python_way():
     from vitfp4 import nvfp4 as api
     m = _module()
     x = torch.randn(6, 100, device="cuda").bfloat16()
-    assert m.cast(x) is None                                   # padded code rows
+    assert m.cast(x) is not None and m.cast(x[:, ::2]) is None  # columns apart
     assert m.cast(x.t()) is None and m.cast(x[:0]) is None     # copies, nothing to do
     p = torch.nn.Parameter(torch.randn(4, 128, device="cuda"))
     assert m.cast(p) is None                                   # gradients recorded

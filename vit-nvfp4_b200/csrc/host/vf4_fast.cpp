@@ -111,17 +111,23 @@ PyObject* guarded(F&& f) {
   Py_RETURN_NONE;
 }
 
-// cast(x) -> (codes, scale): activations, K a multiple of 16
+// Code rows of K bytes, each starting on 16 bytes: the first K columns of padded rows.
+at::Tensor make_codes(int64_t M, int64_t K, int64_t ldc, const at::Tensor& like) {
+  const at::Tensor t = make({M, ldc}, {ldc, 1}, at::kFloat8_e4m3fn, like);
+  return ldc == K ? t : t.narrow(1, 0, K);
+}
+
+// cast(x) -> (codes, scale): activations
 PyObject* cast(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 1) return nullptr;
     Args in;
     const at::Tensor x0 = in.get(a[0]), x = rows_of(x0);
     int64_t ld;
-    if (!in.ok || code_of(x) < 0 || !rows_ok(x, &ld) || x.size(1) % 16) return nullptr;
-    const int64_t M = x.size(0), K = x.size(1), kb = (K + 127) / 128;
-    at::Tensor codes = make({M, K}, {K, 1}, at::kFloat8_e4m3fn, x), scale = make({M, kb}, {1, M}, at::kFloat, x);
-    if (vf4_cast_fp8_block(x.const_data_ptr(), code_of(x), M, K, ld, 1, static_cast<uint8_t*>(codes.mutable_data_ptr()), K,
+    if (!in.ok || code_of(x) < 0 || !rows_ok(x, &ld)) return nullptr;
+    const int64_t M = x.size(0), K = x.size(1), kb = (K + 127) / 128, ldc = (K + 15) / 16 * 16;
+    at::Tensor codes = make_codes(M, K, ldc, x), scale = make({M, kb}, {1, M}, at::kFloat, x);
+    if (vf4_cast_fp8_block(x.const_data_ptr(), code_of(x), M, K, ld, 1, static_cast<uint8_t*>(codes.mutable_data_ptr()), ldc,
                            static_cast<float*>(scale.mutable_data_ptr()), 1, M, stream(in.device)))
       return nullptr;
     g_launched = 1;
@@ -157,7 +163,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // norm(x, y, gate, residual_scale, kind, post_w, post_b, pre_w, pre_b, eps, fp8) -> (x', h | (codes, scale)):
-// both norms, of one kind (1 LayerNorm, 2 RMSNorm); FP8 with K a multiple of 16
+// both norms, of one kind (1 LayerNorm, 2 RMSNorm)
 PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     if (n != 11) return nullptr;
@@ -177,8 +183,7 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!in.ok || code_of(x) < 0 || !rows_ok(x, &ldx) || !rows_ok(y, &ldy) || y0.sizes() != x0.sizes() ||
         y.scalar_type() != x.scalar_type())
       return nullptr;
-    const int64_t M = x.size(0), K = x.size(1), kb = (K + 127) / 128;
-    if (fp8 && K % 16) return nullptr;
+    const int64_t M = x.size(0), K = x.size(1), kb = (K + 127) / 128, ldc = (K + 15) / 16 * 16;
     int64_t groups = 1;
     int pcode = -1;
     if (gate.defined()) {
@@ -196,11 +201,11 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (pcode < 0) pcode = code_of(x);
     if (pcode != VF4_F32 && pcode != code_of(x)) return nullptr;
     at::Tensor out = make({M, K}, {K, 1}, x.scalar_type(), x), h, scale;
-    h = make({M, K}, {K, 1}, fp8 ? at::kFloat8_e4m3fn : x.scalar_type(), x);
+    h = fp8 ? make_codes(M, K, ldc, x) : make({M, K}, {K, 1}, x.scalar_type(), x);
     if (fp8) scale = make({M, kb}, {1, M}, at::kFloat, x);
     if (vf4_gated_residual_norm(x.const_data_ptr(), ldx, y.const_data_ptr(), ldy, code_of(x), M, K, ptr(gate), groups,
                                 (float)rs, (int)kind, ptr(p[0]), ptr(p[1]), (int)kind, ptr(p[2]), ptr(p[3]), pcode,
-                                (float)eps, out.mutable_data_ptr(), h.mutable_data_ptr(), fp8, fp8 ? K : 0,
+                                (float)eps, out.mutable_data_ptr(), h.mutable_data_ptr(), fp8, fp8 ? ldc : 0,
                                 fp8 ? static_cast<float*>(scale.mutable_data_ptr()) : nullptr, 1, M, stream(in.device)))
       return nullptr;
     g_launched = 1;
