@@ -5,7 +5,6 @@ Layout of one case: ``kind`` is ``cast`` (activation cast to E4M3 codes with a s
 ``cross`` (attention of queries over keys of another length) or ``norm`` (post-norm, gate, residual scale,
 residual add, pre-norm, optionally cast to the FP8 block format).
 """
-import functools
 import math
 import os
 import sys
@@ -18,9 +17,8 @@ DT = {"bf16": torch.bfloat16, "f32": torch.float32}
 F8 = torch.float8_e4m3fn
 
 
-@functools.lru_cache(maxsize=None)
 def _api():
-    """The framework's package, imported once as a user's program does (its folder holds a hyphen, so by path)."""
+    """The framework's package (its folder is not importable by name: it holds a hyphen)."""
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "vit-nvfp4_b200")
     if path not in sys.path:
         sys.path.insert(0, path)
