@@ -79,8 +79,9 @@ VF4_DEV void store_row8(T* p, int nv, const Pair* v) {
   }
 }
 
-// Sum over a row's threads: a warp, or a CTA (area: a float per warp; every call within a row has its own, so
-// one barrier per call is enough).
+// Sum over a row's threads: a warp, or a CTA (area: a float per warp).  One barrier per call: a call's area may be
+// written again by the second call after it, whose writers have passed the barrier of the call between, which every
+// reader reaches only after its reads.  So neighbouring calls take different areas, also from one row to the next.
 template <int kThreads>
 VF4_DEV float row_sum(float v, float* area) {
 #pragma unroll
@@ -219,7 +220,10 @@ VF4_DEV void affine8(Pair* v, float r, const void* w, const void* b, int col, in
 // h, 1 h in T, 2 FP8.
 template <typename T, typename P, int kThreads, int NV, bool kVec, int kOut>
 __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads, kThreads == 32 ? (NV > 4 ? 2 : 3) : 1) gated_norm_kernel(const NormParams p) {
+  // one of the two per norm, in turn: with one norm per row, too, no warp writes the area that another may still be
+  // reading for the row before
   __shared__ float red[2][3 * (kThreads / 32)];
+  int side = 0;
   constexpr int kRows = kThreads == 32 ? 8 : 1;
   const int t = kThreads == 32 ? (threadIdx.x & 31) : threadIdx.x;
   const T *X = static_cast<const T*>(p.x), *Y = static_cast<const T*>(p.y);
@@ -244,7 +248,10 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads, kThreads == 3
 #pragma unroll
       for (int j = 0; j < NV; ++j) pairs8(yr[j], v[j]);
       float r2 = 1.f;
-      if (p.post != kNormNone) r2 = centre<kThreads, NV, kVec>(v, nv, p.post, p.K, p.eps, red[0]);
+      if (p.post != kNormNone) {
+        r2 = centre<kThreads, NV, kVec>(v, nv, p.post, p.K, p.eps, red[side]);
+        side ^= 1;
+      }
       const int64_t gate_row = p.gate ? (int64_t)((uint32_t)row / p.rows_per_gate) * p.K : 0;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -273,7 +280,8 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads, kThreads == 3
       for (int j = 0; j < NV; ++j) pairs8(xr[j], v[j]);
     }
     if constexpr (kOut != 0) {
-      const float r1 = centre<kThreads, NV, kVec>(v, nv, p.pre, p.K, p.eps, red[1]);
+      const float r1 = centre<kThreads, NV, kVec>(v, nv, p.pre, p.K, p.eps, red[side]);
+      side ^= 1;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int col = (j * kThreads + t) * 8;
