@@ -75,3 +75,24 @@ def test_fp8_output_of_many_rows(M, K):
     d = dequantize_fp8_block(codes, scale).double()
     assert ((d - hw).abs() <= step * (1 + 2.0 ** -20) + 2 * e2).all()
     assert DT["bf16"] == new.dtype
+
+
+@pytest.mark.parametrize("size", [1.0, 5e37, 2e-13, float("inf")])
+@pytest.mark.parametrize("M,K", [(5, 100), (300, 1024), (3000, 1280), (33, 2048), (9, 5120), (7, 3001)])
+def test_fp8_output_is_bit_for_bit_the_cast(M, K, size):
+    """fp32 rows come out unrounded, so casting them has to give the codes and scales that the fused output holds: at a
+    usual size, above 2^126 (where an approximate quotient 448 / amax would be 0), at a block maximum near the least
+    one, and with an infinite value in every row."""
+    from vitfp4.nvfp4 import gated_residual_norm, quantize_to_fp8_block
+    x, y, gate, w2, _, w1, _ = _case(M, K, "f32", 1, True, "rms", seed=K)
+    if size == float("inf"):
+        w1[K // 3] = size
+    else:
+        w1 = w1 * size
+    kw = dict(gate=gate, residual_scale=0.5, norm="rms", post_weight=w2, pre_weight=w1, eps=EPS)
+    _, h = gated_residual_norm(x, y, **kw)
+    assert h.abs().amax() > 2.0 ** 126 if size > 1 else h.isfinite().all()
+    _, (codes, scale) = gated_residual_norm(x, y, out_dtype=torch.float8_e4m3fn, **kw)
+    want, ws = quantize_to_fp8_block(h)
+    assert torch.equal(scale, ws)
+    assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8))

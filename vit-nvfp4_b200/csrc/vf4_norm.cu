@@ -299,17 +299,9 @@ __global__ void __launch_bounds__(kThreads == 32 ? 256 : kThreads, kThreads == 3
 #pragma unroll
           for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
           if (nv[j] > 0) {
-            // the quotient as one product: h is itself an fp32 result, off by more than the product's two
-            // roundings (the cast's correctly rounded quotient costs four times as much here)
-            float a = __uint_as_float(m);
-            a = a < 1e-12f ? 1e-12f : a;
-            const float q = __fdividef(448.f, a);
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = e4m3x2(f[2 * i] * q, f[2 * i + 1] * q);
-            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.h) + row * p.ldc + col) =
-                make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-            if ((t & 15) == 0) p.scale[row * p.s_m + (col >> 7) * p.s_k] = __fdiv_rn(a, 448.f);
+            const Fp8Block q = fp8_block(m);   // the cast's codes and scale, bit for bit
+            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.h) + row * p.ldc + col) = fp8_encode8(f, q);
+            if ((t & 15) == 0) p.scale[row * p.s_m + (col >> 7) * p.s_k] = q.scale;
           }
         }
       }
