@@ -1,0 +1,44 @@
+"""cross_sdpa where queries hold NaN or infinities and masks leave little or nothing, on each kernel."""
+import math
+
+import pytest
+import torch
+from test_cross_attention_gpu import _check, _inputs
+
+pytestmark = pytest.mark.gpu
+
+# a few rows over short keys (in one chunk, in several), many rows (in one, in several; 64 and 128 columns)
+SHAPES = [(4, 2, 2, 1, 257, 64), (4, 1, 1, 1, 4000, 64), (4, 1, 1, 2, 500, 128), (4, 2, 2, 40, 300, 64), (4, 2, 1, 150, 515, 80), (4, 1, 1, 9, 5000, 128),
+          (4, 1, 1, 33, 20000, 64), (4, 4, 2, 1, 5000, 128)]
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("B,H,Hkv,Sq,Skv,D", SHAPES)
+def test_a_query_that_keeps_no_key_gives_0_whatever_it_holds(B, H, Hkv, Sq, Skv, D, bad):
+    from vitfp4 import _lib
+    from vitfp4.nvfp4 import cross_sdpa
+    q, k, v = _inputs(B, H, Hkv, Sq, Skv, D, seed=Skv, packed=True)
+    keep = torch.rand(B, Skv, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)) < 0.5
+    keep[0] = False                        # nothing, by the mask
+    keep[1, 130:] = False                  # nothing in later tiles and chunks
+    keep[2, : Skv - 30] = False            # nothing in earlier ones
+    want = cross_sdpa(q, k, v, key_mask=keep)
+    _check(want, q, k, v, keep=keep)
+    junk = q.clone()
+    junk[0] = bad
+    for b in (1, 2):
+        junk[b, 0, Sq // 2, D - 3] = bad   # one query of images that keep some keys
+    o = cross_sdpa(junk, k, v, key_mask=keep)
+    assert (o[0] == 0).all()
+    assert o[1, 0, Sq // 2].isnan().all() and o[2, 0, Sq // 2].isnan().all()
+    for b in (1, 2):
+        o[b, 0, Sq // 2] = want[b, 0, Sq // 2]
+    assert torch.equal(o, want)
+    lens = torch.tensor([0, Skv, 0, 130], dtype=torch.int32, device="cuda")
+    full = torch.ones_like(keep)
+    o = cross_sdpa(torch.full_like(q, bad), k, v, kv_lens=lens, key_mask=full)
+    assert (o[0] == 0).all() and (o[2] == 0).all() and o[1].isnan().all() and o[3].isnan().all()
+    full[1] = False
+    o = cross_sdpa(torch.full_like(q, bad), k, v, kv_lens=lens, key_mask=full)
+    assert (o[:3] == 0).all() and o[3].isnan().all()
+    assert _lib.device_error() == 0

@@ -314,7 +314,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) xattn_join_kernel(const XPara
 //               that none of their NaNs reaches a score or meets a weight of 0, and set the tile's extra column:
 //               S gets one more step of its product, with 1 in every query's column and 0 or -3.4e38 in each
 //               key's, so a dropped key's score is -3.4e38 without a thread of the softmax looking at the mask
-//               (which took it as long as its maximum)
+//               (which took it as long as its maximum).  Whether any key at all is kept they tell the softmax warps
+//               after the last tile: a NaN in the query makes dropped scores NaN, and without a kept key that row is 0
 //   warps 4-7   softmax, a thread per row, which holds the row's 128 scores in registers
 //
 // Bound by the exponentials: 16 per clock and SM on the special-function unit is 1024 clocks per 128 x 128
@@ -332,8 +333,8 @@ struct XCfg {
   static constexpr int V_OFF = 0, K_OFF = NV * TILE, Q_OFF = (NV + NK) * TILE;
   static constexpr int QX_OFF = Q_OFF + TILE, KX_OFF = QX_OFF + EXT;
   static constexpr int BAR_OFF = KX_OFF + NK * EXT;
-  static constexpr int NBAR = 3 * (NK + NV) + 6;
-  static constexpr int SMEM = 1024 + BAR_OFF + 8 * NBAR + 16;
+  static constexpr int NBAR = 3 * (NK + NV) + 7;
+  static constexpr int SMEM = 1024 + BAR_OFF + 8 * NBAR + 16;   // behind the barriers: tensor memory address, `seen`
   // 4 x 16 heads of 1024 x 4096 x 128: 146 us with 3, 152 with 4, 157 with 2; 32 x 16 of 64 x 1025 x 80: 36.4, 38.2 and
   // 36.9; 8 x 16 of 1024 x 4096 x 64: 197 with 4, 200 with 3, 205 without the polynomial
   static constexpr int kPolyEvery = DP == 64 ? 4 : 3;
@@ -398,8 +399,9 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
   auto v_free = [&](int i) { return bar + 8u * (3 * C::NK + C::NV + i); };
   auto v_clean = [&](int i) { return bar + 8u * (3 * C::NK + 2 * C::NV + i); };
   const uint32_t q_full = bar + 8u * (3 * (C::NK + C::NV)), s_full = q_full + 8, s_free = q_full + 16, p_full = q_full + 24,
-                 o_full = q_full + 32, p_half = q_full + 40;
+                 o_full = q_full + 32, p_half = q_full + 40, seen_set = q_full + 48;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + C::BAR_OFF + 8 * C::NBAR);
+  volatile uint32_t* seen = tmem_slot + 1;   // masked: whether any of this CTA's keys is kept; valid after seen_set
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* err = &g_xattn_err;
 
@@ -428,6 +430,7 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
     mbar_init(p_full, 4);
     mbar_init(p_half, 4);
     mbar_init(o_full, 1);
+    mbar_init(seen_set, 1);
     fence_mbar_init();
     tma_prefetch(&tmK);
     tma_prefetch(&tmV);
@@ -556,11 +559,15 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
         for (int i = lane; i < C::NK * 128; i += 32)
           *reinterpret_cast<uint4*>(gb + C::KX_OFF + (i >> 3) * 256 + 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
       kept(0);
+      bool some = false;
       for (int t = 0; t < n; ++t) {
         const int use = is_k ? t / C::NK : t / C::NV, st = is_k ? t % C::NK : t % C::NV;
         bool keep[4];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) keep[w] = next[w];
+        for (int w = 0; w < 4; ++w) {
+          keep[w] = next[w];
+          some = some || keep[w];
+        }
         if (t + 1 < n) kept(t + 1);
         // a tile's arrival also says that the one before it in this place is done with
         if (!__all_sync(0xFFFFFFFFu, mbar_wait(is_k ? k_full(st) : v_full(st), (uint32_t)use & 1u, err, kDevErrTimeoutFull))) break;
@@ -582,6 +589,11 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
         fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(is_k ? k_clean(st) : v_clean(st));
+      }
+      some = __any_sync(0xFFFFFFFFu, some);
+      if (is_k && lane == 0) {
+        *seen = some;
+        mbar_arrive(seen_set);
       }
     }
     __syncwarp();
@@ -724,6 +736,13 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
     // O is complete when its last product is
     if (n > 0 && ok) ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full, (uint32_t)(n - 1) & 1u, err, kDevErrTimeoutTmem));
     tc_fence_after();
+    if (masked && ok) {
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait(seen_set, 0, err, kDevErrTimeoutOther));
+      if (*seen == 0) {   // no key kept: 0, also where the query's NaNs have reached m, l and O
+        m = -INFINITY;
+        l = 0.f;
+      }
+    }
     if (act && ok) {
       const int64_t part_row = ((int64_t)item * p.chunks + chunk) * p.R + row;
       const bool parts = p.chunks > 1;
