@@ -42,3 +42,44 @@ def test_a_query_that_keeps_no_key_gives_0_whatever_it_holds(B, H, Hkv, Sq, Skv,
     o = cross_sdpa(torch.full_like(q, bad), k, v, kv_lens=lens, key_mask=full)
     assert (o[:3] == 0).all() and o[3].isnan().all()
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("B,H,Hkv,Sq,Skv,D", SHAPES)
+def test_kept_scores_of_minus_infinity_are_no_dropped_keys(B, H, Hkv, Sq, Skv, D, masked):
+    """Scores below the lowest finite number: a row of them is NaN, as softmax gives it; beside finite ones they weigh 0.
+    Keys and queries are powers of two, so that every sum is exact or overflows whatever its order."""
+    from vitfp4.nvfp4 import cross_sdpa
+    _, _, v = _inputs(B, H, Hkv, Sq, Skv, D, seed=Skv)
+    q = torch.full((B, H, Sq, D), 2.0 ** 70, device="cuda").bfloat16()
+    k = torch.full((B, Hkv, Skv, D), -(2.0 ** 70), device="cuda").bfloat16()      # scores -2^140 D: -inf
+    keep = torch.ones(B, Skv, dtype=torch.bool, device="cuda")
+    if masked:
+        keep[:, 5::3] = False
+    kw = dict(key_mask=keep) if masked else {}
+    assert cross_sdpa(q, k, v, **kw).isnan().all()
+    k2 = k.clone()
+    for at in (0, Skv - 1):          # one key with a score of 0: its value alone
+        k2[:] = k
+        k2[:, :, at] = 0
+        keep[:, at] = True
+        o = cross_sdpa(q, k2, v, **kw)
+        assert torch.equal(o, v[:, :, at, None].repeat_interleave(H // Hkv, 1).expand(B, H, Sq, D))
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("B,H,Hkv,Sq,Skv,D", SHAPES)
+def test_kept_scores_near_the_lowest_number(B, H, Hkv, Sq, Skv, D, masked):
+    """All scores between -2^127 and -2^126 (times a scale that brings them to -2 .. -1): weights as any others."""
+    from vitfp4.nvfp4 import cross_sdpa
+    _, _, v = _inputs(B, H, Hkv, Sq, Skv, D, seed=Skv)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.zeros(B, H, Sq, D, device="cuda").bfloat16()
+    k = torch.zeros(B, Hkv, Skv, D, device="cuda").bfloat16()
+    q[..., 1] = 2.0 ** 63            # one product per score: no sum to round
+    k[..., 1] = (-(2.0 ** 63) * (1 + torch.rand(B, Hkv, Skv, device="cuda", generator=g) * 0.98)).bfloat16()
+    keep = torch.ones(B, Skv, dtype=torch.bool, device="cuda")
+    if masked:
+        keep[:, 5::3] = False
+    o = cross_sdpa(q, k, v, scale=2.0 ** -126, **(dict(key_mask=keep) if masked else {}))
+    _check(o, q, k, v, scale=2.0 ** -126, keep=keep)

@@ -48,7 +48,8 @@ struct XParams {
   float c;                 // |scale| * log2(e)
   int chunk, chunks;       // keys per CTA and CTAs per row tile; chunks > 1: partial results to the workspace
   float* part_o;           // [B * Hkv][chunks][R][D]
-  float2* part_ml;         // [B * Hkv][chunks][R]: {maximum of the scores, sum of the weights}
+  float2* part_ml;         // [B * Hkv][chunks][R]: {maximum of the scores, sum of the weights}; {-inf, 0}: no key kept,
+                           // {-inf, 1}: keys kept, every score -inf
   int tiles;               // 128-row tiles (tcgen05 kernel)
 };
 
@@ -107,6 +108,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) xattn_rows_kernel(const XParam
   const __nv_bfloat16* kp = p.k + b * p.kb + hk * p.kh + el;
   const __nv_bfloat16* vp = p.v + b * p.vb + hk * p.vh + el;
   const uint8_t* mp = p.mask ? p.mask + b * p.mask_b : nullptr;
+  bool some = false;   // any key kept
   for (int base = w0; base < w1; base += KPW * kU) {
     uint4 kc[kU], vc[kU];
     bool kept[kU];
@@ -114,6 +116,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) xattn_rows_kernel(const XParam
     for (int u = 0; u < kU; ++u) {
       const int j = base + u * KPW + grp;
       kept[u] = j < w1 && (!mp || mp[j] != 0);
+      some = some || kept[u];
       kc[u] = vc[u] = make_uint4(0, 0, 0, 0);
       if (kept[u] && on) {
         kc[u] = __ldg(reinterpret_cast<const uint4*>(kp + (int64_t)j * p.ks));
@@ -195,7 +198,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) xattn_rows_kernel(const XParam
       if (lane == 0) red_ml[warp][r] = make_float2(m[r], l[r]);
     }
   }
-  __syncthreads();
+  const bool seen = __syncthreads_or(some);
   for (int t = threadIdx.x; t < R * LPK; t += blockDim.x) {
     const int r = t / LPK, e = (t - r * LPK) * 8;
     if (r >= p.R || e >= p.D) continue;
@@ -214,6 +217,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) xattn_rows_kernel(const XParam
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = fmaf(red_o[w][r][e + i], f, o[i]);
     }
+    if (seen && ls == 0.f) ls = p.chunks > 1 ? 1.f : __uint_as_float(0x7FFFFFFFu);   // every kept score is -inf
     if (p.chunks > 1) {
       const int64_t row = ((int64_t)item * p.chunks + chunk) * p.R + r;
       float4* dst = reinterpret_cast<float4*>(p.part_o + row * p.D + e);
@@ -246,7 +250,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) xattn_join_kernel(const XPara
   const int n = min(p.chunks, (keys_of(p, b) + p.chunk - 1) / p.chunk);   // chunks that hold keys
   const int64_t at = (int64_t)item * p.chunks * p.R + r;
   float mx = -INFINITY;
-  for (int c = lane; c < n; c += 32) mx = fmaxf(mx, p.part_ml[at + (int64_t)c * p.R].x);
+  bool some = false;
+  for (int c = lane; c < n; c += 32) {
+    const float2 ml = p.part_ml[at + (int64_t)c * p.R];
+    mx = fmaxf(mx, ml.x);
+    some = some || ml.y != 0.f;
+  }
+  some = __any_sync(0xFFFFFFFFu, some);
 #pragma unroll
   for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
   const float ms = mx == -INFINITY ? 0.f : mx;
@@ -290,6 +300,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) xattn_join_kernel(const XPara
       acc.w += o.w;
       ls += red_l[w];
     }
+    if (some && mx == -INFINITY) ls = __uint_as_float(0x7FFFFFFFu);   // keys kept, every score -inf
     const float f = ls > 0.f ? __fdividef(1.f, ls) : (ls == 0.f ? 0.f : ls);
     *reinterpret_cast<uint2*>(p.out + o_offset(p, b, hk, r) + e) =
         make_uint2(bf16x2_round(f32x2_pack(acc.x * f, acc.y * f)), bf16x2_round(f32x2_pack(acc.z * f, acc.w * f)));
@@ -312,8 +323,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) xattn_join_kernel(const XPara
 //   warp 1      TMEM allocation, MMAs
 //   warps 2, 3  masks (with a mask or key counts): clear the dropped rows of each K and V tile in shared memory, so
 //               that none of their NaNs reaches a score or meets a weight of 0, and set the tile's extra column:
-//               S gets one more step of its product, with 1 in every query's column and 0 or -3.4e38 in each
-//               key's, so a dropped key's score is -3.4e38 without a thread of the softmax looking at the mask
+//               S gets one more step of its product, with 1 in every query's column and 0 or -inf in each
+//               key's, so a dropped key's score is -inf without a thread of the softmax looking at the mask
 //               (which took it as long as its maximum).  Whether any key at all is kept they tell the softmax warps
 //               after the last tile: a NaN in the query makes dropped scores NaN, and without a kept key that row is 0
 //   warps 4-7   softmax, a thread per row, which holds the row's 128 scores in registers
@@ -575,9 +586,9 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int j = 32 * w + lane;
-          if (is_k)   // 0xFF7F: -3.39e38, the lowest bf16
+          if (is_k)   // 0xFF80: -inf in bf16
             *reinterpret_cast<uint4*>(gb + C::KX_OFF + st * C::EXT + (j >> 3) * 256 + (j & 7) * 16) =
-                make_uint4(keep[w] ? 0u : 0xFF7Fu, 0, 0, 0);
+                make_uint4(keep[w] ? 0u : 0xFF80u, 0, 0, 0);
           if (!keep[w]) {   // the lane clears its own row, starting at a piece of its own: no bank conflicts
 #pragma unroll
             for (int c = 0; c < C::PANELS; ++c)
@@ -623,7 +634,7 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
       mbar_arrive(q_full);
     }
     float m = -INFINITY, l = 0.f;
-    const float grow = 8.f / p.c;
+    const float grow = fminf(8.f / p.c, 3.4e38f);   // finite: -inf + grow stays -inf
     const unsigned long long c2 = f32x2_pack(p.c, p.c);
     bool ok = true;
     for (int t = 0; t < n && ok; ++t) {
@@ -650,8 +661,7 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
           for (int e = 2; e < 30; e += 2) mx[w] = max3nan(mx[w], __uint_as_float(v[32 * w + e]), __uint_as_float(v[32 * w + e + 1]));
           mx[w] = max3nan(mx[w], mx[w], __uint_as_float(v[32 * w + 30]));
         }
-        float top = max3nan(max3nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-        if (top < -1e38f) top = -INFINITY;   // every key so far is dropped
+        const float top = max3nan(max3nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);   // -inf: no key kept so far
         bool ready = t == 0;                 // the product of the tile before is done: O and P's columns are free
         auto finish_previous = [&]() {
           if (ready) return true;
@@ -736,12 +746,12 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
     // O is complete when its last product is
     if (n > 0 && ok) ok = __all_sync(0xFFFFFFFFu, mbar_wait(o_full, (uint32_t)(n - 1) & 1u, err, kDevErrTimeoutTmem));
     tc_fence_after();
-    if (masked && ok) {
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait(seen_set, 0, err, kDevErrTimeoutOther));
-      if (*seen == 0) {   // no key kept: 0, also where the query's NaNs have reached m, l and O
-        m = -INFINITY;
-        l = 0.f;
-      }
+    if (masked && ok) ok = __all_sync(0xFFFFFFFFu, mbar_wait(seen_set, 0, err, kDevErrTimeoutOther));
+    if (n == 0 || (masked && *seen == 0)) {   // no key kept: 0, also where the query's NaNs have reached m, l and O
+      m = -INFINITY;
+      l = 0.f;
+    } else if (l < 0x1p-64f) {   // keys kept, but no score above -inf (the polynomial's weights of 2^-126 are all there is)
+      l = p.chunks > 1 && m == -INFINITY ? 1.f : __uint_as_float(0x7FFFFFFFu);
     }
     if (act && ok) {
       const int64_t part_row = ((int64_t)item * p.chunks + chunk) * p.R + row;
@@ -919,7 +929,7 @@ int vf4_cross_attn(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const v
   p.R = p.G * p.Sq;
   p.negate = scale < 0.f;
   p.c = (scale < 0.f ? -scale : scale) * 1.4426950408889634f;
-  if (p.c < 1e-30f) p.c = 1e-30f;   // a scale of 0: every finite score weighs 1, and c * -inf stays -inf
+  if (p.c < 1.17549435e-38f) p.c = 1.17549435e-38f;   // a scale of 0: the least normal number, so that c * -inf stays -inf
   p.tiles = (p.R + 127) / 128;
   plan_chunks(B, Hkv, p.R, Skv, num_sms(), &p.chunk, &p.chunks);
   if (p.chunks > 1) {
