@@ -344,7 +344,7 @@ struct XCfg {
   static constexpr int V_OFF = 0, K_OFF = NV * TILE, Q_OFF = (NV + NK) * TILE;
   static constexpr int QX_OFF = Q_OFF + TILE, KX_OFF = QX_OFF + EXT;
   static constexpr int BAR_OFF = KX_OFF + NK * EXT;
-  static constexpr int NBAR = 3 * (NK + NV) + 7;
+  static constexpr int NBAR = 3 * (NK + NV) + 8;
   static constexpr int SMEM = 1024 + BAR_OFF + 8 * NBAR + 16;   // behind the barriers: tensor memory address, `seen`
   // 4 x 16 heads of 1024 x 4096 x 128: 146 us with 3, 152 with 4, 157 with 2; 32 x 16 of 64 x 1025 x 80: 36.4, 38.2 and
   // 36.9; 8 x 16 of 1024 x 4096 x 64: 197 with 4, 200 with 3, 205 without the polynomial
@@ -410,7 +410,8 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
   auto v_free = [&](int i) { return bar + 8u * (3 * C::NK + C::NV + i); };
   auto v_clean = [&](int i) { return bar + 8u * (3 * C::NK + 2 * C::NV + i); };
   const uint32_t q_full = bar + 8u * (3 * (C::NK + C::NV)), s_full = q_full + 8, s_free = q_full + 16, p_full = q_full + 24,
-                 o_full = q_full + 32, p_half = q_full + 40, seen_set = q_full + 48;
+                 o_full = q_full + 32, p_half = q_full + 40, seen_set = q_full + 48,
+                 drain = q_full + 56;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + C::BAR_OFF + 8 * C::NBAR);
   volatile uint32_t* seen = tmem_slot + 1;   // masked: whether any of this CTA's keys is kept; valid after seen_set
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -442,6 +443,7 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
     mbar_init(p_half, 4);
     mbar_init(o_full, 1);
     mbar_init(seen_set, 1);
+    mbar_init(drain, 1);
     fence_mbar_init();
     tma_prefetch(&tmK);
     tma_prefetch(&tmV);
@@ -482,19 +484,19 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
         return load(&tmV, base + C::V_OFF + i * C::TILE, v_full(i), v_free(i), t / C::NV, t, v_hm, v_bm);
       };
       bool ok = true;
-      int kt = 0;
-      while (kt < n && kt < C::NK && ok) ok = load_k(kt++);
-      for (int t = 0; t < n && ok; ++t) {
-        ok = load_v(t);
-        if (kt < n && ok) ok = load_k(kt++);   // K of tile t + NK, free once the scores of tile t are there
+      int kt = 0, vt = 0;   // tiles whose copies have been issued
+      while (kt < n && kt < C::NK && (ok = load_k(kt))) ++kt;
+      while (vt < n && ok) {
+        ok = load_v(vt);
+        if (!ok) break;
+        ++vt;
+        if (kt < n && (ok = load_k(kt))) ++kt;   // K of tile vt - 1 + NK, free once the scores of tile vt - 1 are there
       }
-      // no copy may still be writing shared memory when the CTA exits
-      if (ok) {
-        for (int t = max(0, n - C::NK); t < n; ++t)
-          mbar_wait(k_full(t % C::NK), (uint32_t)(t / C::NK) & 1u, err, kDevErrTimeoutFull);
-        for (int t = max(0, n - C::NV); t < n; ++t)
-          mbar_wait(v_full(t % C::NV), (uint32_t)(t / C::NV) & 1u, err, kDevErrTimeoutFull);
-      }
+      // no copy may still be writing shared memory when the CTA exits, also after a wait that gave up
+      for (int t = max(0, kt - C::NK); t < kt; ++t)
+        mbar_wait(k_full(t % C::NK), (uint32_t)(t / C::NK) & 1u, err, kDevErrTimeoutFull);
+      for (int t = max(0, vt - C::NV); t < vt; ++t)
+        mbar_wait(v_full(t % C::NV), (uint32_t)(t / C::NV) & 1u, err, kDevErrTimeoutFull);
     } else if (warp == 1) {
       const int kd = (p.D + 15) / 16;
       const uint32_t id_s = idesc_bf16(128, false), id_o = idesc_bf16((uint32_t)kd * 16u, true);
@@ -553,8 +555,10 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
         __syncwarp();
         if (!C::kOwnP && t + 1 < n) score(t + 1);
       }
-      // the tensor core must be done with shared memory before the CTA exits
-      if (ok && n > 0) mbar_wait(o_full, (uint32_t)(n - 1) & 1u, err, kDevErrTimeoutDrain);
+      // the tensor core must be done with shared and tensor memory before the CTA exits, also after a wait that gave up
+      if (elected) tc_commit(drain);
+      __syncwarp();
+      mbar_wait(drain, 0, err, kDevErrTimeoutDrain);
     } else if (masked) {
       const bool is_k = warp == 2;   // warp 2: K and its extra column, warp 3: V
       const uint8_t* mp = p.mask ? p.mask + b * p.mask_b : nullptr;
