@@ -35,3 +35,14 @@ def test_cpu_tensors_are_refused():
 def test_arguments_are_checked(args, kw):
     with pytest.raises(_lib.VitFp4Error):
         cross_sdpa(*args, **kw)
+
+
+def test_strides_of_single_entries_do_not_matter():
+    from vitfp4.nvfp4 import ops
+    one = torch.zeros(64, dtype=B16).as_strided((1, 2, 3, 8), (49, 24, 8, 1))       # one image, an odd batch stride
+    assert ops._attn_view(one) is one and ops._attn_strides(one) == (0, 24, 8)
+    head = torch.zeros(64, dtype=B16).as_strided((2, 1, 1, 8), (16, 3, 5, 1))
+    assert ops._attn_view(head) is head and ops._attn_strides(head) == (16, 0, 0)
+    two = torch.zeros(128, dtype=B16).as_strided((2, 2, 3, 8), (49, 24, 8, 1))
+    copy = ops._attn_view(two)
+    assert copy is not two and ops._attn_strides(copy) == (48, 24, 8)

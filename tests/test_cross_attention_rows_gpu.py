@@ -83,3 +83,26 @@ def test_kept_scores_near_the_lowest_number(B, H, Hkv, Sq, Skv, D, masked):
         keep[:, 5::3] = False
     o = cross_sdpa(q, k, v, scale=2.0 ** -126, **(dict(key_mask=keep) if masked else {}))
     _check(o, q, k, v, scale=2.0 ** -126, keep=keep)
+
+
+@pytest.mark.parametrize("Sq,Skv,D", [(1, 40, 64), (1, 1, 64), (30, 200, 64), (1, 6000, 128), (140, 1, 80)])
+def test_strides_of_single_entries_mean_nothing(Sq, Skv, D):
+    """One image, one head, one query or one key with a stride that is no multiple of 8 elements."""
+    from vitfp4.nvfp4 import cross_sdpa, ops
+    for H, Hkv in ((2, 2), (2, 1), (1, 1)):
+        q, k, v = _inputs(1, H, Hkv, Sq, Skv, D, seed=Sq)
+        want = cross_sdpa(q, k, v)
+
+        def odd(t):
+            strides = [s + 1 if n == 1 else s for n, s in zip(t.shape, t.contiguous().stride())]
+            return t.new_zeros(t.numel() + 8).as_strided(t.shape, strides).copy_(t)
+
+        qo, ko, vo = odd(q), odd(k), odd(v)
+        assert qo.stride(0) % 8 and ko.stride(0) % 8
+        assert torch.equal(cross_sdpa(qo, ko, vo), want)
+        ops.probe.timing = True          # the Python path
+        try:
+            assert torch.equal(cross_sdpa(qo, ko, vo), want)
+        finally:
+            ops.probe.timing = False
+            ops.probe.reset()

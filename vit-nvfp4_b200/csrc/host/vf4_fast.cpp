@@ -222,6 +222,9 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// Stride of dimension d; of one with a single entry, whose stride may be anything, 0.
+int64_t step(const at::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
 // cross(q, k, v, kv_lens, key_mask, scale | None) -> out: 4-D bf16 in layouts that the kernels read in place
 PyObject* cross(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -232,7 +235,7 @@ PyObject* cross(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t B = q.size(0), H = q.size(1), Sq = q.size(2), D = q.size(3);
     for (const at::Tensor* t : {&q, &k, &v}) {
       if (t->scalar_type() != at::kBFloat16 || t->dim() != 4 || t->size(0) != B || t->size(3) != D || t->numel() == 0 ||
-          t->stride(3) != 1 || ((t->stride(0) | t->stride(1) | t->stride(2)) & 7) || (t->size(2) > 1 && t->stride(2) < D) ||
+          t->stride(3) != 1 || ((step(*t, 0) | step(*t, 1) | step(*t, 2)) & 7) || (t->size(2) > 1 && t->stride(2) < D) ||
           (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 15))
         return nullptr;
     }
@@ -254,8 +257,8 @@ PyObject* cross(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor out = make({B, H, Sq, D}, {Sq * H * D, D, H * D, 1}, at::kBFloat16, q), work;
     const int64_t need = vf4_cross_attn_workspace_size(B, H, Hkv, Sq, Skv, D);
     if (need) work = make({need}, {1}, at::kByte, q);
-    if (vf4_cross_attn(q.const_data_ptr(), q.stride(0), q.stride(1), q.stride(2), k.const_data_ptr(), k.stride(0), k.stride(1),
-                       k.stride(2), v.const_data_ptr(), v.stride(0), v.stride(1), v.stride(2), B, H, Hkv, Sq, Skv, D,
+    if (vf4_cross_attn(q.const_data_ptr(), step(q, 0), step(q, 1), step(q, 2), k.const_data_ptr(), step(k, 0), step(k, 1),
+                       step(k, 2), v.const_data_ptr(), step(v, 0), step(v, 1), step(v, 2), B, H, Hkv, Sq, Skv, D,
                        (float)scale, static_cast<const int32_t*>(ptr(lens)), static_cast<const uint8_t*>(ptr(mask)),
                        mask.defined() ? mask.stride(0) : 0, out.mutable_data_ptr(), Sq * H * D, D, H * D,
                        need ? work.mutable_data_ptr() : nullptr, need, stream(in.device)))

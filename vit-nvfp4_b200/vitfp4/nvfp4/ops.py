@@ -719,10 +719,16 @@ def attention_packed_qkv(qkv: torch.Tensor, num_heads: int, scale: float, head_g
     return out
 
 
+def _attn_strides(t: torch.Tensor) -> tuple[int, int, int]:
+    """Strides of batch, head and sequence; those of dimensions of one entry, which may be anything, as 0."""
+    (nb, nh, ns, _), (sb, sh, ss, _) = t.shape, t.stride()
+    return sb if nb > 1 else 0, sh if nh > 1 else 0, ss if ns > 1 else 0
+
+
 def _attn_view(t: torch.Tensor) -> torch.Tensor:
     """(B, H, S, D) with the strides the cross attention kernels read in place (copied otherwise)."""
-    sb, sh, ss, sd = t.stride()
-    if sd == 1 and not (sb | sh | ss) & 7 and not t.data_ptr() & 15 and (ss >= t.shape[3] or t.shape[2] <= 1):
+    sb, sh, ss = _attn_strides(t)
+    if t.stride(3) == 1 and not (sb | sh | ss) & 7 and not t.data_ptr() & 15 and (ss >= t.shape[3] or t.shape[2] <= 1):
         return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
 
@@ -743,9 +749,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: fl
         return out
     n = _lib.lib().vf4_cross_attn_workspace_size(B, H, Hkv, Sq, Skv, D)
     ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=q.device) if n else None
-    qb, qh, qs, _ = q.stride()
-    kb, kh, ks, _ = k.stride()
-    vb, vh, vs, _ = v.stride()
+    (qb, qh, qs), (kb, kh, ks), (vb, vh, vs) = _attn_strides(q), _attn_strides(k), _attn_strides(v)
     _call("vf4_cross_attn", "cross_attn", (B * H, Sq, Skv, D), 4.0 * B * H * Sq * Skv * D, q.data_ptr(), qb, qh, qs,
           k.data_ptr() or None, kb, kh, ks, v.data_ptr() or None, vb, vh, vs, B, H, Hkv, Sq, Skv, D, scale,
           None if kv_lens is None else kv_lens.data_ptr(), None if key_mask is None else key_mask.data_ptr(),
