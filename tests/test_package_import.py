@@ -1,0 +1,32 @@
+"""What importing and building the package loads and needs (no GPU)."""
+import os
+import subprocess
+import sys
+
+import pytest
+from conftest import PKG_DIR
+
+
+def _python(code, **env):
+    r = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": PKG_DIR, **env}, stdout=subprocess.PIPE,
+                       stderr=subprocess.STDOUT, text=True)
+    assert r.returncode == 0, r.stdout
+    return r.stdout
+
+
+def test_importing_the_package_loads_no_built_file():
+    """build() imports the package first: what an earlier build left must not be in the process by then."""
+    if not os.path.exists(os.path.join(PKG_DIR, "vitfp4", "_fast.so")):
+        pytest.skip("vitfp4/_fast.so is not built")
+    out = _python("""
+import sys
+import vitfp4
+from vitfp4 import _build, nvfp4
+from vitfp4.nvfp4 import ops
+assert "vitfp4._fast" not in sys.modules
+loaded = lambda: [l for l in open("/proc/self/maps") if "libvitfp4" in l or "_fast.so" in l]
+assert not loaded(), loaded()
+assert ops._fast_module is sys.modules["vitfp4._fast"] and loaded()
+print("fine")
+""")
+    assert "fine" in out

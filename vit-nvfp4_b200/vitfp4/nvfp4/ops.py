@@ -6,6 +6,8 @@ CPU path.
 """
 from __future__ import annotations
 
+import sys
+
 import torch
 
 from .. import _lib
@@ -395,25 +397,35 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor | None, gate: torch.Ten
     return x_out, h, scale
 
 
-try:   # the plain calls in one C++ step; where it is not built they take the functions of this file
-    from .. import _fast as _fast_module
-except ImportError:
-    _fast_module = None
+def __getattr__(name: str):
+    """``_fast_module``: the plain calls in one C++ step (vitfp4._fast); None where it is not built, and the calls take
+    the functions of this file.  Loaded by the first call that asks for it, as the library itself is, so that importing
+    the package, to build both, loads neither."""
+    if name != "_fast_module":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    try:
+        from .. import _fast as module
+    except ImportError:
+        module = None
+    globals()[name] = module
+    return module
 
 
 def _fast(name: str):
     """The C++ form of an op's plain call -> its outputs, or None for any other call, which then goes the Python way
     (also while the probe times calls)."""
-    fn = getattr(_fast_module, name, None)
-    if fn is None:
-        return lambda *a: None
+    fn = launched = None
 
     def call(*a):
+        nonlocal fn, launched
         if probe.timing:
             return None
+        if fn is None:
+            module = sys.modules[__name__]._fast_module
+            fn, launched = getattr(module, name, lambda *a: None), getattr(module, "launched", None)
         r = fn(*a)
         if r is not None:
-            probe.launches += _fast_module.launched()
+            probe.launches += launched()
         return r
     return call
 
