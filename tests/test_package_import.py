@@ -30,3 +30,23 @@ assert ops._fast_module is sys.modules["vitfp4._fast"] and loaded()
 print("fine")
 """)
     assert "fine" in out
+
+
+@pytest.mark.parametrize("missing", ["compiler", "headers", "toolkit"])
+def test_a_module_that_cannot_be_built_is_done_without(missing, tmp_path, monkeypatch):
+    from vitfp4 import _build
+    old = tmp_path / "_fast.so"
+    old.write_bytes(b"")
+    monkeypatch.setattr(_build, "FAST", str(old))
+    if missing == "headers":
+        gxx = tmp_path / "g++"
+        gxx.write_text("#!/bin/sh\necho no headers; exit 1\n")
+        gxx.chmod(0o755)
+    elif missing == "toolkit":
+        def none():
+            raise RuntimeError("nvcc not found")
+        monkeypatch.setattr(_build, "_nvcc", none)
+    monkeypatch.setenv("PATH", str(tmp_path))
+    with pytest.warns(UserWarning, match="Python path"):
+        assert _build.build_fast(force=True) is None
+    assert not old.exists()

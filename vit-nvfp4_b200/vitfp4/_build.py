@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import warnings
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(PKG), "csrc")
@@ -48,27 +49,38 @@ FAST_SRC = os.path.join(CSRC, "host", "vf4_fast.cpp")
 FAST = os.path.join(PKG, "_fast.so")
 
 
-def build_fast(force: bool = False) -> str:
-    """Compile csrc/host/vf4_fast.cpp against torch and libvitfp4.so; returns the module's path."""
-    deps = [FAST_SRC, os.path.join(INCLUDE, "vitfp4.h")]
-    if not force and os.path.exists(FAST) and all(os.path.getmtime(d) <= os.path.getmtime(FAST) for d in deps):
-        return FAST
+def _fast_command(out: str) -> list[str]:
     import sysconfig
 
     import torch
     root = os.path.dirname(torch.__file__)
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *[f for p in inc for f in ("-isystem", p)], "-I", INCLUDE, FAST_SRC, "-o", out,
+            "-L", PKG, "-l:libvitfp4.so", "-Wl,-rpath,$ORIGIN", "-L", os.path.join(root, "lib"),
+            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+
+
+def build_fast(force: bool = False) -> str | None:
+    """Compile csrc/host/vf4_fast.cpp against torch and libvitfp4.so; returns the module's path.  Where that cannot be
+    done (no g++, no headers) it warns and returns None, with no older module left behind: the calls work without."""
+    deps = [FAST_SRC, os.path.join(INCLUDE, "vitfp4.h")]
+    if not force and os.path.exists(FAST) and all(os.path.getmtime(d) <= os.path.getmtime(FAST) for d in deps):
+        return FAST
     tmp = FAST + ".tmp"
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *[f for p in inc for f in ("-isystem", p)], "-I", INCLUDE, FAST_SRC, "-o", tmp,
-           "-L", PKG, "-l:libvitfp4.so", "-Wl,-rpath,$ORIGIN", "-L", os.path.join(root, "lib"),
-           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
-    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if r.returncode:
-        sys.stderr.write(r.stdout)
-        raise RuntimeError("g++ failed for vf4_fast.cpp")
+    try:
+        r = subprocess.run(_fast_command(tmp), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        why = r.stdout if r.returncode else None
+    except (OSError, RuntimeError) as e:   # no g++, no CUDA toolkit
+        why = str(e)
+    if why is not None:
+        if os.path.exists(FAST):
+            os.remove(FAST)
+        warnings.warn(f"vitfp4/_fast.so was not built; plain calls of the small ops take the Python path: {why}",
+                      stacklevel=2)
+        return None
     os.replace(tmp, FAST)
     return FAST
 
