@@ -50,3 +50,23 @@ def test_a_module_that_cannot_be_built_is_done_without(missing, tmp_path, monkey
     with pytest.warns(UserWarning, match="Python path"):
         assert _build.build_fast(force=True) is None
     assert not old.exists()
+
+
+def test_a_module_built_for_another_torch_is_neither_kept_nor_loaded(tmp_path, monkeypatch):
+    import torch
+
+    from vitfp4 import _build
+    if not os.path.exists(_build.FAST):
+        pytest.skip("vitfp4/_fast.so is not built")
+    here = _build.build_fast()
+    stamp = os.stat(here).st_mtime_ns
+    assert _build.build_fast() == here and os.stat(here).st_mtime_ns == stamp      # nothing to do
+    code = "import torch\ntorch.__version__ = '9.9.0'\nfrom vitfp4.nvfp4 import ops\nassert ops._fast_module is None"
+    _python(code)
+    other = tmp_path / "_fast.so"
+    other.write_bytes(open(here, "rb").read())
+    monkeypatch.setattr(_build, "FAST", str(other))
+    monkeypatch.setattr(_build, "_fast_command", lambda out: ["touch", out])       # stands in for the compiler
+    assert _build.build_fast() == str(other) and other.stat().st_size > 0
+    monkeypatch.setattr(torch, "__version__", "9.9.0")
+    assert _build.build_fast() == str(other) and other.stat().st_size == 0         # built anew

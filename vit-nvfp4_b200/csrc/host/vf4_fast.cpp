@@ -282,4 +282,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, null
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__fast(void) { return PyModule_Create(&module); }
+// built_for: torch's release (its C++ interface); the package loads no module that names another.  Nothing of torch is
+// called before that.
+PyMODINIT_FUNC PyInit__fast(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", VF4_BUILT_FOR)) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -49,6 +49,21 @@ FAST_SRC = os.path.join(CSRC, "host", "vf4_fast.cpp")
 FAST = os.path.join(PKG, "_fast.so")
 
 
+def fast_built_for() -> str:
+    """What the module is compiled against, as it names it itself (``built_for``): torch's C++ interface holds for one
+    release.  The module is neither kept nor loaded beside another."""
+    import torch
+    return f"vf4_fast for torch {torch.__version__}, python {sys.version_info[0]}.{sys.version_info[1]}"
+
+
+def _fast_is_current() -> bool:
+    deps = [FAST_SRC, os.path.join(INCLUDE, "vitfp4.h")]
+    if not os.path.exists(FAST) or any(os.path.getmtime(d) > os.path.getmtime(FAST) for d in deps):
+        return False
+    with open(FAST, "rb") as f:
+        return fast_built_for().encode() + b"\0" in f.read()
+
+
 def _fast_command(out: str) -> list[str]:
     import sysconfig
 
@@ -57,7 +72,7 @@ def _fast_command(out: str) -> list[str]:
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DVF4_BUILT_FOR="{fast_built_for()}"',
             *[f for p in inc for f in ("-isystem", p)], "-I", INCLUDE, FAST_SRC, "-o", out,
             "-L", PKG, "-l:libvitfp4.so", "-Wl,-rpath,$ORIGIN", "-L", os.path.join(root, "lib"),
             "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
@@ -66,8 +81,7 @@ def _fast_command(out: str) -> list[str]:
 def build_fast(force: bool = False) -> str | None:
     """Compile csrc/host/vf4_fast.cpp against torch and libvitfp4.so; returns the module's path.  Where that cannot be
     done (no g++, no headers) it warns and returns None, with no older module left behind: the calls work without."""
-    deps = [FAST_SRC, os.path.join(INCLUDE, "vitfp4.h")]
-    if not force and os.path.exists(FAST) and all(os.path.getmtime(d) <= os.path.getmtime(FAST) for d in deps):
+    if not force and _fast_is_current():
         return FAST
     tmp = FAST + ".tmp"
     try:

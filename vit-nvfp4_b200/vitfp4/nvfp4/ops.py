@@ -398,13 +398,15 @@ def gated_residual_norm(x: torch.Tensor, y: torch.Tensor | None, gate: torch.Ten
 
 
 def __getattr__(name: str):
-    """``_fast_module``: the plain calls in one C++ step (vitfp4._fast); None where it is not built, and the calls take
-    the functions of this file.  Loaded by the first call that asks for it, as the library itself is, so that importing
+    """``_fast_module``: the plain calls in one C++ step (vitfp4._fast); None where it is not built (for this torch), and
+    the calls take the functions of this file.  Loaded by the first call that asks for it, as the library itself is, so that importing
     the package, to build both, loads neither."""
     if name != "_fast_module":
         raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
     try:
-        from .. import _fast as module
+        from .. import _build, _fast as module
+        if getattr(module, "built_for", None) != _build.fast_built_for():
+            module = None
     except ImportError:
         module = None
     globals()[name] = module
