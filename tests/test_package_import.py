@@ -70,3 +70,23 @@ def test_a_module_built_for_another_torch_is_neither_kept_nor_loaded(tmp_path, m
     assert _build.build_fast() == str(other) and other.stat().st_size > 0
     monkeypatch.setattr(torch, "__version__", "9.9.0")
     assert _build.build_fast() == str(other) and other.stat().st_size == 0         # built anew
+
+
+def test_the_package_imports_where_torch_has_no_cuda():
+    """A torch built without CUDA lacks the functions that name the current device and stream; the format's helpers need
+    neither."""
+    _python("""
+import torch
+for name in ("_cuda_getCurrentRawStream", "_cuda_getDevice"):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+from vitfp4 import _lib
+from vitfp4.nvfp4 import cross_sdpa, dequantize_fp8_block, quantize_to_fp8_block
+assert dequantize_fp8_block(torch.ones(2, 130).to(torch.float8_e4m3fn), torch.full((2, 2), 3.0)).eq(3).all()
+try:
+    quantize_to_fp8_block(torch.zeros(2, 128))
+except _lib.VitFp4Error as e:
+    assert "CUDA" in str(e)
+else:
+    raise AssertionError
+""")

@@ -240,7 +240,8 @@ def _there(fn, first: torch.Tensor, *args):
 
 
 _entry: dict = {}
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+# (a torch built without CUDA has neither; no call gets this far there)
+_raw_stream, _current_device = (getattr(torch._C, n, None) for n in ("_cuda_getCurrentRawStream", "_cuda_getDevice"))
 _F8, _BF16, _F32, _U8 = torch.float8_e4m3fn, torch.bfloat16, torch.float32, torch.uint8
 _CODES = {torch.bfloat16: _lib.VF4_BF16, torch.float32: _lib.VF4_F32}
 
