@@ -5,12 +5,13 @@
 // calls the C ABI of libvitfp4.so on torch's current stream and returns the outputs -- or returns None, without having
 // done anything, for whatever is not the plain case: then the caller goes the Python path, which copes with it
 // (copies, other devices, the probe, torch.library where gradients are recorded) or says what is wrong.  Plain means:
-// exact tensors on the current CUDA device, no gradients recorded, layouts that the kernels read as they are (more than
+// exact tensors on the current CUDA device, no dispatch mode, no gradients recorded, layouts that the kernels read as they are (more than
 // two dimensions: contiguous).
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -26,7 +27,7 @@ bool plain(PyObject* o) { return THPVariable_CheckExact(o); }
 
 // A call's tensors: unpacked, checked for their device and gradients.
 struct Args {
-  bool ok = true;
+  bool ok = !c10::impl::dispatch_mode_enabled();   // a tracer would not see the call
   const bool grad = at::GradMode::is_enabled();
   int device = -1;
 

@@ -68,6 +68,6 @@ def cross_sdpa(query, key, value, *, kv_lens=None, key_mask=None, scale=None):
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not math.isfinite(scale):
         raise _lib.VitFp4Error(f"scale is not finite: {scale}")
-    if _traced(query, key, value):
+    if _traced(query, key, value, kv_lens, key_mask):
         return cross_attention_op(query, key, value, scale, kv_lens, key_mask)
     return ops.cross_attention(query, key, value, scale, kv_lens, key_mask)

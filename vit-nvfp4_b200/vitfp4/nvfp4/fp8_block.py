@@ -19,6 +19,7 @@ from .. import _lib
 from . import ops
 
 _BLOCK = 128
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def _check_operand(name: str, codes: torch.Tensor, scale: torch.Tensor, block_rows: int) -> None:
@@ -78,15 +79,15 @@ def _(x, w, w_scale, bias):
 
 
 def _traced(*ts: torch.Tensor | None) -> bool:
-    """Whether a call has to go through its torch.library op: under torch.compile, or where gradients are
-    recorded (the op has no backward and says so).  Plain calls skip the dispatcher, which costs more host time
-    than the small kernels run."""
-    if torch.compiler.is_compiling():
+    """Whether a call has to go through its torch.library op: under torch.compile or a dispatch mode (tracers, fake
+    tensors), with tensors of a subclass, or where gradients are recorded (the op has no backward and says so).
+    Plain calls skip the dispatcher, which costs more host time than the small kernels run."""
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack():
         return True
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
-                return True
+    grad = torch.is_grad_enabled()
+    for t in ts:
+        if t is not None and (grad and t.requires_grad or type(t) not in _PLAIN):
+            return True
     return False
 
 
@@ -130,7 +131,7 @@ def fp8_block_gemm(a, a_scale, b, b_scale, *, bias=None, out_dtype=torch.bfloat1
         raise _lib.VitFp4Error(f"a and b differ in K: {tuple(a.shape)} and {tuple(b.shape)}")
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise _lib.VitFp4Error(f"out_dtype is bf16 or fp32, got {out_dtype}")
-    if _traced(a_scale, b_scale, bias):
+    if _traced(a, a_scale, b, b_scale, bias):
         return gemm_fp8_block_op(a, a_scale, b, b_scale, bias, out_dtype == torch.float32)
     return ops.gemm_fp8_block(a, a_scale, b, b_scale, bias, out_dtype)
 
@@ -145,5 +146,5 @@ def fp8_block_linear(x, w, w_scale, *, bias=None):
     if x.shape[-1] != w.shape[1]:
         raise _lib.VitFp4Error(f"x has {x.shape[-1]} columns, the weight {w.shape[1]}")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    y = (linear_fp8_block_op if _traced(x, w_scale, bias) else ops.linear_fp8_block)(x2, w, w_scale, bias)
+    y = (linear_fp8_block_op if _traced(x, w, w_scale, bias) else ops.linear_fp8_block)(x2, w, w_scale, bias)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], w.shape[0])
