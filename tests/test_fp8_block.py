@@ -64,3 +64,15 @@ def test_dequantize_activation_and_weight_blocks():
     w = torch.tensor([[1.0, 2.0], [3.0, 4.0]])
     d = dequantize_fp8_block(codes, w)
     assert d[0, 0] == 2 and d[127, 199] == 4 and d[128, 0] == 6 and d[129, 128] == 8
+
+
+def test_codes_of_more_dimensions_are_checked():
+    a, sa = _op(6, 256, 1)
+    b, sb = _op(130, 256, 128)
+    with pytest.raises(_lib.VitFp4Error, match="CUDA"):                    # taken, as far as there is a GPU
+        fp8_block_gemm(a.view(2, 3, 256), sa.view(2, 3, 2), b, sb)
+    for codes, scale in ((a.view(2, 3, 256), sa), (a.view(2, 3, 256), sa.view(3, 2, 2)), (a.view(2, 3, 256), torch.ones(2, 3, 1)),
+                         (a.view(2, 3, 256), torch.tensor(1.0)), (a[0, 0], sa[0, 0]), (a[:, :0].view(2, 3, 0), sa[:, :0].view(2, 3, 0))):
+        with pytest.raises(_lib.VitFp4Error) as e:
+            fp8_block_gemm(codes, scale, b, sb)
+        assert "CUDA" not in str(e.value)

@@ -121,10 +121,16 @@ def dequantize_fp8_block(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tens
 
 
 def fp8_block_gemm(a, a_scale, b, b_scale, *, bias=None, out_dtype=torch.bfloat16):
-    """A (M, K) x B (N, K) in the FP8 block format -> (M, N) in bf16 or fp32, one rounding of the fp32 sum.
+    """A (..., K) x B (N, K) in the FP8 block format -> (..., N) in bf16 or fp32, one rounding of the fp32 sum.
 
-    ``a_scale`` (M, ceil(K / 128)), ``b_scale`` (ceil(N / 128), ceil(K / 128)), any strides; ``bias`` (N,) bf16 or
+    ``a_scale`` (..., ceil(K / 128)), ``b_scale`` (ceil(N / 128), ceil(K / 128)), any strides; ``bias`` (N,) bf16 or
     fp32.  Codes whose rows do not start on 16-byte boundaries are copied first."""
+    lead = a.shape[:-1]
+    if len(lead) != 1:
+        if a.dim() < 1 or a_scale.dim() < 1 or a_scale.shape[:-1] != lead or not a.shape[-1]:
+            raise _lib.VitFp4Error(f"a: codes (..., K) and scales (..., ceil(K / 128)) needed, got {tuple(a.shape)} and "
+                                   f"{tuple(a_scale.shape)}")
+        a, a_scale = a.reshape(-1, a.shape[-1]), a_scale.reshape(lead.numel(), a_scale.shape[-1])
     _check_operand("a", a, a_scale, 1)
     _check_weight(b, b_scale, bias)
     if a.shape[1] != b.shape[1]:
@@ -132,8 +138,10 @@ def fp8_block_gemm(a, a_scale, b, b_scale, *, bias=None, out_dtype=torch.bfloat1
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise _lib.VitFp4Error(f"out_dtype is bf16 or fp32, got {out_dtype}")
     if _traced(a, a_scale, b, b_scale, bias):
-        return gemm_fp8_block_op(a, a_scale, b, b_scale, bias, out_dtype == torch.float32)
-    return ops.gemm_fp8_block(a, a_scale, b, b_scale, bias, out_dtype)
+        y = gemm_fp8_block_op(a, a_scale, b, b_scale, bias, out_dtype == torch.float32)
+    else:
+        y = ops.gemm_fp8_block(a, a_scale, b, b_scale, bias, out_dtype)
+    return y if len(lead) == 1 else y.view(*lead, b.shape[0])
 
 
 def fp8_block_linear(x, w, w_scale, *, bias=None):
