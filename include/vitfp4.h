@@ -373,8 +373,8 @@ VF4_API int vf4_linear_fp8_block(const void* x, int dtype, int64_t M, int64_t K,
  * m / (M / gate_groups), or NULL; gate, weights and biases all of param_dtype
  * (VF4_F32, or dtype).  All arithmetic in fp32; x'
  * (M, K) is rounded once to dtype and enters N_pre before that rounding.  h: (M, K) in dtype, or (h_fp8) codes
- * in rows of ldc bytes with scales at m * stride_m + (column / 128) * stride_k as vf4_cast_fp8_block writes them,
- * cast from the fp32 values.  y NULL: h = N_pre(x) alone (x_out unused).  pre 0: x' alone.  x_out may be x
+ * in rows of ldc bytes with scales at m * stride_m + (column / 128) * stride_k, bit for bit what vf4_cast_fp8_block writes
+ * for the fp32 values.  y NULL: h = N_pre(x) alone (x_out unused).  pre 0: x' alone.  x_out may be x
  * or y when its rows are contiguous there.  16-byte aligned rows with K % 8 == 0 take vector accesses. */
 VF4_API int vf4_gated_residual_norm(const void* x, int64_t ldx, const void* y, int64_t ldy, int dtype, int64_t M,
                                     int64_t K, const void* gate, int64_t gate_groups, float residual_scale, int post,
@@ -383,15 +383,17 @@ VF4_API int vf4_gated_residual_norm(const void* x, int64_t ldx, const void* y, i
                                     int64_t ldc, float* scale, int64_t stride_m, int64_t stride_k,
                                     vf4_stream_t stream);
 
-/* Cross attention: queries over keys and values of another length (an encoder's states), bf16 operands, exact
- * softmax, fp32 accumulation: attention pooling, resamplers, decoders over a ViT's tokens.  No counterpart in the
- * reference.
+/* Cross attention: queries over keys and values of another length (an encoder's states), bf16 operands, softmax and
+ * accumulation in fp32: attention pooling, resamplers, decoders over a ViT's tokens.  Beyond a few rows over short
+ * keys the weights are rounded to bf16 for their product with the values (not for their sum).  No counterpart in
+ * the reference.
  *   q (B, H, Sq, D), k and v (B, Hkv, Skv, D), out (B, H, Sq, D): element (b, h, s, d) at b * *_b + h * *_h +
  *   s * *_s + d; strides multiples of 8 elements (0 for a broadcast batch or head), 16-byte aligned pointers;
  *   H % Hkv == 0, query head h using key head h / (H / Hkv); D % 8 == 0, D <= 128; any Sq and Skv.
  *   kv_lens: NULL or (B,) int32 device values, keys j >= kv_lens[b] are not used (clamped to 0 .. Skv).
  *   key_mask: NULL or (B, Skv) bytes with rows mask_b apart, 0 = not used.  Unused keys and values may hold
- *   anything (NaN included).  A query whose keys are all unused gives 0.
+ *   anything (NaN included).  A query whose keys are all unused gives 0, whatever it holds; one whose used keys all
+ *   score -inf gives NaN.
  * workspace: vf4_cross_attn_workspace_size bytes (asked with the device current that the call runs on; 0: none
  * needed), 16-byte aligned, used
  * until the call's work is done; calls that may overlap need one each.  Deterministic. */

@@ -11,7 +11,11 @@
 // A row lives in the registers of its threads (8 consecutive columns per thread and step, so that 16 lanes
 // hold a block of 128).  Each thread takes the mean and the squared deviations of its own values, one pass
 // over the threads joins them, all in fp32; x' enters the second norm before it is rounded for storage.
-// Bound by memory for fp32 rows (65792 x 1024: 5.1 TB/s); bf16 rows by their instructions as much (101 us, 5.3 TB/s).
+// Bound by memory for fp32 rows (32896 x 1024: 105 us, 5.1 TB/s); bf16 rows by their instructions as much (65792 x 1024,
+// both norms: 100 us, 5.4 TB/s; without the post-norm 97, without the pre-norm 74, the pre-norm alone 50; to FP8 123, as the
+// codes are the cast's own, whose correctly rounded quotient takes four instructions where a product takes one).
+// Rows that are no multiple of 8 columns or not 16-byte aligned are read and written element by element: 30000 x 1171
+// takes 200 us, 30000 x 1168 73.
 #include "vf4_fp8_block.cuh"
 #include "vf4_host.h"
 
@@ -323,8 +327,11 @@ static void launch_norm(const NormParams& p, int out, cudaStream_t s) {
 
 // Threads per row and steps of 8 columns per thread by the rows' number and length.  Up to 1280 columns a warp
 // takes a row, unless there are so few rows that most SMs would get none or one (257 rows of 1024: 8.6 us with a
-// warp per row, 3.9 with a CTA); then, as for longer rows, a CTA takes a row, of as many threads as the row fills
-// in one or two steps.
+// warp per row, 3.9 with a CTA); then, as for longer rows, a CTA takes a row.  Threads x steps of longer rows, both norms,
+// bf16: up to 2048 columns 256 x 1 (257 rows of 2048: 3.5 us, 3.9 with 128 x 2; but 32896 rows 161 us, 120 with 128 x 2),
+// up to 4096 256 x 2 (16400 rows 127, with 512 x 1 205), up to 5120 320 x 2 (13000 rows 141, with 640 x 1 287), up to 8192
+// 256 x 4 (8200 rows 133, with 512 x 2 220), beyond 512 x 4 (4100 rows of 16384: 155, with 1024 x 2 209): the more threads
+// share a row, the longer its two reductions take beside its loads.
 template <typename T, typename P, bool kVec>
 static void dispatch_norm(const NormParams& p, int out, cudaStream_t s) {
   const bool few = p.M <= 8 * (int64_t)num_sms();

@@ -317,7 +317,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) xattn_join_kernel(const XPara
 // is; beyond, P takes S's place and the next S follows O += P V.
 //
 // The running maximum m is only moved (and O and the sums rescaled) when it grows by more than 2^8: P stays
-// below 256, which bf16 and the fp32 sums hold as well as P <= 1.
+// below 256, which bf16 and the fp32 sums hold as well as P <= 1.  P is rounded to bf16 (half a step, 2^-9 to
+// 2^-8 of each weight): the second product's operands are of one type, and in 32 bits V would have to be
+// converted and the product run at half the rate.  The sums take P unrounded.  The relative error against 64 bits
+// is 0.0023, with the fp32 weights of the kernel above 0.0017, which the output's own rounding makes.
 //
 //   warp 0      TMA of K and V tiles (128-byte swizzle, panels of 64 elements)
 //   warp 1      TMEM allocation, MMAs
@@ -828,9 +831,11 @@ static bool plain_rows(int64_t R, int64_t Skv) {
 static void plan_chunks(int64_t B, int64_t Hkv, int64_t R, int64_t Skv, int sms, int* chunk, int* chunks) {
   const bool plain = plain_rows(R, Skv);
   const int64_t items = B * Hkv * (plain ? 1 : (R + 127) / 128);
-  // plain kernel: 4 CTAs per SM, at least 1024 keys each; tcgen05: as many CTAs as are resident at
-  // once, at least 512 keys each (with key counts that differ, shorter chunks would even the CTAs out, but measured
-  // slower: 4 images of up to 16391 keys, 32 heads over 8 of 128 elements: 45 us, 53 with twice as many)
+  // plain kernel: 4 CTAs per SM, at least 1024 keys each (16 problems of one row over 4000 keys of 64 elements 12.4 us;
+  // with 512 9.8, with 2048 18.8; 128 problems 30.2 with each); tcgen05: as many CTAs as are resident at
+  // once, at least 512 keys each (16 problems of 64 rows over 1025 keys 11.1 us; with 256 10.3, with 1024 13.2; 32 over
+  // 4100 keys of 80 elements 21.0, 21.0 and 22.7).  With key counts that differ, shorter chunks would even the CTAs
+  // out, but measured slower: 4 images of up to 16391 keys, 32 heads over 8 of 128 elements: 45 us, 53 with twice as many
   const int64_t want = plain ? (int64_t)sms * 4 : (int64_t)sms * 2, least = plain ? 1024 : 512;
   int64_t n = want / items;
   if (n > (Skv + least - 1) / least) n = (Skv + least - 1) / least;

@@ -1,8 +1,9 @@
 """Cross attention: queries over an encoder's keys and values of another length.
 
 The attention of pooling heads (one latent query per image), resamplers (tens of latents) and decoders over a
-ViT's tokens, with shared key / value heads, a key count per image and a mask of keys.  bf16 operands, exact
-softmax, fp32 accumulation, on the kernels of vf4_cross_attn.  No counterpart in the reference, whose attention is a
+ViT's tokens, with shared key / value heads, a key count per image and a mask of keys.  bf16 operands, softmax and
+accumulation in fp32, the weights rounded to bf16 for their product with the values (not for their sum, and not for
+up to 4 rows over short keys), on the kernels of vf4_cross_attn.  No counterpart in the reference, whose attention is a
 ViT's self attention (src/vit_nvfp4/nvfp4/attention.py:53-86).  Inference only: the op has no backward pass.
 """
 from __future__ import annotations
@@ -35,7 +36,7 @@ def cross_sdpa(query, key, value, *, kv_lens=None, key_mask=None, scale=None):
     key head h // (H // Hkv)), D a multiple of 8 up to 128; any strides (views of packed projections and expanded
     tensors are read in place).  ``kv_lens`` (B,) int32 or int64: keys from kv_lens[b] on are not used.  ``key_mask``
     (B, Skv) bool: False keys are not used.  Unused keys and values may hold anything; a query without any used key
-    gives 0.  ``scale`` defaults to 1 / sqrt(D).  The result is laid out as (B, Sq, H, D), ready for the output
+    gives 0, whatever it holds.  ``scale`` defaults to 1 / sqrt(D).  The result is laid out as (B, Sq, H, D), ready for the output
     projection."""
     if not torch.compiler.is_compiling():
         out = ops.fast_cross(query, key, value, kv_lens, key_mask, scale)

@@ -52,7 +52,7 @@ def gated_residual_norm(x, y, *, gate=None, residual_scale=1.0, norm="layer", po
     ``norm`` is "layer" or "rms"; ``post_norm`` / ``pre_norm`` False leave that norm out (h is then None without a
     pre-norm).  ``gate`` is (K,), or (G, K) with the rows divided into G equal runs (a gate per image).
     ``out_dtype`` None or x's: h in x's type; ``torch.float8_e4m3fn``: h = (codes, scales) in the FP8 block format
-    that ``fp8_block_gemm`` reads.  ``y`` None: (x, N_pre(x)).  Arithmetic in fp32; x' is rounded once for storage
+    that ``fp8_block_gemm`` reads, those that ``quantize_to_fp8_block`` gives for the fp32 values.  ``y`` None: (x, N_pre(x)).  Arithmetic in fp32; x' is rounded once for storage
     and enters N_pre unrounded."""
     if post_norm and pre_norm and norm in ops.NORM_KINDS and not torch.compiler.is_compiling() and \
             (out_dtype is None or out_dtype == torch.float8_e4m3fn):
