@@ -76,3 +76,12 @@ def test_codes_of_more_dimensions_are_checked():
         with pytest.raises(_lib.VitFp4Error) as e:
             fp8_block_gemm(codes, scale, b, sb)
         assert "CUDA" not in str(e.value)
+
+
+def test_inputs_without_columns_are_refused():
+    w, ws = _op(5, 128, 128)
+    for x in (torch.tensor(1.0), torch.zeros(2, 3, 0), torch.zeros(0)):
+        with pytest.raises(_lib.VitFp4Error):
+            quantize_to_fp8_block(x)
+        with pytest.raises(_lib.VitFp4Error):
+            fp8_block_linear(x, w, ws)

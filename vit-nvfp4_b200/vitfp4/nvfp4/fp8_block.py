@@ -102,7 +102,9 @@ def quantize_to_fp8_block(x: torch.Tensor, block_rows: int = 1):
             return out
     if block_rows not in (1, _BLOCK):
         raise _lib.VitFp4Error(f"block_rows is 1 or {_BLOCK}, got {block_rows}")
-    if x.dim() < 1 or x.dim() != 2 and block_rows != 1:
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise _lib.VitFp4Error(f"at least one column needed, got {tuple(x.shape)}")
+    if x.dim() != 2 and block_rows != 1:
         raise _lib.VitFp4Error(f"a 2-D weight is needed for {_BLOCK} x {_BLOCK} blocks, got {tuple(x.shape)}")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     codes, scale = (cast_fp8_block_op if _traced(x) else ops.cast_fp8_block)(x2, block_rows)
@@ -151,8 +153,8 @@ def fp8_block_linear(x, w, w_scale, *, bias=None):
         if out is not None:
             return out
     _check_weight(w, w_scale, bias)
-    if x.shape[-1] != w.shape[1]:
-        raise _lib.VitFp4Error(f"x has {x.shape[-1]} columns, the weight {w.shape[1]}")
+    if x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise _lib.VitFp4Error(f"x of shape {tuple(x.shape)} and a weight of {w.shape[1]} columns")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     y = (linear_fp8_block_op if _traced(x, w, w_scale, bias) else ops.linear_fp8_block)(x2, w, w_scale, bias)
     return y if x.dim() == 2 else y.reshape(*x.shape[:-1], w.shape[0])
