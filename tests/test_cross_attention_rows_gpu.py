@@ -106,3 +106,30 @@ def test_strides_of_single_entries_mean_nothing(Sq, Skv, D):
         finally:
             ops.probe.timing = False
             ops.probe.reset()
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("power", [4, 10, 17, 22, 40])
+@pytest.mark.parametrize("B,H,Hkv,Sq,Skv,D", SHAPES)
+def test_huge_scores_pick_the_key_of_the_largest(B, H, Hkv, Sq, Skv, D, power, sign):
+    """Scores of 2^(2 power) times whole numbers below 256, exact in fp32 whatever the order: the largest stands at least
+    2^(2 power) above the next one, so its value comes out alone, rounded by nothing."""
+    from vitfp4.nvfp4 import cross_sdpa
+    _, _, v = _inputs(B, H, Hkv, Sq, Skv, D, seed=Skv)
+    g = torch.Generator(device="cuda").manual_seed(power)
+    n = torch.randint(20, 180, (B, Hkv, Skv), device="cuda", generator=g).float()
+    q = torch.zeros(B, H, Sq, D, device="cuda").bfloat16()
+    k = torch.zeros(B, Hkv, Skv, D, device="cuda").bfloat16()
+    q[..., 3] = sign * 2.0 ** power
+    keep = torch.ones(B, Skv, dtype=torch.bool, device="cuda")
+    keep[:, 7::5] = False
+    for at in (0, Skv // 2 // 5 * 5, Skv - 1):
+        m = n.clone()
+        m[:, :, at] = 190.0 if sign > 0 else 10.0
+        k[..., 3] = (m * 2.0 ** power).bfloat16()
+        keep[:, at] = True
+        want = v[:, :, at, None].repeat_interleave(H // Hkv, 1).expand(B, H, Sq, D)
+        for kw in ({}, {"key_mask": keep}):
+            o = cross_sdpa(q, k, v, scale=1.0, **kw)
+            # (the largest weight may be the polynomial's 2^0, off by 2^-20: half a step of bf16 covers it)
+            assert torch.equal(o, want), (at, float((o.float() - want.float()).abs().max()))

@@ -698,7 +698,17 @@ __global__ void __launch_bounds__(XCfg<DP>::THREADS, 2)
             }
           }
         }
-        const float nm = m == -INFINITY ? 0.f : -m * p.c;
+        // c s - c m as one FMA is off by the rounding of c m, the same factor for all of the row's weights and its sum:
+        // harmless up to 2^24, where it is 2^0.5, but beyond 2^31 it leaves the range of the weights.  There m is
+        // taken off first
+        float nm = m == -INFINITY ? 0.f : -m * p.c;
+        const bool far = fabsf(nm) > 0x1p24f;
+        if (__builtin_expect(__any_sync(0xFFFFFFFFu, far), 0)) {
+          const float off = far ? m : 0.f;
+#pragma unroll
+          for (int e = 0; e < 128; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) - off);
+          nm = far ? 0.f : nm;
+        }
         const unsigned long long nm2 = f32x2_pack(nm, nm);
         unsigned long long l2[2] = {0ull, 0ull};
         // P in place of the scores: pair i of the registers becomes word i
